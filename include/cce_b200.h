@@ -51,7 +51,8 @@ enum {
     CCE_ERR_CUDA = -4,       /* a CUDA runtime/driver call failed (see cce_b200_last_cuda_error) */
     CCE_ERR_DEVICE = -5,     /* not an sm_100 device */
     CCE_ERR_KERNEL_WAIT = -6, /* status word non-zero: a kernel abandoned a bounded wait */
-    CCE_ERR_TOO_LARGE = -7,   /* problem needs more scratch than the fixed buffer of cce_b200_lse_forward_static */
+    CCE_ERR_TOO_LARGE = -7,   /* problem needs more scratch than the entry point has: the fixed buffer of
+                                 cce_b200_lse_forward_static, the shared memory of cce_b200_sample */
     CCE_ERR_UNSUPPORTED = -8  /* feature not compiled into this build (wait tracing needs -DCCE_TRACE=1) */
 };
 
@@ -293,6 +294,61 @@ int cce_b200_de_peer_collect_push(float* acc, int64_t acc_rows, int64_t D, void*
 int cce_b200_de_peer_scatter(const void* gathered, int32_t world, int64_t acc_rows, int64_t D, int32_t dtype,
                              const void* rows, int32_t rows_dtype, int64_t n_rows, const int64_t* n_rows_dev,
                              void* d_e, void* stream);
+
+/* ---- The head as it answers: logits of the classifier that the loss above trains, and tokens.
+ * (No counterpart in the reference, which covers the training loss only.)
+ *
+ * out[t][v] = cap(e[t] . c[v] + bias[v] + scale[a] * sum_j lora_b[a][v][j] * (lora_a[a][j] . e[t]))
+ * with a = adapter_ids[t] and cap(x) = softcap * tanh(x / softcap): the projection of every token, with
+ * the low-rank adapter of the token's own request beside the shared classifier.  A token whose id lies
+ * outside [0, n_adapters) has none.  fp32 accumulation; the inner products with lora_a are kept in fp32.
+ * op: dtype, e, c, bias, softcap and strides as above; n_rows = n_total = tokens, valids and
+ * n_rows_dev NULL.  fp32 operands are computed as the three-term bf16 split. */
+#define CCE_B200_MAX_RANK 256
+typedef struct cce_b200_logits_args {
+    cce_b200_operands op;
+    void* out;                /* [n_total][V], dense rows */
+    int32_t out_dtype;        /* CCE_DT_* */
+    int32_t ids_dtype;        /* CCE_IDX_* */
+    const void* lora_a;       /* [n_adapters][rank][D], dense, in op.dtype; NULL (with lora_b, adapter_ids): none */
+    const void* lora_b;       /* [n_adapters][V][rank], dense, in op.dtype */
+    const float* lora_scale;  /* [n_adapters] or NULL (1) */
+    const void* adapter_ids;  /* [n_total] */
+    int64_t n_adapters;
+    int64_t rank;             /* 1 .. CCE_B200_MAX_RANK */
+} cce_b200_logits_args;
+size_t cce_b200_logits_workspace_bytes(const cce_b200_logits_args* a);
+int cce_b200_logits(const cce_b200_logits_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token for every row of logits, drawn with the given uniform number u.
+ *   weights  w_v = exp((l_v - max) / temperature); 0 for NaN, -inf, and weights below 2^-40
+ *   order    l descending, equal logits by the lower index
+ *   kept     the shortest of three prefixes of that order: the first top_k; the first n whose weights
+ *            reach top_p * (sum of the top_k); those with w >= min_p.  The first is always kept.
+ *   token    the first kept v in ascending order whose running sum of weights exceeds u * (sum of the kept)
+ * temperature <= 0 takes the first of the largest logits; a row without a number above -inf gives -1.
+ * logprobs (optional): the logarithm of the token's share of the kept weights; 0 for the largest, -inf for -1.
+ * A setting is an array with one value per row, or (array NULL) the *_all value for every row; top_k <= 0
+ * or >= V, top_p >= 1 and min_p <= 0 switch a filter off.  Sums are exact (64-bit fixed point), so the result
+ * does not depend on the launch.  V is bounded by the shared memory of eight SMs (CCE_ERR_TOO_LARGE above
+ * about 380 000 fp32 or 770 000 16-bit logits).  No workspace. */
+typedef struct cce_b200_sample_args {
+    const void* logits;  /* [B][V], row stride ld elements */
+    int64_t B, V, ld;
+    int32_t dtype;       /* CCE_DT_* */
+    const float* u;      /* [B], in [0, 1) */
+    const float* temperature;
+    const int64_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    double temperature_all;
+    double top_p_all;
+    double min_p_all;
+    int64_t top_k_all;
+    int64_t* tokens;     /* [B] */
+    float* logprobs;     /* [B] or NULL */
+} cce_b200_sample_args;
+int cce_b200_sample(const cce_b200_sample_args* a, void* stream);
 
 /* Synchronises `stream` and returns CCE_OK or CCE_ERR_KERNEL_WAIT; the raw word goes to *word.
  * Without this read an abandoned wait still shows: the log-sum-exp (hence the loss) and dE of that

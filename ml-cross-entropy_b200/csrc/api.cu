@@ -14,6 +14,8 @@
 
 #include "engine.cuh"
 #include "engine_pair.cuh"
+#include "head_logits.cuh"
+#include "sample.cuh"
 #include "small_kernels.cuh"
 
 using namespace cce;
@@ -127,6 +129,12 @@ int device_info(DeviceInfo** out) {
                                       PAIR_SMEM));
         CCE_CUDA(cudaFuncSetAttribute(pair_engine_kernel<MODE_GEMM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       PAIR_SMEM + PEER_STAGE_BYTES));
+        for (const void* k : {(const void*)head_logits_kernel<float>, (const void*)head_logits_kernel<__half>,
+                              (const void*)head_logits_kernel<__nv_bfloat16>})
+            CCE_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, HEAD_SMEM));
+        for (const void* k : {(const void*)sample_kernel<float>, (const void*)sample_kernel<__half>,
+                              (const void*)sample_kernel<__nv_bfloat16>})
+            CCE_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMP_SMEM));
         d.attr_set = true;
     }
     *out = &d;
@@ -619,7 +627,7 @@ const char* cce_b200_strerror(int code) {
         case CCE_ERR_KERNEL_WAIT: return "a kernel abandoned a bounded wait (status word non-zero)";
         case CCE_ERR_UNSUPPORTED: return "not available in this build of the library";
         case CCE_ERR_TOO_LARGE:
-            return "problem needs more scratch than the fixed buffer of cce_b200_lse_forward_static";
+            return "problem does not fit the fixed buffer of cce_b200_lse_forward_static, or the shared memory of cce_b200_sample";
         default: return "unknown error";
     }
 }
@@ -1508,3 +1516,5 @@ int cce_b200_gemm(const void* A, const void* Bm, void* out, int64_t M, int64_t N
 }
 
 }  // extern "C"
+
+#include "api_serving.cuh"

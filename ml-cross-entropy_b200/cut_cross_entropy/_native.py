@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 import torch
@@ -46,6 +46,9 @@ EXPORTS = (
     "cce_b200_de_peer_collect",
     "cce_b200_de_peer_collect_push",
     "cce_b200_de_peer_scatter",
+    "cce_b200_logits_workspace_bytes",
+    "cce_b200_logits",
+    "cce_b200_sample",
     "cce_b200_gemm",
     "cce_b200_read_status",
     "cce_b200_lse_forward_static_status",
@@ -112,6 +115,42 @@ class BackwardArgs(Structure):
         ("de_peer_world", c_int32),
         ("exchange_sms", c_int32),
         ("de_peer_acc", c_void_p * MAX_PEERS),
+    ]
+
+
+class LogitsArgs(Structure):
+    _fields_ = [
+        ("op", Operands),
+        ("out", c_void_p),
+        ("out_dtype", c_int32),
+        ("ids_dtype", c_int32),
+        ("lora_a", c_void_p),
+        ("lora_b", c_void_p),
+        ("lora_scale", c_void_p),
+        ("adapter_ids", c_void_p),
+        ("n_adapters", c_int64),
+        ("rank", c_int64),
+    ]
+
+
+class SampleArgs(Structure):
+    _fields_ = [
+        ("logits", c_void_p),
+        ("B", c_int64),
+        ("V", c_int64),
+        ("ld", c_int64),
+        ("dtype", c_int32),
+        ("u", c_void_p),
+        ("temperature", c_void_p),
+        ("top_k", c_void_p),
+        ("top_p", c_void_p),
+        ("min_p", c_void_p),
+        ("temperature_all", c_double),
+        ("top_p_all", c_double),
+        ("min_p_all", c_double),
+        ("top_k_all", c_int64),
+        ("tokens", c_void_p),
+        ("logprobs", c_void_p),
     ]
 
 
@@ -195,6 +234,12 @@ def lib() -> ctypes.CDLL:
     L.cce_b200_de_peer_scatter.argtypes = [
         c_void_p, c_int32, c_int64, c_int64, c_int32, c_void_p, c_int32, c_int64, c_void_p, c_void_p, c_void_p,
     ]  # fmt: skip
+    L.cce_b200_logits_workspace_bytes.restype = c_size_t
+    L.cce_b200_logits_workspace_bytes.argtypes = [POINTER(LogitsArgs)]
+    L.cce_b200_logits.restype = c_int32
+    L.cce_b200_logits.argtypes = [POINTER(LogitsArgs), c_void_p, c_size_t, c_void_p]
+    L.cce_b200_sample.restype = c_int32
+    L.cce_b200_sample.argtypes = [POINTER(SampleArgs), c_void_p]
     L.cce_b200_gemm.restype = c_int32
     L.cce_b200_gemm.argtypes = [
         c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,

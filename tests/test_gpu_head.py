@@ -1,0 +1,450 @@
+"""Head operators on the GPU against the float64 oracle: logits with adapters, sampling, and both together."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from cut_cross_entropy import _native, linear_logits, linear_sample, sample_tokens
+from oracle import head_oracle as H
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+# ------------------------------------------------------------------ logits
+
+
+def _tolerance(ref, mag, dtype, out_dtype, K, softcap):
+    """Rounding of the result (half a step of out_dtype), fp32 accumulation of K products in any order with
+    truncation (a whole step 2^-23 each), the two-step adapter product's (within the same K), for fp32 operands the
+    split's dropped terms (2^-15 of every product), and the soft-cap's tanh (4 steps of 1)."""
+    tol = torch.finfo(out_dtype).eps / 2 * ref.abs() + K * 2.0**-23 * mag
+    if dtype == FP32:
+        tol = tol + 2.0**-15 * mag
+    if softcap is not None:
+        tol = tol + softcap * 2.0**-21
+    return tol * 1.01 + torch.finfo(out_dtype).smallest_normal
+
+
+def _inputs(T, V, D, dtype, n=0, r=0, bias=None, seed=0, layout="each"):
+    g = torch.Generator().manual_seed(seed)
+    kw = dict(e=torch.randn(T, D, generator=g).to(dtype), c=(torch.randn(V, D, generator=g) * 2 / D**0.5).to(dtype))
+    if bias is not None:
+        kw["bias"] = (torch.randn(V, generator=g) * 0.3).to(bias)
+    if n:
+        kw["lora_a"] = (torch.randn(n, r, D, generator=g) / D**0.5).to(dtype)
+        kw["lora_b"] = torch.randn(n, V, r, generator=g).to(dtype)
+        kw["lora_scale"] = torch.rand(n, generator=g) + 0.5
+        ids = torch.randint(-1, n, (T,), generator=g)
+        kw["adapter_ids"] = ids.sort().values if layout == "runs" else ids
+    return kw
+
+
+def _to_dev(kw):
+    return {k: v.to(DEV) if isinstance(v, torch.Tensor) else v for k, v in kw.items()}
+
+
+def _check_logits(kw, out_dtype=None, softcap=None):
+    ref, mag = H.linear_logits(**kw, softcap=softcap)
+    got = linear_logits(**_to_dev(kw), softcap=softcap, out_dtype=out_dtype)
+    dtype = kw["e"].dtype
+    out_dtype = out_dtype or dtype
+    assert got.dtype == out_dtype and got.shape == ref.shape
+    K = kw["e"].size(-1) + (kw["lora_a"].size(1) if "lora_a" in kw else 0) + 8
+    err = (got.cpu().double() - ref).abs()
+    assert bool((err <= _tolerance(ref, mag, dtype, out_dtype, K, softcap)).all()), err.max()
+    return got
+
+
+@pytest.mark.parametrize("T", [1, 2, 16, 17, 31, 33, 64, 100, 255, 256, 257, 300, 520])
+def test_logits_token_counts(T):
+    _check_logits(_inputs(T, 384, 192, BF16, n=3, r=16, seed=T), out_dtype=FP32)
+
+
+@pytest.mark.parametrize("V", [1, 7, 127, 128, 129, 1000, 19077])
+@pytest.mark.parametrize("D", [1, 8, 63, 64, 200, 1001])
+def test_logits_sizes(V, D):
+    _check_logits(_inputs(5, V, D, BF16, n=2, r=8, bias=FP32, seed=V + D))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("out_dtype", [None, BF16, FP16, FP32])
+@pytest.mark.parametrize("bias", [None, BF16, FP16, FP32])
+def test_logits_types(dtype, out_dtype, bias):
+    _check_logits(_inputs(37, 300, 136, dtype, n=2, r=12, bias=bias), out_dtype=out_dtype, softcap=5.0)
+
+
+@pytest.mark.parametrize("r", [1, 3, 4, 8, 15, 16, 17, 24, 32, 64, 100, 256])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_logits_ranks(r, dtype):
+    _check_logits(_inputs(40, 260, 128, dtype, n=4, r=r, seed=r), out_dtype=FP32)
+
+
+@pytest.mark.parametrize("n", [1, 2, 50, 300])
+@pytest.mark.parametrize("layout", ["each", "runs"])
+@pytest.mark.parametrize("T", [3, 290])
+def test_logits_adapter_mixes(n, layout, T):
+    _check_logits(_inputs(T, 200, 64, BF16, n=n, r=16, layout=layout, seed=n), out_dtype=FP32)
+
+
+def test_logits_without_adapters_and_with_none_chosen():
+    kw = _inputs(20, 500, 128, BF16, n=3, r=16)
+    kw["adapter_ids"].fill_(-1)
+    with_none = linear_logits(**_to_dev(kw), out_dtype=FP32)
+    for k in ("lora_a", "lora_b", "lora_scale", "adapter_ids"):
+        del kw[k]
+    assert torch.equal(with_none, _check_logits(kw, out_dtype=FP32))
+
+
+@pytest.mark.parametrize("ids_dtype", [torch.int32, torch.int64])
+def test_logits_ids_outside_the_adapters_mean_none(ids_dtype):
+    kw = _inputs(8, 300, 64, BF16, n=2, r=8)
+    kw["adapter_ids"] = torch.tensor([0, 1, 2, 100, -1, -7, 2**31 - 1, 1]).to(ids_dtype)
+    _check_logits(kw, out_dtype=FP32)
+
+
+def test_logits_scale_forms():
+    kw = _inputs(8, 300, 64, BF16, n=2, r=8)
+    kw["lora_scale"] = torch.full((2,), 0.75)
+    want = linear_logits(**_to_dev(kw), out_dtype=FP32)
+    assert torch.equal(linear_logits(**_to_dev(dict(kw, lora_scale=0.75)), out_dtype=FP32), want)
+    kw["lora_scale"] = None
+    _check_logits(kw, out_dtype=FP32)
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_logits_a_broken_adapter_stays_with_its_own_requests(bad):
+    kw = _inputs(48, 300, 128, BF16, n=3, r=16)
+    kw["adapter_ids"] = torch.arange(48) % 4 - 1
+    good = linear_logits(**_to_dev(kw), out_dtype=FP32)
+    kw["lora_a"][1] = bad
+    kw["lora_b"][1] = bad
+    got = linear_logits(**_to_dev(kw), out_dtype=FP32)
+    others = (kw["adapter_ids"] != 1).to(DEV)
+    assert torch.equal(got[others], good[others])
+    assert not torch.isfinite(got[~others]).any()
+
+
+def test_logits_strides_and_shapes():
+    kw = _inputs(24, 300, 128, BF16, n=2, r=16, bias=BF16)
+    want = linear_logits(**_to_dev(kw), out_dtype=FP32)
+    d = _to_dev(kw)
+    pad = lambda x, by: torch.cat([x, torch.full((*x.shape[:-1], by), math.nan, dtype=x.dtype, device=DEV)], -1)
+    for name, by in (("e", 8), ("e", 3), ("c", 16), ("c", 1), ("lora_a", 5), ("lora_b", 1)):
+        view = pad(d[name], by)[..., : d[name].size(-1)]
+        assert torch.equal(linear_logits(**dict(d, **{name: view}), out_dtype=FP32), want), (name, by)
+    for name in ("e", "c", "lora_a", "lora_b"):  # bases off a 16-byte boundary, and transposed storage
+        x = d[name]
+        off = torch.empty(x.numel() + 1, dtype=x.dtype, device=DEV)[1:].view(x.shape).copy_(x)
+        assert torch.equal(linear_logits(**dict(d, **{name: off}), out_dtype=FP32), want), name
+        tr = x.transpose(-1, -2).contiguous().transpose(-1, -2)
+        assert torch.equal(linear_logits(**dict(d, **{name: tr}), out_dtype=FP32), want), name
+    shaped = dict(d, e=d["e"].view(2, 3, 4, 128), adapter_ids=d["adapter_ids"].view(2, 3, 4))
+    assert torch.equal(linear_logits(**shaped, out_dtype=FP32), want.view(2, 3, 4, 300))
+    one = dict(d, e=d["e"][5], adapter_ids=d["adapter_ids"][5])
+    assert torch.equal(linear_logits(**one, out_dtype=FP32), want[5])
+    same = dict(d, e=d["e"][:1].expand(24, 128))
+    assert torch.equal(linear_logits(**same, out_dtype=FP32)[0], want[0])
+
+
+def test_logits_empty():
+    kw = _to_dev(_inputs(0, 300, 64, BF16, n=2, r=8))
+    assert linear_logits(**kw).shape == (0, 300)
+    kw = _to_dev(_inputs(4, 0, 64, BF16))
+    assert linear_logits(**kw).shape == (4, 0)
+
+
+def test_logits_refusals_on_the_device():
+    kw = _to_dev(_inputs(4, 300, 64, BF16, n=2, r=8))
+    with pytest.raises(ValueError):
+        linear_logits(**dict(kw, c=kw["c"].half()))
+    with pytest.raises(ValueError):
+        linear_logits(**dict(kw, lora_a=kw["lora_a"].float()))
+    with pytest.raises(ValueError):
+        linear_logits(**dict(kw, adapter_ids=kw["adapter_ids"].cpu()))
+    with pytest.raises(NotImplementedError):
+        linear_logits(kw["e"].double(), kw["c"].double())
+    with pytest.raises(NotImplementedError):
+        linear_logits(kw["e"], kw["c"], out_dtype=torch.float64)
+
+
+def test_logits_parameters_need_no_grad_and_autocast_casts():
+    kw = _to_dev(_inputs(4, 300, 64, FP32))
+    c = torch.nn.Parameter(kw["c"])
+    with pytest.raises(RuntimeError):
+        linear_logits(kw["e"], c)
+    with torch.no_grad(), torch.autocast("cuda", dtype=BF16):
+        got = linear_logits(kw["e"], c)
+    assert torch.equal(got, linear_logits(kw["e"].bfloat16(), kw["c"].bfloat16()))
+
+
+def test_logits_do_not_depend_on_the_batch_mates():
+    """A token's logits are the same bits alone and in a batch of any size (one order of the sums)."""
+    kw = _to_dev(_inputs(300, 500, 320, BF16, n=3, r=24))
+    full = linear_logits(**kw, out_dtype=FP32)
+    for t in (0, 17, 255, 256, 299):
+        one = dict(kw, e=kw["e"][t : t + 1], adapter_ids=kw["adapter_ids"][t : t + 1])
+        assert torch.equal(linear_logits(**one, out_dtype=FP32)[0], full[t])
+
+
+def test_logits_output_past_two_to_the_31():
+    """16384 x 140000 16-bit logits: offsets pass 2^31 elements."""
+    kw = _to_dev(_inputs(16384, 140000, 64, BF16))
+    got = linear_logits(**kw)
+    rows = torch.tensor([0, 8191, 15338, 15339, 16383], device=DEV)
+    ref, mag = H.linear_logits(kw["e"][rows].cpu(), kw["c"].cpu())
+    err = (got[rows].cpu().double() - ref).abs()
+    assert bool((err <= _tolerance(ref, mag, BF16, BF16, 64, None)).all())
+
+
+# ---------------------------------------------------------------- sampling
+
+
+def _check_sample(logits, u, **kw):
+    ref_tok, ref_lp = H.sample_tokens(logits.cpu(), u.cpu(), **{k: v.cpu() if torch.is_tensor(v) else v for k, v in kw.items()})
+    tok, lp = sample_tokens(logits, u, return_logprobs=True, **kw)
+    assert tok.dtype == torch.int64 and lp.dtype == FP32
+    assert torch.equal(tok.cpu(), ref_tok), (tok.cpu() != ref_tok).nonzero().flatten().tolist()[:8]
+    lp = lp.cpu().double()
+    none = torch.isinf(ref_lp)
+    assert torch.equal(torch.isinf(lp), none)
+    # rounding to fp32 (half a step), and weights rounded to 2^-43 of the largest in a sum of at least one
+    tol = 2.0**-24 * ref_lp.abs() * 1.01 + 2.0**-43 * logits.size(-1) + 1e-12
+    assert bool(((lp - ref_lp).abs()[~none] <= tol[~none]).all())
+    assert torch.equal(sample_tokens(logits, u, **kw), tok)
+    return tok
+
+
+def _rows(B, V, dtype, seed=0, peak=10.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(B, V, generator=g) * 2.5
+    x[torch.arange(B)[:, None], torch.randint(0, V, (B, min(V, 20)), generator=g)] += peak * torch.rand(B, min(V, 20), generator=g)
+    return x.to(dtype).to(DEV), torch.rand(B, generator=g).to(DEV)
+
+
+SETTINGS = {
+    "plain": dict(),
+    "cool": dict(temperature=0.3),
+    "hot": dict(temperature=3.0),
+    "k1": dict(top_k=1),
+    "k50": dict(top_k=50),
+    "k3000": dict(top_k=3000, temperature=2.0),
+    "p": dict(top_p=0.9),
+    "p_small": dict(top_p=0.05),
+    "p_near_1": dict(top_p=0.9999, temperature=1.5),
+    "min_p": dict(min_p=0.02),
+    "min_p_1": dict(min_p=1.0),
+    "all": dict(temperature=0.8, top_k=200, top_p=0.95, min_p=0.001),
+    "greedy": dict(temperature=0.0, top_k=40, top_p=0.5),
+}
+
+
+@pytest.mark.parametrize("V", [1, 2, 7, 32, 511, 512, 513, 4095, 8193, 20000, 70001, 150000])
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+def test_sample_sizes(V, dtype):
+    x, u = _rows(12, V, dtype, seed=V)
+    for kw in SETTINGS.values():
+        _check_sample(x, u, **kw)
+
+
+@pytest.mark.parametrize("name", list(SETTINGS))
+def test_sample_flat_and_tied(name):
+    """Near-uniform rows (thousands of tokens of almost equal weight) and rows with few distinct values."""
+    kw = SETTINGS[name]
+    g = torch.Generator().manual_seed(3)
+    u = torch.rand(16, generator=g).to(DEV)
+    _check_sample((torch.randn(16, 30000, generator=g) * 0.01).to(DEV), u, **kw)
+    _check_sample((torch.randn(16, 30000, generator=g) * 1e-7 + 5).to(DEV), u, **kw)
+    _check_sample(torch.randint(-2, 3, (16, 30000), generator=g).float().to(DEV), u, **kw)
+    _check_sample(torch.zeros(16, 30000, device=DEV), u, **kw)
+    signed_zeros = torch.where(torch.rand(16, 5000, generator=g) < 0.5, -0.0, 0.0).to(DEV)
+    _check_sample(signed_zeros, u, **kw)
+
+
+@pytest.mark.parametrize("name", list(SETTINGS))
+def test_sample_masked_and_extreme_rows(name):
+    kw = SETTINGS[name]
+    V = 9000
+    g = torch.Generator().manual_seed(5)
+    low = torch.finfo(FP32).min
+    x = torch.randn(16, V, generator=g) * 3
+    x[0] = -math.inf
+    x[1] = math.nan
+    x[2] = low
+    x[3] = -math.inf
+    x[3, 8999] = -5.0
+    x[4, torch.rand(V, generator=g) < 0.99] = -math.inf
+    x[5, torch.rand(V, generator=g) < 0.99] = low
+    x[6, torch.rand(V, generator=g) < 0.5] = math.nan
+    x[7, ::1000] = math.inf
+    x[8, 4321] = math.inf
+    x[9] = torch.finfo(FP32).max
+    x[9, ::2] = low
+    x[10] *= 1e30
+    x[11] *= 1e-30
+    x[12] = torch.linspace(-45, 0, V)
+    x[13] = 1e4 + torch.randn(V, generator=g)
+    x[14] = torch.tensor([0.0, -30.0, math.nan]).repeat(V // 3)
+    x[15, 1:] = -math.inf
+    u = torch.rand(16, generator=g).to(DEV)
+    _check_sample(x.to(DEV), u, **kw)
+    tok = sample_tokens(x.to(DEV), u, **kw).cpu()
+    assert tok[0] == -1 and tok[1] == -1 and tok[2] >= 0 and tok[3] == 8999 and tok[8] == 4321 and tok[15] == 0
+
+
+def test_sample_border_numbers():
+    x, _ = _rows(6, 5000, FP32)
+    below_one = 1.0 - 2.0**-24
+    for u in (0.0, below_one, 0.5, 2.0**-24):
+        for kw in SETTINGS.values():
+            _check_sample(x, torch.full((6,), u, device=DEV), **kw)
+    # outside the documented range: the last kept token, and the first
+    last = sample_tokens(x, torch.full((6,), below_one, device=DEV), top_k=3)
+    for u in (1.0, 2.0, math.inf):
+        assert torch.equal(sample_tokens(x, torch.full((6,), u, device=DEV), top_k=3), last)
+    first = sample_tokens(x, torch.zeros(6, device=DEV), top_k=3)
+    for u in (-1.0, math.nan):
+        assert torch.equal(sample_tokens(x, torch.full((6,), u, device=DEV), top_k=3), first)
+
+
+@pytest.mark.parametrize("T", [1e-30, 1e-3, 1e4, 1e30, math.inf])
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=77), dict(top_p=0.7), dict(top_k=999, top_p=0.3, min_p=0.5)])
+def test_sample_extreme_temperatures(T, kw):
+    x, u = _rows(4, 12345, FP32, seed=9)
+    x[2, ::3] = -math.inf
+    x[3, ::3] = torch.finfo(FP32).min
+    _check_sample(x, u, temperature=T, **kw)
+
+
+def test_sample_every_row_has_its_own_settings():
+    B, V = 64, 33333
+    x, u = _rows(B, V, BF16, seed=11)
+    g = torch.Generator().manual_seed(12)
+    r = lambda: torch.rand(B, generator=g).to(DEV)
+    kw = dict(
+        temperature=torch.where(r() < 0.2, 0.0, 0.2 + 2 * r()),
+        top_k=(r() ** 4 * 2 * V).long(),
+        top_p=torch.where(r() < 0.3, 1.0, r()),
+        min_p=torch.where(r() < 0.3, 0.0, 0.3 * r()),
+    )
+    tok = _check_sample(x, u, **kw)
+    # a row alone gives the same token, and so do numbers in place of tensors
+    for i in (0, 13, 63):
+        one = {k: v[i : i + 1] for k, v in kw.items()}
+        assert sample_tokens(x[i : i + 1], u[i : i + 1], **one).item() == tok[i].item()
+        assert sample_tokens(x[i], u[i], **{k: v[i].item() for k, v in kw.items()}).item() == tok[i].item()
+    assert torch.equal(sample_tokens(x, u, **dict(kw, top_k=kw["top_k"].int(), top_p=kw["top_p"].double())), tok)
+    shaped = sample_tokens(x.view(4, 16, V), u.view(4, 16), **{k: v.view(4, 16) for k, v in kw.items()})
+    assert torch.equal(shaped, tok.view(4, 16))
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+def test_sample_strides_and_alignment(dtype):
+    x, u = _rows(9, 20001, dtype, seed=2)
+    kw = dict(top_k=300, top_p=0.9)
+    want = sample_tokens(x, u, **kw)
+    for off in range(1, 9):
+        wide = torch.full((9, 20001 + 16), math.inf, dtype=dtype, device=DEV)  # must not be read as logits
+        wide[:, off : off + 20001] = x
+        assert torch.equal(sample_tokens(wide[:, off : off + 20001], u, **kw), want), off
+    assert torch.equal(sample_tokens(x.t().contiguous().t(), u, **kw), want)
+    assert torch.equal(sample_tokens(x[:1].expand(9, -1), u, **kw)[:1], want[:1])
+    assert torch.equal(sample_tokens(x[::2], u[::2], **kw), want[::2])
+
+
+def test_sample_empty_and_too_large():
+    assert sample_tokens(torch.zeros(0, 10, device=DEV), torch.zeros(0, device=DEV)).shape == (0,)
+    with pytest.raises(_native.NativeError):
+        sample_tokens(torch.zeros(1, 500_000, device=DEV), torch.zeros(1, device=DEV))
+    x, u = _rows(2, 500_000, BF16)
+    _check_sample(x, u, top_k=20, top_p=0.9)
+    x, u = _rows(2, 380_000, FP32)
+    _check_sample(x, u, top_p=0.99)
+
+
+def test_sample_frequencies_follow_the_weights():
+    """Evenly spread numbers u give every token its share, up to one draw."""
+    N = 4096
+    x, _ = _rows(1, 50, FP32, seed=4, peak=2.0)
+    u = (torch.arange(N, device=DEV) + 0.5) / N
+    tok = sample_tokens(x.expand(N, -1).contiguous(), u.float(), temperature=2.0)
+    share = torch.softmax(x[0].double() / 2, 0) * N
+    assert bool(((torch.bincount(tok, minlength=50) - share).abs() <= 1.0 + 1e-6).all())
+
+
+# ---------------------------------------------------------------- together
+
+
+def _step_inputs(T=21, V=5003, D=320):
+    kw = _inputs(T, V, D, BF16, n=3, r=16, bias=FP32)
+    kw["e"] = kw["e"] * 3
+    return _to_dev(kw), torch.rand(T, generator=torch.Generator().manual_seed(1)).to(DEV)
+
+
+def test_linear_sample_is_the_two_operators():
+    kw, u = _step_inputs()
+    s = dict(temperature=0.9, top_k=100, top_p=0.95)
+    tok, lp = linear_sample(**kw, u=u, softcap=30.0, return_logprobs=True, **s)
+    logits = linear_logits(**kw, softcap=30.0, out_dtype=FP32)
+    assert torch.equal(tok, _check_sample(logits, u, **s))
+    assert torch.equal(linear_sample(**kw, u=u, softcap=30.0, **s), tok)
+    assert bool((lp <= 0).all())
+
+
+def test_linear_sample_on_another_stream():
+    kw, u = _step_inputs()
+    want = linear_sample(**kw, u=u, top_p=0.9)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = linear_sample(**kw, u=u, top_p=0.9)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+def test_decoding_steps_captured_and_replayed():
+    """Two captured steps with their own workspaces, replayed on new embeddings, adapters and numbers."""
+    kw, u = _step_inputs()
+    temp = torch.full((21,), 0.7, device=DEV)
+    k = torch.full((21,), 40, device=DEV)
+    step = lambda: linear_sample(**kw, u=u, temperature=temp, top_k=k, return_logprobs=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    outs = []
+    for gr in graphs:
+        with torch.cuda.graph(gr):
+            outs.append(step())
+    g = torch.Generator().manual_seed(8)
+    for i in range(4):
+        kw["e"].copy_(torch.randn(21, 320, generator=g) * 3)
+        kw["adapter_ids"].copy_(torch.randint(-1, 3, (21,), generator=g))
+        u.copy_(torch.rand(21, generator=g))
+        temp.copy_(torch.rand(21, generator=g))
+        k.copy_(torch.randint(0, 100, (21,), generator=g))
+        graphs[i % 2].replay()
+        want = step()
+        for a, b in zip(outs[i % 2], want):
+            assert torch.equal(a, b)
+
+
+def test_training_and_answering_share_the_head():
+    """The loss's own numbers from the logits: lse and the correct-token logit agree with linear_cross_entropy."""
+    from cut_cross_entropy import linear_cross_entropy
+
+    kw = _to_dev(_inputs(64, 3001, 256, BF16, bias=FP32))
+    targets = torch.randint(0, 3001, (64,), device=DEV)
+    loss, lse = linear_cross_entropy(**kw, targets=targets, softcap=20.0, reduction="none", return_lse=True)
+    x = linear_logits(**kw, softcap=20.0, out_dtype=FP32).double()
+    # both sum 256 bf16 products in fp32: K 2^-23 of the products' magnitude each, ex2 and lg2 within 2^-20
+    tol = 2 * 264 * 2.0**-23 * H.linear_logits(**{k: v.cpu() for k, v in kw.items()})[1].max().item() + 2.0**-18
+    assert (torch.logsumexp(x, 1) - lse).abs().max().item() <= tol
+    nll = torch.logsumexp(x, 1) - x.gather(1, targets[:, None]).squeeze(1)
+    assert (nll - loss).abs().max().item() <= 2 * tol

@@ -1,0 +1,175 @@
+"""Head operators without a GPU: refusals, argument checks of the C entry points, the oracle's known answers."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from cut_cross_entropy import _native, linear_logits, linear_sample, sample_tokens
+from oracle import head_oracle as H
+
+
+def _lora(n=2, r=8, D=16, V=10, T=4):
+    return dict(lora_a=torch.zeros(n, r, D), lora_b=torch.zeros(n, V, r), adapter_ids=torch.zeros(T, dtype=torch.int64))
+
+
+@pytest.mark.parametrize(
+    "kw, err",
+    [
+        (dict(e=torch.zeros(4, 15)), ValueError),
+        (dict(c=torch.zeros(10, 16, 1)), ValueError),
+        (dict(bias=torch.zeros(9)), ValueError),
+        (dict(softcap=0.0), ValueError),
+        (dict(softcap=-1.0), ValueError),
+        (dict(lora_scale=1.0), ValueError),
+        (dict(_lora(), lora_b=None), ValueError),
+        (dict(_lora(), adapter_ids=None), ValueError),
+        (dict(_lora(r=257)), ValueError),
+        (dict(_lora(n=0)), ValueError),
+        (dict(_lora(D=8)), ValueError),
+        (dict(_lora(V=11)), ValueError),
+        (dict(_lora(T=5)), ValueError),
+        (dict(_lora(), adapter_ids=torch.zeros(4)), ValueError),
+        (dict(_lora(), lora_scale=torch.ones(3)), ValueError),
+        (dict(e=torch.zeros(4, 16, requires_grad=True)), RuntimeError),
+        (dict(), RuntimeError),  # host tensors
+    ],
+)
+def test_linear_logits_refusals(kw, err):
+    args = dict(e=torch.zeros(4, 16), c=torch.zeros(10, 16))
+    args.update(kw)
+    with pytest.raises(err):
+        linear_logits(**args)
+
+
+@pytest.mark.parametrize(
+    "kw, err",
+    [
+        (dict(u=torch.zeros(3)), ValueError),
+        (dict(u=torch.zeros(4, dtype=torch.int64)), ValueError),
+        (dict(logits=torch.zeros(4, 0)), ValueError),
+        (dict(temperature=-1.0), ValueError),
+        (dict(temperature=math.nan), ValueError),
+        (dict(top_k=-1), ValueError),
+        (dict(top_k=2.5), ValueError),
+        (dict(top_k=torch.ones(4)), ValueError),
+        (dict(top_k=torch.ones(3, dtype=torch.int64)), ValueError),
+        (dict(top_p=1.5), ValueError),
+        (dict(top_p=-0.1), ValueError),
+        (dict(min_p=1.1), ValueError),
+        (dict(min_p=torch.ones(4, 1)), ValueError),
+        (dict(temperature=torch.ones(4, dtype=torch.bool)), ValueError),
+        (dict(logits=torch.zeros(4, 7, requires_grad=True)), RuntimeError),
+        (dict(), RuntimeError),
+    ],
+)
+def test_sample_tokens_refusals(kw, err):
+    args = dict(logits=torch.zeros(4, 7), u=torch.zeros(4))
+    args.update(kw)
+    with pytest.raises(err):
+        sample_tokens(**args)
+
+
+def test_linear_sample_refuses_a_u_of_another_shape():
+    with pytest.raises(ValueError):
+        linear_sample(torch.zeros(4, 16), torch.zeros(10, 16), torch.zeros(3))
+
+
+def test_c_entry_points_check_their_arguments():
+    L = _native.lib()
+    bad = -1  # CCE_ERR_ARG
+    assert L.cce_b200_logits(None, None, 0, None) == bad
+    assert L.cce_b200_sample(None, None) == bad
+    assert L.cce_b200_logits_workspace_bytes(None) == 0
+
+    buf = ctypes.create_string_buffer(64)
+    ptr = ctypes.addressof(buf)
+
+    def logits_args(**kw):
+        a = _native.LogitsArgs()
+        a.op.e = a.op.c = a.out = ptr
+        a.op.n_total = a.op.n_rows = 4
+        a.op.V, a.op.D, a.op.lde, a.op.ldc, a.op.dtype = 10, 16, 16, 16, _native.DT_BF16
+        a.out_dtype = _native.DT_BF16
+        for k, v in kw.items():
+            setattr(a.op if hasattr(a.op, k) else a, k, v)
+        return a
+
+    lora = dict(lora_a=ptr, lora_b=ptr, adapter_ids=ptr, n_adapters=2, rank=8)
+    assert L.cce_b200_logits_workspace_bytes(logits_args()) > 0
+    # room for one padded fp32 row of inner products per token
+    assert (L.cce_b200_logits_workspace_bytes(logits_args(n_total=1000, n_rows=1000, **lora))
+            - L.cce_b200_logits_workspace_bytes(logits_args(n_total=1000, n_rows=1000))) == 1000 * 16 * 4  # fmt: skip
+    for kw in (
+        dict(e=None), dict(V=0), dict(D=0), dict(lde=15), dict(n_rows=3), dict(out_dtype=3), dict(dtype=7),
+        dict(lora_a=ptr), dict(lora, rank=0), dict(lora, rank=257), dict(lora, n_adapters=0),
+        dict(lora, ids_dtype=2), dict(has_softcap=1, softcap=0.0),
+    ):  # fmt: skip
+        assert L.cce_b200_logits_workspace_bytes(logits_args(**kw)) == 0, kw
+        assert L.cce_b200_logits(logits_args(**kw), ptr, 1 << 40, None) == bad, kw
+    assert L.cce_b200_logits(logits_args(), None, 0, None) == bad
+    assert L.cce_b200_logits(logits_args(), ptr, 0, None) == -3  # CCE_ERR_WORKSPACE
+    assert L.cce_b200_logits(logits_args(n_total=0, n_rows=0), None, 0, None) == 0
+
+    def sample_args(**kw):
+        a = _native.SampleArgs()
+        a.logits = a.u = a.tokens = ptr
+        a.B, a.V, a.ld, a.dtype = 2, 10, 10, _native.DT_F32
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return a
+
+    for kw in (dict(logits=None), dict(u=None), dict(tokens=None), dict(V=0), dict(B=-1), dict(ld=9), dict(dtype=3)):
+        assert L.cce_b200_sample(sample_args(**kw), None) == bad, kw
+    assert L.cce_b200_sample(sample_args(logits=ptr + 2), None) == -2  # CCE_ERR_ALIGN
+    assert L.cce_b200_sample(sample_args(B=0, logits=None), None) == 0
+
+
+def test_struct_sizes_match_the_header(tmp_path):
+    import shutil
+    import subprocess
+    from pathlib import Path
+
+    gcc = shutil.which("gcc")
+    if gcc is None:
+        pytest.skip("no C compiler")
+    root = Path(__file__).resolve().parent.parent
+    src = tmp_path / "s.c"
+    src.write_text(
+        '#include "cce_b200.h"\n#include <stdio.h>\n#include <stddef.h>\n'
+        "int main(void) { printf(\"%zu %zu %zu %zu\\n\", sizeof(cce_b200_logits_args), "
+        "offsetof(cce_b200_logits_args, rank), sizeof(cce_b200_sample_args), "
+        "offsetof(cce_b200_sample_args, logprobs)); return 0; }\n"
+    )
+    subprocess.run([gcc, "-I", str(root / "include"), "-o", str(tmp_path / "s"), str(src)], check=True)
+    got = subprocess.run([str(tmp_path / "s")], check=True, capture_output=True, text=True).stdout.split()
+    A, S = _native.LogitsArgs, _native.SampleArgs
+    assert [int(g) for g in got] == [ctypes.sizeof(A), A.rank.offset, ctypes.sizeof(S), S.logprobs.offset]
+
+
+def test_oracle_sampling_known_answers():
+    x = torch.log(torch.tensor([0.1, 0.4, 0.2, 0.3]))
+    assert H.sample_row(x, 0.0)[0] == 0
+    assert H.sample_row(x, 0.0999)[0] == 0 and H.sample_row(x, 0.1001)[0] == 1
+    assert H.sample_row(x, 0.71)[0] == 3
+    assert H.sample_row(x, 0.99, top_k=2)[0] == 3 and H.sample_row(x, 0.0, top_k=2)[0] == 1
+    assert H.sample_row(x, 0.99, top_p=0.39)[0] == 1  # one token reaches it
+    assert H.sample_row(x, 0.99, top_p=0.41)[0] == 3
+    assert H.sample_row(x, 0.0, min_p=0.6)[0] == 1 and H.sample_row(x, 0.99, min_p=0.6)[0] == 3
+    assert H.sample_row(x, 0.3, temperature=0.0) == (1, 0.0)
+    assert H.sample_row(torch.full((4,), -math.inf), 0.3) == (-1, -math.inf)
+    assert math.isclose(H.sample_row(x, 0.99, top_k=2)[1], math.log(0.3 / 0.7), rel_tol=1e-6)
+    # equal logits: the lower index comes first
+    assert H.sample_row(torch.zeros(5), 0.99, top_k=2)[0] == 1
+
+
+def test_oracle_logits_known_answer():
+    e = torch.tensor([[1.0, 2.0]])
+    c = torch.tensor([[1.0, 0.0], [0.0, 1.0], [1.0, 1.0]])
+    a, b = torch.tensor([[[1.0, 1.0]]]), torch.tensor([[[1.0], [0.0], [2.0]]])
+    x, _ = H.linear_logits(e, c, bias=torch.tensor([0.5, 0.0, 0.0]), lora_a=a, lora_b=b,
+                           adapter_ids=torch.tensor([0]), lora_scale=torch.tensor([2.0]))  # fmt: skip
+    assert x.tolist() == [[1.0 + 0.5 + 6.0, 2.0, 3.0 + 12.0]]
