@@ -330,8 +330,8 @@ int cce_b200_logits(const cce_b200_logits_args* a, void* workspace, size_t works
  * logprobs (optional): the logarithm of the token's share of the kept weights; 0 for the largest, -inf for -1.
  * A setting is an array with one value per row, or (array NULL) the *_all value for every row; top_k <= 0
  * or >= V, top_p >= 1 and min_p <= 0 switch a filter off.  Sums are exact (64-bit fixed point), so the result
- * does not depend on the launch.  V is bounded by the shared memory of eight SMs (CCE_ERR_TOO_LARGE above
- * about 380 000 fp32 or 770 000 16-bit logits).  No workspace. */
+ * does not depend on the launch.  V is bounded by the shared memory of sixteen SMs (CCE_ERR_TOO_LARGE above
+ * 2^20, or about 780 000 fp32 logits).  No workspace. */
 typedef struct cce_b200_sample_args {
     const void* logits;  /* [B][V], row stride ld elements */
     int64_t B, V, ld;

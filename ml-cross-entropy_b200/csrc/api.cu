@@ -133,8 +133,10 @@ int device_info(DeviceInfo** out) {
                               (const void*)head_logits_kernel<__nv_bfloat16>})
             CCE_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, HEAD_SMEM));
         for (const void* k : {(const void*)sample_kernel<float>, (const void*)sample_kernel<__half>,
-                              (const void*)sample_kernel<__nv_bfloat16>})
+                              (const void*)sample_kernel<__nv_bfloat16>}) {
             CCE_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMP_SMEM));
+            CCE_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        }
         d.attr_set = true;
     }
     *out = &d;

@@ -48,7 +48,7 @@ def sample_tokens(
     The first is always kept.  The token is the first kept one, by index, whose running sum of weights exceeds
     ``u`` times their sum.  The sums are exact, so equal inputs give equal tokens in every batch.
 
-    :param logits: ``(..., V)``, bf16, fp16 or fp32; V at most about 380 000 in fp32, 770 000 in 16 bits.
+    :param logits: ``(..., V)``, bf16, fp16 or fp32; V at most 2**20, in fp32 about 780 000.
     :param u: ``(...)`` float32 in [0, 1).
     :param temperature: number or ``(...)`` tensor; 0 takes the first of the largest logits.
     :param top_k: number or ``(...)`` tensor; ``None``, 0 or V and more: off.

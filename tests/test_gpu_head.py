@@ -359,10 +359,12 @@ def test_sample_strides_and_alignment(dtype):
 def test_sample_empty_and_too_large():
     assert sample_tokens(torch.zeros(0, 10, device=DEV), torch.zeros(0, device=DEV)).shape == (0,)
     with pytest.raises(_native.NativeError):
-        sample_tokens(torch.zeros(1, 500_000, device=DEV), torch.zeros(1, device=DEV))
-    x, u = _rows(2, 500_000, BF16)
+        sample_tokens(torch.zeros(1, 1_000_000, device=DEV), torch.zeros(1, device=DEV))
+    with pytest.raises(_native.NativeError):
+        sample_tokens(torch.zeros(1, 2**20 + 1, device=DEV, dtype=BF16), torch.zeros(1, device=DEV))
+    x, u = _rows(2, 2**20, BF16)
     _check_sample(x, u, top_k=20, top_p=0.9)
-    x, u = _rows(2, 380_000, FP32)
+    x, u = _rows(2, 700_000, FP32)
     _check_sample(x, u, top_p=0.99)
 
 
