@@ -96,6 +96,15 @@ bool pair_enabled() {
     return on;
 }
 
+template <typename T>
+cudaError_t head_logits_attributes() {
+    for (auto* k : {head_logits_kernel<T, 0>, head_logits_kernel<T, 1>, head_logits_kernel<T, 2>, head_logits_kernel<T, 4>}) {
+        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, HEAD_SMEM);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
 struct DeviceInfo {
     int sms = 0;
     int cc_major = 0;
@@ -129,9 +138,9 @@ int device_info(DeviceInfo** out) {
                                       PAIR_SMEM));
         CCE_CUDA(cudaFuncSetAttribute(pair_engine_kernel<MODE_GEMM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       PAIR_SMEM + PEER_STAGE_BYTES));
-        for (const void* k : {(const void*)head_logits_kernel<float>, (const void*)head_logits_kernel<__half>,
-                              (const void*)head_logits_kernel<__nv_bfloat16>})
-            CCE_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, HEAD_SMEM));
+        CCE_CUDA(head_logits_attributes<float>());
+        CCE_CUDA(head_logits_attributes<__half>());
+        CCE_CUDA(head_logits_attributes<__nv_bfloat16>());
         for (const void* k : {(const void*)sample_kernel<float>, (const void*)sample_kernel<__half>,
                               (const void*)sample_kernel<__nv_bfloat16>}) {
             CCE_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMP_SMEM));

@@ -21,31 +21,115 @@ int check_logits_args(const cce_b200_logits_args* a) {
 
 struct LogitsPlan {
     OperandPlan ops;
-    long long ldh;
-    size_t off_h, total;
+    long long ldh, n_col, n_group;
+    bool sorted;         // the columns are ordered by adapter
+    int pitch16;         // row length of the 16-bit h; 0: every group of columns is mixed
+    int shrink_ranks;    // ranks that the shrink kernel writes: whole padding blocks of both forms of h
+    long long ld_cols;
+    size_t off_bad, off_group, off_cols, off_ncol, off_e_cols, off_h, off_h16, total;
 };
 
 LogitsPlan plan_logits(const cce_b200_logits_args* a) {
-    LogitsPlan pl;
-    pl.ops = plan_operands(&a->op, 256);
-    pl.ldh = a->lora_b ? cdiv(a->rank, ADAPTER_RANK_PAD) * ADAPTER_RANK_PAD : 0;
-    pl.off_h = pl.ops.end;
-    pl.total = align_up(pl.off_h + (size_t)a->op.n_total * pl.ldh * 4, 256);
+    LogitsPlan pl = {};
+    const long long T = a->op.n_total;
+    pl.n_col = T;
+    bool mma = false;
+    if (a->lora_b) {
+        // TMA reads the adapters' rows: 16-byte pitch and base
+        mma = a->op.dtype != CCE_DT_F32 && a->rank % 8 == 0 && (reinterpret_cast<uintptr_t>(a->lora_b) & 15) == 0;
+        // Columns ordered by adapter need up to 15 more per adapter.  They are free while the product is bound by
+        // reading the classifier (up to 256 columns) and cheaper than mixed groups up to twice the tokens.
+        const long long padded = T + (HEAD_GROUP - 1) * std::min<long long>(T, a->n_adapters + 1);
+        pl.sorted = mma && T > 1 && padded <= std::max<long long>(BN, 2 * T);
+        if (pl.sorted) pl.n_col = cdiv(padded, HEAD_GROUP) * HEAD_GROUP;
+        pl.n_group = cdiv(pl.n_col, HEAD_GROUP);
+    }
+    // the status word and, behind it, the flags that are cleared with it
+    size_t off = 256;
+    auto take = [&](size_t bytes) {
+        const size_t at = off;
+        off = align_up(off + bytes, 256);
+        return at;
+    };
+    pl.off_bad = take((size_t)pl.n_group * 4);
+    pl.off_group = take((size_t)pl.n_group * 4);
+    if (pl.sorted) {
+        pl.off_cols = take((size_t)pl.n_col * 4);
+        pl.off_ncol = take(4);
+    }
+    pl.ops = plan_operands(&a->op, off, pl.sorted);  // ordered columns bring their own copy of e
+    off = pl.ops.end;
+    if (pl.sorted) {
+        pl.ld_cols = cdiv(a->op.D, 8) * 8;
+        pl.off_e_cols = take((size_t)pl.n_col * pl.ld_cols * 2);
+    }
+    if (a->lora_b) {
+        pl.ldh = cdiv(a->rank, ADAPTER_RANK_PAD) * ADAPTER_RANK_PAD;
+        pl.pitch16 = mma ? h16_pitch((int)a->rank) : 0;
+        pl.shrink_ranks = (int)(!mma ? pl.ldh : a->rank <= 32 ? 32 : cdiv(a->rank, 64) * 64);
+        pl.off_h = take((size_t)pl.n_col * pl.ldh * 4);
+        pl.off_h16 = take((size_t)pl.n_col * pl.pitch16 * 2);
+    }
+    pl.total = off;
     return pl;
 }
 
-template <typename T>
-int launch_shrink(const ShrinkParams& sp, cudaStream_t st) {
-    const dim3 grid((unsigned)cdiv(sp.T, SHRINK_TOK), (unsigned)(sp.ldh / SHRINK_RANK));
-    adapter_shrink_kernel<T><<<grid, SHRINK_WARPS * 32, 0, st>>>(sp);
+// Launches with the leave to start while the kernel before it in the stream still runs (a kernel that waits for it
+// itself before it reads what that one wrote).
+template <typename K, typename... Args>
+int launch_behind(K* kernel, dim3 grid, int threads, int smem, cudaStream_t st, bool overlap, const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = overlap ? 1 : 0;
+    cudaLaunchKernelEx(&cfg, kernel, args...);
     CCE_LAUNCH_CHECK();
     return CCE_OK;
 }
 
 template <typename T>
-int launch_head(const CUtensorMap& tc, const CUtensorMap& te, const HeadParams& hp, int grid, cudaStream_t st) {
-    head_logits_kernel<T><<<grid, HEAD_THREADS, HEAD_SMEM, st>>>(tc, te, hp);
-    CCE_LAUNCH_CHECK();
+int launch_shrink(const ShrinkParams& sp, long long n_col, cudaStream_t st) {
+    const dim3 grid((unsigned)cdiv(n_col, SHRINK_TOK), (unsigned)(sp.rank_blocks + (sp.col_token ? 1 : 0)));
+    return launch_behind(adapter_shrink_kernel<T>, grid, SHRINK_WARPS * 32, 0, st, sp.col_token != nullptr, sp);
+}
+
+// With adapters the projection may start while the shrink kernel, launched just before it, still runs.
+template <typename T>
+int launch_head(const CUtensorMap (&tm)[4], const HeadParams& hp, int grid, cudaStream_t st) {
+    const bool segmented = hp.out_dtype == CCE_DT_F32 && cdiv(hp.n_kblk, HEAD_KSUB) > HEAD_SEGMENT;
+    const auto kernel = !segmented          ? head_logits_kernel<T, 0>
+                        : hp.n_tok <= 64    ? head_logits_kernel<T, 1>
+                        : hp.n_tok <= 128   ? head_logits_kernel<T, 2>
+                                            : head_logits_kernel<T, 4>;
+    return launch_behind(kernel, dim3(grid), HEAD_THREADS, HEAD_SMEM, st, hp.lora_b != nullptr, tm[0], tm[1], tm[2],
+                         tm[3], hp);
+}
+
+// The adapters' rows of B, [n][V][rank], as a 3-D map: a box of 64 ranks x 128 classifier rows of one adapter.
+int make_tmap_adapters(CUtensorMap* m, const void* base, int dtype, long long rank, long long V, long long n) {
+    EncodeTiledFn enc = get_encode();
+    if (!enc) {
+        g_last_cuda = -1;
+        return CCE_ERR_CUDA;
+    }
+    cuuint64_t dims[3] = {(cuuint64_t)rank, (cuuint64_t)V, (cuuint64_t)n};
+    cuuint64_t strides[2] = {(cuuint64_t)rank * 2, (cuuint64_t)(rank * V) * 2};
+    cuuint32_t box[3] = {(cuuint32_t)BK, (cuuint32_t)BM, 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = enc(m, dtype == CCE_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                     3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        g_last_cuda = int(r);
+        return CCE_ERR_CUDA;
+    }
     return CCE_OK;
 }
 
@@ -93,13 +177,30 @@ int cce_b200_logits(const cce_b200_logits_args* a, void* workspace, size_t works
     if (rc) return rc;
     char* ws = reinterpret_cast<char*>(workspace);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    CCE_CUDA(cudaMemsetAsync(ws, 0, 256, st));
+    CCE_CUDA(cudaMemsetAsync(ws, 0, pl.off_bad + (size_t)pl.n_group * 4, st));
     Staged sg;
-    rc = stage_operands(&op, pl.ops, ws, st, &sg);
+    rc = stage_operands(&op, pl.ops, ws, st, &sg, pl.sorted ? ws + pl.off_e_cols : nullptr);
     if (rc) return rc;
 
     const int elem = op.dtype == CCE_DT_F32 ? 4 : 2;
     auto aligned16 = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
+    const int* col_token = pl.sorted ? reinterpret_cast<const int*>(ws + pl.off_cols) : nullptr;
+    const int* n_col_dev = pl.sorted ? reinterpret_cast<const int*>(ws + pl.off_ncol) : nullptr;
+    if (pl.sorted) {
+        LayoutParams lp = {};
+        lp.ids = a->adapter_ids;
+        lp.ids_i64 = a->ids_dtype == CCE_IDX_I64;
+        lp.n_adapters = (int)a->n_adapters;
+        lp.T = (int)op.n_total;
+        lp.n_col = (int)pl.n_col;
+        lp.col_token = reinterpret_cast<int*>(ws + pl.off_cols);
+        lp.n_col_dev = reinterpret_cast<int*>(ws + pl.off_ncol);
+        lp.group = reinterpret_cast<int*>(ws + pl.off_group);
+        adapter_layout_kernel<<<1, LAYOUT_THREADS, 0, st>>>(lp);
+        CCE_LAUNCH_CHECK();
+        sg.e = ws + pl.off_e_cols;
+        sg.lde = pl.ld_cols;
+    }
     if (a->lora_b) {
         ShrinkParams sp = {};
         sp.e = op.e;
@@ -111,16 +212,24 @@ int cce_b200_logits(const cce_b200_logits_args* a, void* workspace, size_t works
         sp.n_adapters = (int)a->n_adapters;
         sp.rank = (int)a->rank;
         sp.T = (int)op.n_total;
+        sp.col_token = col_token;
+        sp.n_col_dev = n_col_dev;
+        sp.e_cols = ws + pl.off_e_cols;
+        sp.ld_cols = pl.ld_cols;
+        sp.rank_blocks = pl.shrink_ranks / SHRINK_RANK;
         sp.D = op.D;
         sp.vec = aligned16(op.e) && aligned16(a->lora_a) && (op.D * elem) % 16 == 0 && (op.lde * elem) % 16 == 0;
         sp.h = reinterpret_cast<float*>(ws + pl.off_h);
         sp.ldh = (int)pl.ldh;
+        sp.h16 = pl.pitch16 ? ws + pl.off_h16 : nullptr;
+        sp.group = reinterpret_cast<int*>(ws + pl.off_group);
+        sp.group_bad = reinterpret_cast<int*>(ws + pl.off_bad);
         if (op.dtype == CCE_DT_F32)
-            rc = launch_shrink<float>(sp, st);
+            rc = launch_shrink<float>(sp, pl.n_col, st);
         else if (op.dtype == CCE_DT_BF16)
-            rc = launch_shrink<__nv_bfloat16>(sp, st);
+            rc = launch_shrink<__nv_bfloat16>(sp, pl.n_col, st);
         else
-            rc = launch_shrink<__half>(sp, st);
+            rc = launch_shrink<__half>(sp, pl.n_col, st);
         if (rc) return rc;
     }
 
@@ -128,12 +237,16 @@ int cce_b200_logits(const cce_b200_logits_args* a, void* workspace, size_t works
     hp.T = (int)op.n_total;
     hp.V = (int)op.V;
     hp.n_kblk = (int)cdiv(sg.Dk, BK);
-    hp.n_ntile = (int)cdiv(op.n_total, BN);
-    hp.n_tok = (int)(cdiv(cdiv(op.n_total, hp.n_ntile), 16) * 16);  // even shares of the tokens
-    hp.n_vtile = (int)cdiv(op.V, BM);
-    hp.n_stage = std::min(HEAD_MAX_STAGES, HEAD_RING_BYTES / (A_BYTES + hp.n_tok * BK * 2));
+    hp.n_col = (int)pl.n_col;
+    hp.col_token = col_token;
+    hp.n_col_dev = n_col_dev;
+    const long long n_ntile = cdiv(pl.n_col, BN);
+    hp.n_tok = (int)(cdiv(cdiv(pl.n_col, n_ntile), HEAD_GROUP) * HEAD_GROUP);  // even shares of the columns
+    hp.n_acc = hp.n_tok <= 64 ? HEAD_MAX_ACC : hp.n_tok <= 128 ? HEAD_MAX_ACC / 2 : 2;
+    hp.n_vtile = (int)cdiv(op.V, 2 * BM);
+    hp.n_stage = std::min(HEAD_MAX_STAGES, HEAD_RING_BYTES / (HEAD_KSUB * (A_BYTES + hp.n_tok / 2 * BK * 2)));
     const int cdt = compute_dtype(&op);
-    hp.idesc = make_idesc(cdt == CCE_DT_BF16 ? 1 : 0, 0, 0, BM, hp.n_tok);
+    hp.idesc = make_idesc(cdt == CCE_DT_BF16 ? 1 : 0, 0, 0, 2 * BM, 0);
     hp.status = reinterpret_cast<int*>(ws);
     hp.bias = sg.bias;
     hp.has_softcap = op.has_softcap;
@@ -149,18 +262,27 @@ int cce_b200_logits(const cce_b200_logits_args* a, void* workspace, size_t works
         hp.b_vec = aligned16(a->lora_b) && (a->rank * elem) % 16 == 0;
         hp.h = reinterpret_cast<const float*>(ws + pl.off_h);
         hp.ldh = (int)pl.ldh;
+        hp.group = reinterpret_cast<const int*>(ws + pl.off_group);
+        hp.group_bad = reinterpret_cast<const int*>(ws + pl.off_bad);
     }
-    CUtensorMap tc, te;
-    rc = make_tmap(&tc, sg.c, cdt, sg.Dk, op.V, sg.ldc, BK, BM);
+    CUtensorMap tm[4];  // classifier, tokens, adapters' B, h
+    rc = make_tmap(&tm[0], sg.c, cdt, sg.Dk, op.V, sg.ldc, BK, BM);
     if (rc) return rc;
-    rc = make_tmap(&te, sg.e, cdt, sg.Dk, op.n_total, sg.lde, BK, hp.n_tok);
+    rc = make_tmap(&tm[1], sg.e, cdt, sg.Dk, pl.n_col, sg.lde, BK, hp.n_tok / 2);
     if (rc) return rc;
-    const long long n_items = (long long)hp.n_vtile * hp.n_ntile;
-    if (n_items >= (1LL << 31)) return CCE_ERR_ARG;
-    const int grid = (int)std::min<long long>(dev->sms, n_items);
-    if (op.dtype == CCE_DT_F32) return launch_head<float>(tc, te, hp, grid, st);
-    if (op.dtype == CCE_DT_BF16) return launch_head<__nv_bfloat16>(tc, te, hp, grid, st);
-    return launch_head<__half>(tc, te, hp, grid, st);
+    tm[2] = tm[3] = tm[1];
+    if (pl.pitch16) {
+        rc = make_tmap_adapters(&tm[2], a->lora_b, cdt, a->rank, op.V, a->n_adapters);
+        if (rc) return rc;
+        rc = make_tmap(&tm[3], ws + pl.off_h16, cdt, pl.pitch16, pl.n_col, pl.pitch16, BK, 8);
+        if (rc) return rc;
+    }
+    const long long n_items = (long long)hp.n_vtile * n_ntile;
+    if (n_items >= (1LL << 30)) return CCE_ERR_ARG;
+    const int grid = 2 * (int)std::min<long long>(dev->sms / 2, n_items);
+    if (op.dtype == CCE_DT_F32) return launch_head<float>(tm, hp, grid, st);
+    if (op.dtype == CCE_DT_BF16) return launch_head<__nv_bfloat16>(tm, hp, grid, st);
+    return launch_head<__half>(tm, hp, grid, st);
 }
 
 int cce_b200_sample(const cce_b200_sample_args* a, void* stream) {

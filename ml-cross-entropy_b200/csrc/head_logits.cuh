@@ -4,41 +4,57 @@
 //
 // (no adapter term where ids[t] lies outside [0, n); cap(x) = softcap * tanh(x / softcap)).
 //
-// adapter_shrink_kernel computes h[t][j] = s_a (A[a][j] . e_t), T x rank fp32 values.
-// head_logits_kernel is the projection.  Its tiles are 128 classifier rows x up to 256 tokens, with
-// the classifier on the M side of the tensor-core product and the tokens on the N side: a decode
-// batch of 1..16 tokens then costs an N = 16 product instead of padding 128 rows, the token
-// operand of a stage shrinks to 2 KB, and a thread of the epilogue (one TMEM lane) owns one
-// vocabulary entry, so that a warp's store covers 32 neighbouring logits of one token and its
-// row of B is read once for all tokens of an adapter.
+// adapter_shrink_kernel computes h[t][j] = s_a (A[a][j] . e_t), T x rank values.
+// head_logits_kernel is the projection, on CTA pairs (tcgen05 cta_group::2).  Its tiles are 256 classifier
+// rows x up to 256 tokens, with the classifier on the M side of the tensor-core product and the tokens
+// on the N side: a decode batch of 1..16 tokens then costs an N = 16 product instead of padding 128
+// rows, the token operand shrinks to 1 KB per CTA and 64 reduction elements, and a thread of the epilogue
+// (one TMEM lane) owns one vocabulary entry, so that a warp's store covers 32 neighbouring logits of one token.
 //
-//   warp 0      : TMA producer  (128-byte swizzled ring; as many stages as shared memory holds)
-//   warp 1      : tcgen05.mma issuer, owns the TMEM allocation (2 accumulators of 128 x 256 fp32)
+//   warp 0      : TMA producer of both CTAs (128-byte swizzled ring; as many stages as shared memory holds)
+//   warp 1      : tcgen05.mma issuer (leader CTA), owner of the TMEM (2 accumulators of 128 x 256 fp32 per CTA)
 //   warps 2..9  : epilogue; warp w reads TMEM lanes 32*(w%4)..+31, two warps share a quarter
 //
-// The adapters' second product stays on the fp32 pipe of the epilogue: every token picks its own
-// rows of B, h is kept in fp32, and an infinity in one request's adapter cannot reach another's row
-// (a masked tensor-core product would multiply it by zero).
+// The adapters' second product.  The accumulator's columns are looked at in groups of 16.  A group whose tokens
+// all use one adapter (or none) takes it on the tensor cores, as further reduction blocks of the same columns: A
+// operand = the tile's rows of B, B operand = the group's h, split into two 16-bit terms (hi + lo) so that it keeps
+// 16 or more bits.  A group of several adapters is added by the epilogue in fp32, every token with its own rows
+// of B: a masked tensor-core product would multiply one request's adapter by another's zeros, and an infinity
+// there would reach the wrong row.  The same holds for groups whose h does not fit the 16-bit type.
+// Unless the adapters are many (api_serving.cuh has the rule) adapter_layout_kernel orders the columns by
+// adapter, each adapter's run padded to whole groups, so that no group is mixed.
 #pragma once
 #include "engine.cuh"
+#include "ptx_pair.cuh"
 
 namespace cce {
 
 constexpr int HEAD_EPI_WARPS = 8;
 constexpr int HEAD_THREADS = 64 + 32 * HEAD_EPI_WARPS;
-constexpr int HEAD_MAX_STAGES = 12;
+constexpr int HEAD_KSUB = 2;                   // 64-element K sub-blocks per ring stage
+constexpr int HEAD_MAX_STAGES = 8;
 constexpr int HEAD_SMEM = 227 * 1024;          // everything: the ring decides how many bytes are in flight
 constexpr int HEAD_RING_BYTES = HEAD_SMEM - 1024 /*align slack*/ - 512 /*barriers*/;
-constexpr int ADAPTER_RANK_PAD = 16;           // h rows are padded to this many ranks with zeros
+constexpr int HEAD_GROUP = 16;                 // tokens that share one decision about their adapters
+constexpr int ADAPTER_RANK_PAD = 16;           // fp32 rows of h are padded to this many ranks with zeros
+constexpr int GROUP_NONE = -1, GROUP_MIXED = -2;
+constexpr int HEAD_MAX_ACC = 8;
+// fp32 logits: the tensor core truncates every addition, so a sum over all of D drifts (2.4e-6 of the logits'
+// norm at D = 2304).  The accumulator is therefore emptied every HEAD_SEGMENT stages into fp32 registers,
+// which add with rounding (2e-7).  16-bit logits are rounded far above the drift and take the sum in one piece.
+constexpr int HEAD_SEGMENT = 2;
 
 struct HeadParams {
     int T, V;          // tokens, classifier rows
     int n_kblk;        // ceil(K / 64)
-    int n_tok;         // tokens per tile: a multiple of 16, at most 256
-    int n_ntile;       // token tiles
-    int n_vtile;       // classifier tiles of 128 rows
+    int n_tok;         // columns (tokens) a tile has room for: a multiple of 16, at most 256
+    int n_col;         // columns: T, or with col_token an upper bound of *n_col_dev
+    int n_vtile;       // classifier tiles of 256 rows
     int n_stage;
-    uint32_t idesc;
+    int n_acc;         // accumulators in TMEM: 512 columns in n_acc parts of at least n_tok
+    const int* col_token;  // null (column = token), or [n_col]: the token of every column, -1 for padding
+    const int* n_col_dev;
+    uint32_t idesc;    // without its N field
     int* status;
     const float* bias;  // fp32 [V] or null
     int has_softcap;
@@ -52,31 +68,74 @@ struct HeadParams {
     int n_adapters;
     int rank;
     int b_vec;           // rows of B can be read 16 bytes at a time
-    const float* h;      // [T][ldh] fp32, zero padded to ldh = rank rounded up to ADAPTER_RANK_PAD
+    const float* h;      // [column][ldh] fp32, zero padded to ldh = rank rounded up to ADAPTER_RANK_PAD
     int ldh;
+    const int* group;    // [ceil(columns / 16)]: the adapter of a group, GROUP_NONE or GROUP_MIXED
+    const int* group_bad;  // likewise; non-zero: h does not fit the 16-bit type, treat as mixed
 };
+
+// The column tiles of a launch, from the number of columns that the device knows.
+struct HeadTiles {
+    int n_col, n_ntile, n_tok;
+    __device__ __forceinline__ explicit HeadTiles(const HeadParams& p) {
+        n_col = p.n_col_dev ? min(*p.n_col_dev, p.n_col) : p.n_col;
+        n_ntile = (n_col + p.n_tok - 1) / p.n_tok;
+        n_tok = ((n_col + n_ntile - 1) / n_ntile + HEAD_GROUP - 1) / HEAD_GROUP * HEAD_GROUP;  // even shares
+    }
+};
+
+// Layout of the 16-bit rows of h: rank <= 32 (one 64-element block): hi in columns 0..31, lo in 32..63; above that,
+// for every 64 ranks a block of hi and a block of lo.
+__host__ __device__ inline int h16_pitch(int rank) { return rank <= 32 ? 64 : (rank + 63) / 64 * 128; }
 
 template <typename T>
 __device__ __forceinline__ float to_float(T x) { return float(x); }
 
-// 16 consecutive values of a row of B (ranks k0 .. k0+15 of `rank`; zeros past it) as fp32
-template <typename T>
-__device__ __forceinline__ void load_b16(const T* row, int k0, int rank, bool vec, float (&b)[ADAPTER_RANK_PAD]) {
-    constexpr int VE = 16 / int(sizeof(T));
-    if (vec) {  // rank is a multiple of VE
-#pragma unroll
-        for (int q = 0; q < ADAPTER_RANK_PAD / VE; ++q) {
-            uint4 u = make_uint4(0u, 0u, 0u, 0u);
-            if (k0 + q * VE < rank) u = __ldg(reinterpret_cast<const uint4*>(row + k0 + q * VE));
-            const T* x = reinterpret_cast<const T*>(&u);
-#pragma unroll
-            for (int i = 0; i < VE; ++i) b[q * VE + i] = to_float(x[i]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < ADAPTER_RANK_PAD; ++i) b[i] = (k0 + i < rank) ? to_float(row[k0 + i]) : 0.0f;
-    }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+__device__ __forceinline__ int group_adapter(const HeadParams& p, int g) {
+    const int a = p.group[g];
+    return a >= 0 && p.group_bad[g] ? GROUP_MIXED : a;
 }
+
+// The runs of neighbouring groups of a column tile that share an adapter: f(adapter, first column, columns) for each.
+// The producers of both CTAs and the MMA issuer call this and see the same sequence.  f returns false to stop.
+template <typename F>
+__device__ __forceinline__ bool walk_runs(const HeadParams& p, const HeadTiles& tiles, int col0, F f) {
+    const int g0 = col0 / HEAD_GROUP;
+    const int g1 = (min(tiles.n_col, col0 + tiles.n_tok) + HEAD_GROUP - 1) / HEAD_GROUP;
+    int a = GROUP_NONE, first = g0;
+    for (int g = g0; g <= g1; ++g) {
+        const int b = g < g1 ? group_adapter(p, g) : GROUP_NONE;
+        if (g == g1 || b != a) {
+            if (a >= 0 && !f(a, (first - g0) * HEAD_GROUP, (g - first) * HEAD_GROUP)) return false;
+            a = b;
+            first = g;
+        }
+    }
+    return true;
+}
+
+// 16 consecutive values of a row of B (ranks k0 .. k0+15 of `rank`; zeros past it), as they are stored
+template <typename T, bool VEC>
+struct BRow {
+    T x[ADAPTER_RANK_PAD];
+    __device__ __forceinline__ void load(const T* row, int k0, int rank) {
+        constexpr int VE = 16 / int(sizeof(T));
+        if constexpr (VEC) {  // rank is a multiple of VE
+#pragma unroll
+            for (int q = 0; q < ADAPTER_RANK_PAD / VE; ++q) {
+                uint4 u = make_uint4(0u, 0u, 0u, 0u);
+                if (k0 + q * VE < rank) u = __ldg(reinterpret_cast<const uint4*>(row + k0 + q * VE));
+                *reinterpret_cast<uint4*>(x + q * VE) = u;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < ADAPTER_RANK_PAD; ++i) x[i] = (k0 + i < rank) ? row[k0 + i] : T(0.0f);
+        }
+    }
+};
 
 __device__ __forceinline__ int adapter_of(const HeadParams& p, int t) {
     const long long a = p.ids_i64 ? reinterpret_cast<const long long*>(p.ids)[t]
@@ -84,38 +143,30 @@ __device__ __forceinline__ int adapter_of(const HeadParams& p, int t) {
     return (a >= 0 && a < p.n_adapters) ? int(a) : -1;
 }
 
-// x[j] += sum_k B[a_j][v][k] h[t0 + j][k] for the 32 tokens of one chunk; lane j holds a_j
-template <typename T>
-__device__ __forceinline__ void add_adapters(const HeadParams& p, int v, bool v_ok, int t0, int ncol, int my_id,
-                                             float (&x)[32]) {
-    if (!__any_sync(0xffffffffu, my_id >= 0)) return;
+// x[j] += sum_k B[a_j][v][k] h[col0 + j][k] for the 16 columns j of a mixed group; a_j comes from lane lane0 + j of my_id
+// (-1: none).  No branch depends on the token, so that the loads of several tokens are in flight.  Not inlined:
+// one copy serves every form of the kernel, and x (local memory) is touched by mixed groups only.
+template <typename T, bool VEC>
+__device__ __noinline__ void add_adapters(const HeadParams& p, int v, int col0, int n_col, int my_id, int lane0,
+                                          float* x) {
     const T* B = reinterpret_cast<const T*>(p.lora_b);
-#pragma unroll 1
     for (int k0 = 0; k0 < p.rank; k0 += ADAPTER_RANK_PAD) {
-        int cur = -1;
-        float b[ADAPTER_RANK_PAD];
+#pragma unroll 8
+        for (int j = 0; j < HEAD_GROUP; ++j) {
+            const int a = __shfl_sync(0xffffffffu, my_id, lane0 + j);
+            BRow<T, VEC> b;
+            b.load(B + ((size_t)max(a, 0) * p.V + v) * p.rank, k0, p.rank);
+            const float4* hp = reinterpret_cast<const float4*>(p.h + (size_t)min(col0 + j, n_col - 1) * p.ldh + k0);
+            float s = 0.0f;
 #pragma unroll
-        for (int i = 0; i < ADAPTER_RANK_PAD; ++i) b[i] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            const int a = __shfl_sync(0xffffffffu, my_id, j);  // warp-uniform; -1 past the last token
-            if (a >= 0) {
-                if (a != cur) {
-                    cur = a;
-                    if (v_ok) load_b16(B + ((size_t)a * p.V + v) * p.rank, k0, p.rank, p.b_vec != 0, b);
-                }
-                const float4* hp = reinterpret_cast<const float4*>(p.h + (size_t)(t0 + j) * p.ldh + k0);
-                float s = 0.0f;
-#pragma unroll
-                for (int q = 0; q < ADAPTER_RANK_PAD / 4; ++q) {
-                    const float4 hv = hp[q];
-                    s = fmaf(b[4 * q], hv.x, s);
-                    s = fmaf(b[4 * q + 1], hv.y, s);
-                    s = fmaf(b[4 * q + 2], hv.z, s);
-                    s = fmaf(b[4 * q + 3], hv.w, s);
-                }
-                x[j] += s;
+            for (int q = 0; q < ADAPTER_RANK_PAD / 4; ++q) {
+                const float4 hv = hp[q];
+                s = fmaf(to_float(b.x[4 * q]), hv.x, s);
+                s = fmaf(to_float(b.x[4 * q + 1]), hv.y, s);
+                s = fmaf(to_float(b.x[4 * q + 2]), hv.z, s);
+                s = fmaf(to_float(b.x[4 * q + 3]), hv.w, s);
             }
+            if (a >= 0) x[j] += s;
         }
     }
 }
@@ -130,11 +181,57 @@ template <>
 __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 
 template <typename O>
-__device__ __forceinline__ void store_column_chunk(const HeadParams& p, int v, int t0, int ncol, const float (&x)[32]) {
-    O* dst = reinterpret_cast<O*>(p.out) + (size_t)t0 * p.V + v;
+__device__ __forceinline__ void store_chunk(const HeadParams& p, int v, int my_token, const float (&x)[32]) {
+    O* dst = reinterpret_cast<O*>(p.out) + v;
+    const bool v_ok = v < p.V;
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-        if (j < ncol) dst[(size_t)j * p.V] = from_float<O>(x[j]);
+    for (int j = 0; j < 32; ++j) {
+        const int t = __shfl_sync(0xffffffffu, my_token, j);
+        if (t >= 0 && v_ok) dst[(size_t)t * p.V] = from_float<O>(x[j]);
+    }
+}
+
+// bias, mixed groups, soft-cap and store of one chunk of 32 columns; v is this lane's classifier row
+template <typename BT>
+__device__ __forceinline__ void finish_chunk(const HeadParams& p, const HeadTiles& tiles, int v, float bias, int c0,
+                                             int col_end, float (&x)[32]) {
+    const int lane = threadIdx.x & 31;
+    const int ncol = min(32, col_end - c0);
+    const int my_token = lane < ncol ? (p.col_token ? p.col_token[c0 + lane] : c0 + lane) : -1;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) x[j] += bias;
+    if (p.lora_b) {
+        const bool m0 = group_adapter(p, c0 / HEAD_GROUP) == GROUP_MIXED;
+        const bool m1 = ncol > HEAD_GROUP && group_adapter(p, c0 / HEAD_GROUP + 1) == GROUP_MIXED;
+        if (m0 || m1) {  // uniform over the warp
+            const int my_id = my_token >= 0 ? adapter_of(p, my_token) : -1;
+            const int row = min(v, p.V - 1);
+            float y[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) y[j] = x[j];
+            for (int g = 0; g < 2; ++g) {
+                if (!(g ? m1 : m0)) continue;
+                const int j0 = g * HEAD_GROUP;
+                if (p.b_vec)
+                    add_adapters<BT, true>(p, row, c0 + j0, tiles.n_col, my_id, j0, y + j0);
+                else
+                    add_adapters<BT, false>(p, row, c0 + j0, tiles.n_col, my_id, j0, y + j0);
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j] = y[j];
+        }
+    }
+    if (p.has_softcap) {
+        const float inv = 1.0f / p.softcap;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) x[j] = apply_softcap(x[j], p.softcap, inv);
+    }
+    if (p.out_dtype == 2)
+        store_chunk<float>(p, v, my_token, x);
+    else if (p.out_dtype == 1)
+        store_chunk<__nv_bfloat16>(p, v, my_token, x);
+    else
+        store_chunk<__half>(p, v, my_token, x);
 }
 
 struct HeadSmem {
@@ -144,36 +241,42 @@ struct HeadSmem {
     volatile int* abort_flag;
 };
 
-// BT: element type of the adapters (and of e)
-template <typename BT>
-__global__ void __launch_bounds__(HEAD_THREADS, 1)
+// BT: element type of the adapters (and of e).  CHUNKS > 0: the accumulator is emptied every HEAD_SEGMENT stages
+// into the epilogue's registers, CHUNKS chunks of 32 columns per warp (tiles of up to 64 CHUNKS columns); 0: it is not.
+template <typename BT, int CHUNKS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HEAD_THREADS, 1)
 head_logits_kernel(const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmE,
-                   const HeadParams p) {
+                   const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmH, const __grid_constant__ HeadParams p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const uint32_t stage_bytes = A_BYTES + p.n_tok * BK * 2;
+    const uint32_t sub_e = p.n_tok / 2 * BK * 2;  // this CTA's half of the tokens x 64 reduction elements
+    const uint32_t off_e = HEAD_KSUB * A_BYTES;   // of a stage: the token operand
+    const uint32_t stage_bytes = off_e + HEAD_KSUB * sub_e;
     HeadSmem s;
     s.stages = base;
     uint64_t* bars = reinterpret_cast<uint64_t*>(base + HEAD_RING_BYTES);
-    s.full = bars;
-    s.empty = bars + HEAD_MAX_STAGES;
-    s.tfull = bars + 2 * HEAD_MAX_STAGES;
-    s.tempty = s.tfull + 2;
-    s.tdown = s.tfull + 4;
-    s.tmem_base = reinterpret_cast<uint32_t*>(s.tfull + 5);
+    s.full = bars;                          // leader: both CTAs' bytes -> MMA
+    s.empty = bars + HEAD_MAX_STAGES;       // per CTA: MMA -> producer
+    s.tfull = bars + 2 * HEAD_MAX_STAGES;   // per CTA: MMA -> epilogue
+    s.tempty = s.tfull + HEAD_MAX_ACC;      // leader: both CTAs' epilogues -> MMA
+    s.tdown = s.tempty + HEAD_MAX_ACC;
+    s.tmem_base = reinterpret_cast<uint32_t*>(s.tdown + 1);
     s.abort_flag = reinterpret_cast<int*>(s.tmem_base + 1);
 
+    constexpr bool SEGMENTED = CHUNKS > 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int n_items = p.n_vtile * p.n_ntile;
-    if (int(blockIdx.x) >= n_items) return;  // uniform over the CTA
+    const int rank = int(cluster_ctarank());
+    const uint32_t acc_cols = TMEM_COLS / p.n_acc;
+    const int n_pairs = int(gridDim.x >> 1), pair = int(blockIdx.x >> 1);
+    const int n_kstage = (p.n_kblk + HEAD_KSUB - 1) / HEAD_KSUB;
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.n_stage; ++i) {
             mbar_init(smem_u32(&s.full[i]), 1);
             mbar_init(smem_u32(&s.empty[i]), 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < p.n_acc; ++i) {
             mbar_init(smem_u32(&s.tfull[i]), 1);
-            mbar_init(smem_u32(&s.tempty[i]), HEAD_EPI_WARPS);
+            mbar_init(smem_u32(&s.tempty[i]), 2 * HEAD_EPI_WARPS);
         }
         mbar_init(smem_u32(s.tdown), 1);
         *s.abort_flag = 0;
@@ -183,11 +286,13 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmC, const __grid_constan
         tma_prefetch_desc(&tmE);
     }
     if (warp == 1) {
-        tmem_alloc(smem_u32(s.tmem_base), TMEM_COLS);
-        tmem_relinquish();
+        tmem_alloc_pair(smem_u32(s.tmem_base), TMEM_COLS);
+        tmem_relinquish_pair();
     }
     tc_fence_before();
     __syncthreads();
+    cluster_arrive();  // both CTAs' barriers exist before either one signals the other
+    cluster_wait();
     tc_fence_after();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(s.tmem_base);
 
@@ -195,140 +300,346 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmC, const __grid_constan
         if (lane == 0) {
             int stage = 0;
             uint32_t phase = 0;
-            bool ok = true;
-            for (int item = blockIdx.x; ok && item < n_items; item += gridDim.x) {
-                const int row_c = (item / p.n_ntile) * BM, row_e = (item % p.n_ntile) * p.n_tok;
-                for (int kb = 0; kb < p.n_kblk; ++kb) {
-                    if (!mbar_wait(smem_u32(&s.empty[stage]), phase ^ 1u, s.abort_flag, p.status,
-                                   ERR_WAIT_SMEM_EMPTY)) {
-                        ok = false;
-                        break;
-                    }
-                    const uint32_t bar = smem_u32(&s.full[stage]);
-                    const uint32_t sa = smem_u32(s.stages) + stage * stage_bytes;
-                    mbar_expect_tx(bar, stage_bytes);
-                    tma_load_2d(sa, &tmC, bar, kb * BK, row_c);
-                    tma_load_2d(sa + A_BYTES, &tmE, bar, kb * BK, row_e);
-                    if (++stage == p.n_stage) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
+            auto free_stage = [&]() -> bool {
+                return mbar_wait(smem_u32(&s.empty[stage]), phase ^ 1u, s.abort_flag, p.status, ERR_WAIT_SMEM_EMPTY);
+            };
+            auto next_stage = [&]() {
+                if (++stage == p.n_stage) {
+                    stage = 0;
+                    phase ^= 1u;
                 }
+            };
+            auto sub_blocks = [&](int ks) { return min(HEAD_KSUB, p.n_kblk - ks * HEAD_KSUB); };
+            auto open_stage = [&](uint32_t bytes) {  // announces the bytes of both CTAs
+                if (rank == 0) mbar_expect_tx(smem_u32(&s.full[stage]), 2 * bytes);
+            };
+            auto load_c = [&](int ks, int row) {
+                const uint32_t bar = map_to_cta(smem_u32(&s.full[stage]), 0);
+                const uint32_t sa = smem_u32(s.stages) + stage * stage_bytes;
+                for (int j = 0; j < sub_blocks(ks); ++j)
+                    tma_load_2d_pair(sa + j * A_BYTES, &tmC, bar, (ks * HEAD_KSUB + j) * BK, row);
+            };
+            auto load_e = [&](int ks, int row) {
+                const uint32_t bar = map_to_cta(smem_u32(&s.full[stage]), 0);
+                const uint32_t sb = smem_u32(s.stages) + stage * stage_bytes + off_e;
+                for (int j = 0; j < sub_blocks(ks); ++j)
+                    tma_load_2d_pair(sb + j * sub_e, &tmE, bar, (ks * HEAD_KSUB + j) * BK, row);
+            };
+            // The first tile's classifier rows are known before the columns are, if there is one column tile: a
+            // ring of them is requested before the wait for the kernels that order the columns.
+            int ahead = 0;
+            if (p.lora_b && p.n_col <= p.n_tok) {
+                ahead = min(p.n_stage, n_kstage);
+                for (int ks = 0; ks < ahead; ++ks) {
+                    open_stage(sub_blocks(ks) * (A_BYTES + sub_e));
+                    load_c(ks, pair * 2 * BM + rank * BM);
+                    next_stage();
+                }
+                stage = 0;
+                phase = 0;
+            }
+            if (p.lora_b) pdl_wait();
+            const HeadTiles tiles(p);
+            const int n_items = p.n_vtile * tiles.n_ntile;
+            bool ok = true;
+            for (int item = pair; ok && item < n_items; item += n_pairs) {
+                const int row_c = (item / tiles.n_ntile) * 2 * BM + rank * BM;
+                const int col0 = (item % tiles.n_ntile) * tiles.n_tok;
+                const int row_e = col0 + rank * (tiles.n_tok / 2);
+                for (int ks = 0; ok && ks < n_kstage; ++ks) {
+                    if (ks >= ahead) {
+                        ok = free_stage();
+                        if (!ok) break;
+                        open_stage(sub_blocks(ks) * (A_BYTES + sub_e));
+                        load_c(ks, row_c);
+                    }
+                    load_e(ks, row_e);
+                    next_stage();
+                }
+                ahead = 0;
+                if (!ok || !p.lora_b) continue;
+                ok = walk_runs(p, tiles, col0, [&](int a, int run0, int ncol) -> bool {
+                    const int half = ncol / 2;  // rows of h that this CTA supplies: a multiple of 8
+                    const int terms = p.rank <= 32 ? 1 : 2;
+                    for (int r0 = 0; r0 < p.rank; r0 += BK) {
+                        if (!free_stage()) return false;
+                        open_stage(A_BYTES + terms * half * BK * 2);
+                        const uint32_t bar = map_to_cta(smem_u32(&s.full[stage]), 0);
+                        const uint32_t sa = smem_u32(s.stages) + stage * stage_bytes;
+                        tma_load_3d_pair(sa, &tmB, bar, r0, row_c, a);
+                        for (int i = 0; i < terms; ++i)
+                            for (int y = 0; y < half; y += 8)
+                                tma_load_2d_pair(sa + off_e + i * sub_e + y * BK * 2, &tmH, bar, r0 * 2 + i * BK,
+                                                 col0 + run0 + rank * half + y);
+                        next_stage();
+                    }
+                    return true;
+                });
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (lane == 0 && rank == 0) {
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
-            bool ok = true;
             const uint64_t adesc0 = make_smem_desc(smem_u32(s.stages), 16, 1024);
-            for (int item = blockIdx.x; ok && item < n_items; item += gridDim.x) {
-                if (!mbar_wait(smem_u32(&s.tempty[acc]), acc_phase ^ 1u, s.abort_flag, p.status,
-                               ERR_WAIT_TMEM_EMPTY))
-                    break;
+            const uint32_t empty0 = smem_u32(s.empty), empty1 = map_to_cta(empty0, 1);
+            const uint32_t tfull0 = smem_u32(s.tfull), tfull1 = map_to_cta(tfull0, 1);
+            // A filled stage, `issue(descriptor A, descriptor B)`, and the stage's release in both CTAs.
+            auto use = [&](auto issue) -> bool {
+                if (!mbar_wait(smem_u32(&s.full[stage]), phase, s.abort_flag, p.status, ERR_WAIT_SMEM_FULL)) return false;
                 tc_fence_after();
-                const uint32_t d_tmem = tmem_base + acc * BN;
-                for (int kb = 0; kb < p.n_kblk; ++kb) {
-                    if (!mbar_wait(smem_u32(&s.full[stage]), phase, s.abort_flag, p.status, ERR_WAIT_SMEM_FULL)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    // the address field of a descriptor counts 16-byte units
-                    const uint64_t ad = adesc0 + ((stage * stage_bytes) >> 4);
-                    const uint64_t bd = ad + (A_BYTES >> 4);
-#pragma unroll
-                    for (int k = 0; k < BK / UMMA_K; ++k)
-                        tc_mma_f16(d_tmem, ad + k * (UMMA_K * 2 >> 4), bd + k * (UMMA_K * 2 >> 4), p.idesc,
-                                   (kb | k) ? 1u : 0u);
-                    tc_commit(smem_u32(&s.empty[stage]));
-                    if (++stage == p.n_stage) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
+                // the address field of a descriptor counts 16-byte units
+                const uint64_t ad = adesc0 + ((stage * stage_bytes) >> 4);
+                issue(ad, ad + (off_e >> 4));
+                tc_commit_pair(empty0 + 8 * stage);
+                tc_commit_pair(empty1 + 8 * stage);
+                if (++stage == p.n_stage) {
+                    stage = 0;
+                    phase ^= 1u;
                 }
-                if (ok) tc_commit(smem_u32(&s.tfull[acc]));
-                if (++acc == 2) {
-                    acc = 0;
-                    acc_phase ^= 1u;
+                return true;
+            };
+            constexpr int STEP = UMMA_K * 2 >> 4;  // descriptor units per MMA step
+            if (p.lora_b) pdl_wait();
+            const HeadTiles tiles(p);
+            const int n_items = p.n_vtile * tiles.n_ntile;
+            const uint32_t idesc = p.idesc | (uint32_t(tiles.n_tok >> 3) << 17);
+            bool ok = true;
+            for (int item = pair; ok && item < n_items; item += n_pairs) {
+                uint32_t d_tmem = 0;
+                for (int ks = 0; ok && ks < n_kstage; ++ks) {
+                    const bool opens = SEGMENTED ? ks % HEAD_SEGMENT == 0 : ks == 0;
+                    if (opens) {
+                        ok = mbar_wait(smem_u32(&s.tempty[acc]), acc_phase ^ 1u, s.abort_flag, p.status,
+                                       ERR_WAIT_TMEM_EMPTY);
+                        if (!ok) break;
+                        tc_fence_after();
+                        d_tmem = tmem_base + acc * acc_cols;
+                    }
+                    const int n = min(HEAD_KSUB, p.n_kblk - ks * HEAD_KSUB);
+                    ok = use([&](uint64_t ad, uint64_t bd) {
+                        for (int j = 0; j < n; ++j)
+#pragma unroll
+                            for (int k = 0; k < BK / UMMA_K; ++k)
+                                tc_mma_f16_pair(d_tmem, ad + j * (A_BYTES >> 4) + k * STEP,
+                                                bd + j * (sub_e >> 4) + k * STEP, idesc, (!opens || j || k) ? 1u : 0u);
+                    });
+                    if (!ok) break;
+                    const bool last = ks + 1 == n_kstage;
+                    if (last && p.lora_b) {
+                        const int tile0 = (item % tiles.n_ntile) * tiles.n_tok;
+                        ok = walk_runs(p, tiles, tile0, [&](int, int run0, int ncol) -> bool {
+                            const uint32_t run_idesc = p.idesc | (uint32_t(ncol >> 3) << 17);
+                            const uint32_t lo = p.rank <= 32 ? 2 * STEP : sub_e >> 4;  // from the hi to the lo terms
+                            for (int r0 = 0; r0 < p.rank; r0 += BK) {
+                                const int steps = (min(BK, p.rank - r0) + UMMA_K - 1) / UMMA_K;
+                                if (!use([&](uint64_t ad, uint64_t bd) {
+                                        for (int k = 0; k < steps; ++k) {
+                                            tc_mma_f16_pair(d_tmem + run0, ad + k * STEP, bd + k * STEP, run_idesc, 1u);
+                                            tc_mma_f16_pair(d_tmem + run0, ad + k * STEP, bd + lo + k * STEP, run_idesc, 1u);
+                                        }
+                                    }))
+                                    return false;
+                            }
+                            return true;
+                        });
+                        if (!ok) break;
+                    }
+                    if (last || (SEGMENTED && (ks + 1) % HEAD_SEGMENT == 0)) {
+                        tc_commit_pair(tfull0 + 8 * acc);
+                        tc_commit_pair(tfull1 + 8 * acc);
+                        if (++acc == p.n_acc) {
+                            acc = 0;
+                            acc_phase ^= 1u;
+                        }
+                    }
                 }
             }
         }
     } else {
         const int q = warp & 3;              // TMEM lane quarter this warp may read
-        const int half = (warp - 2) >> 2;    // the quarter's two warps take alternate chunks of 32 tokens
+        const int half = (warp - 2) >> 2;    // the quarter's two warps take alternate chunks of 32 columns
+        const uint32_t tempty0 = map_to_cta(smem_u32(s.tempty), 0);
         int acc = 0;
         uint32_t acc_phase = 0;
         int ok = 1;
-        const float inv_softcap = p.has_softcap ? 1.0f / p.softcap : 0.0f;
-        for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
-            const int v = (item / p.n_ntile) * BM + q * 32 + lane;
-            const bool v_ok = v < p.V;
-            const int tok0 = (item % p.n_ntile) * p.n_tok;
-            const int tok_end = min(p.T, tok0 + p.n_tok);
-            const float bias = (p.bias && v_ok) ? __ldg(p.bias + v) : 0.0f;
-            // an abandoned wait: the rest of this CTA's tiles is written as NaN
-            if (ok) ok = mbar_wait(smem_u32(&s.tfull[acc]), acc_phase, s.abort_flag, p.status, ERR_WAIT_TMEM_FULL);
-            ok = __all_sync(0xffffffffu, ok);
-            if (ok) tc_fence_after();
-            const uint32_t taddr = tmem_base + acc * BN + (uint32_t(q * 32) << 16);
-#pragma unroll 1
-            for (int t0 = tok0 + half * 32; t0 < tok_end; t0 += 64) {
-                const int ncol = min(32, tok_end - t0);
-                float x[32];
-                if (ok) {
-                    uint32_t r[32];
-                    tmem_ld32(taddr + (t0 - tok0), r);
-                    tmem_ld_wait();
+        if (p.lora_b) pdl_wait();
+        const HeadTiles tiles(p);
+        const int n_items = p.n_vtile * tiles.n_ntile;
+        const int n_seg = SEGMENTED ? (n_kstage + HEAD_SEGMENT - 1) / HEAD_SEGMENT : 1;
+        for (int item = pair; item < n_items; item += n_pairs) {
+            const int v = (item / tiles.n_ntile) * 2 * BM + rank * BM + q * 32 + lane;
+            const int col0 = (item % tiles.n_ntile) * tiles.n_tok;
+            const int col_end = min(tiles.n_col, col0 + tiles.n_tok);
+            const float bias = (p.bias && v < p.V) ? __ldg(p.bias + v) : 0.0f;
+            float sum[SEGMENTED ? CHUNKS : 1][32];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(r[j]) + bias;
+            for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+                for (int j = 0; j < 32; ++j) sum[c][j] = 0.0f;
+            for (int seg = 0; seg < n_seg; ++seg) {
+                // an abandoned wait: the rest of this CTA's tiles is written as NaN
+                if (ok) ok = mbar_wait(smem_u32(&s.tfull[acc]), acc_phase, s.abort_flag, p.status, ERR_WAIT_TMEM_FULL);
+                ok = __all_sync(0xffffffffu, ok);
+                if (ok) tc_fence_after();
+                const uint32_t taddr = tmem_base + acc * acc_cols + (uint32_t(q * 32) << 16);
+                if constexpr (SEGMENTED) {
+#pragma unroll
+                    for (int c = 0; c < CHUNKS; ++c) {
+                        const int col = half * 32 + c * 64;
+                        if (col0 + col < col_end && ok) {  // uniform over the warp
+#pragma unroll
+                            for (int i = 0; i < 32; i += 16) {
+                                uint32_t r[16];
+                                tmem_ld16(taddr + col + i, r);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) sum[c][i + j] += __uint_as_float(r[j]);
+                            }
+                        }
+                    }
                 } else {
+#pragma unroll 1
+                    for (int c0 = col0 + half * 32; c0 < col_end; c0 += 64) {
+                        float x[32];
+                        uint32_t r[32];
+                        if (ok) {
+                            tmem_ld32(taddr + (c0 - col0), r);
+                            tmem_ld_wait();
+                        }
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) x[j] = __int_as_float(0x7fc00000);
+                        for (int j = 0; j < 32; ++j) x[j] = ok ? __uint_as_float(r[j]) : __int_as_float(0x7fc00000);
+                        finish_chunk<BT>(p, tiles, v, bias, c0, col_end, x);
+                    }
                 }
-                if (p.lora_b) {
-                    const int my_id = lane < ncol ? adapter_of(p, t0 + lane) : -1;
-                    add_adapters<BT>(p, v, v_ok, t0, ncol, my_id, x);
-                }
-                if (p.has_softcap) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) x[j] = apply_softcap(x[j], p.softcap, inv_softcap);
-                }
-                if (v_ok) {
-                    if (p.out_dtype == 2)
-                        store_column_chunk<float>(p, v, t0, ncol, x);
-                    else if (p.out_dtype == 1)
-                        store_column_chunk<__nv_bfloat16>(p, v, t0, ncol, x);
-                    else
-                        store_column_chunk<__half>(p, v, t0, ncol, x);
+                tc_fence_before();
+                __syncwarp();
+                if (ok && lane == 0) mbar_arrive_cluster(tempty0 + 8 * acc);
+                if (++acc == p.n_acc) {
+                    acc = 0;
+                    acc_phase ^= 1u;
                 }
             }
-            tc_fence_before();
-            __syncwarp();
-            if (ok && lane == 0) mbar_arrive(smem_u32(&s.tempty[acc]));
-            if (++acc == 2) {
-                acc = 0;
-                acc_phase ^= 1u;
+            if constexpr (SEGMENTED) {
+#pragma unroll 1
+                for (int c = 0; c < CHUNKS; ++c) {
+                    const int c0 = col0 + half * 32 + c * 64;
+                    if (c0 >= col_end) break;
+                    float x[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {  // a selection: registers cannot be indexed
+                        float s_c = sum[0][j];
+#pragma unroll
+                        for (int i = 1; i < CHUNKS; ++i) s_c = c == i ? sum[i][j] : s_c;
+                        x[j] = ok ? s_c : __int_as_float(0x7fc00000);
+                    }
+                    finish_chunk<BT>(p, tiles, v, bias, c0, col_end, x);
+                }
             }
         }
     }
 
-    // tear-down: wait (bounded) for every MMA this CTA issued, then release TMEM
+    // tear-down: the leader waits (bounded) for its MMAs; neither CTA leaves, or frees TMEM, while
+    // the other may still read its shared memory or signal its barriers
     tc_fence_before();
     __syncthreads();
-    if (warp == 1) {
+    if (warp == 1 && rank == 0) {
         if (lane == 0) {
-            tc_commit(smem_u32(s.tdown));
+            tc_commit_pair(smem_u32(s.tdown));
             mbar_wait(smem_u32(s.tdown), 0, s.abort_flag, p.status, ERR_WAIT_TEARDOWN);
         }
         __syncwarp();
+    }
+    cluster_arrive();
+    cluster_wait();
+    if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem_base, TMEM_COLS);
+        tmem_dealloc_pair(tmem_base, TMEM_COLS);
     }
 }
 
-// h[t][j] = scale[a_t] * (A[a_t][j] . e_t), zero where a token has no adapter and for the padding ranks.
-// One block per (8 consecutive tokens, 4 ranks): its 8 warps split D, each lane reads 16 bytes of the
+// The columns in order of their adapter: column runs of one adapter each, padded to whole groups of 16, tokens
+// without an adapter last.  One block; thread a walks all ids and places the tokens of adapters a, a + 1024, ...
+// (T steps: 0.3 us at 32 tokens, small beside the projection at thousands), so that the order is that of the tokens.
+constexpr int LAYOUT_THREADS = 1024;
+constexpr int LAYOUT_CHUNK = 4096;  // ids in shared memory at a time
+
+struct LayoutParams {
+    const void* ids;
+    int ids_i64;
+    int n_adapters, T, n_col;  // n_col: room in col_token
+    int* col_token;
+    int* n_col_dev;
+    int* group;
+};
+
+__global__ void __launch_bounds__(LAYOUT_THREADS)
+adapter_layout_kernel(const LayoutParams p) {
+    __shared__ __align__(16) int ids[LAYOUT_CHUNK];
+    __shared__ int warp_sum[32];
+    __shared__ int base;
+    pdl_launch();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // f(token, id) for every token in order, in the warps that have an adapter; the ids pass through shared memory
+    auto each = [&](bool active, auto f) {
+        for (int t0 = 0; t0 < p.T; t0 += LAYOUT_CHUNK) {
+            const int n = min(LAYOUT_CHUNK, p.T - t0);
+            __syncthreads();
+            for (int i = tid; i < (n + 3) / 4 * 4; i += LAYOUT_THREADS) {
+                if (i >= n) {
+                    ids[i] = -1;  // no thread's adapter
+                    continue;
+                }
+                const long long a = p.ids_i64 ? reinterpret_cast<const long long*>(p.ids)[t0 + i]
+                                              : (long long)reinterpret_cast<const int*>(p.ids)[t0 + i];
+                ids[i] = (a >= 0 && a < p.n_adapters) ? int(a) : p.n_adapters;
+            }
+            __syncthreads();
+            if (!active) continue;
+            for (int i = 0; i < n; i += 4) {
+                const int4 q = *reinterpret_cast<const int4*>(ids + i);
+                f(t0 + i, q.x);
+                f(t0 + i + 1, q.y);
+                f(t0 + i + 2, q.z);
+                f(t0 + i + 3, q.w);
+            }
+        }
+    };
+    if (tid == 0) base = 0;
+    for (int a0 = 0; a0 <= p.n_adapters; a0 += LAYOUT_THREADS) {
+        const int a = a0 + tid;
+        const bool active = a0 + warp * 32 <= p.n_adapters;
+        int count = 0;
+        each(active, [&](int, int id) { count += id == a; });
+        const int padded = a <= p.n_adapters ? (count + HEAD_GROUP - 1) / HEAD_GROUP * HEAD_GROUP : 0;
+        int incl = padded;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (lane == 31) warp_sum[warp] = incl;
+        __syncthreads();
+        int first = base + incl - padded;
+        for (int w = 0; w < warp; ++w) first += warp_sum[w];
+        int at = first;
+        each(active, [&](int t, int id) {
+            if (id == a && at < p.n_col) p.col_token[at++] = t;
+        });
+        for (; at < min(first + padded, p.n_col); ++at) p.col_token[at] = -1;
+        for (int g = first; g < min(first + padded, p.n_col); g += HEAD_GROUP)
+            p.group[g / HEAD_GROUP] = a < p.n_adapters ? a : GROUP_NONE;
+        __syncthreads();
+        if (tid == LAYOUT_THREADS - 1) base = first + padded;
+        __syncthreads();
+    }
+    if (tid == 0) *p.n_col_dev = base;
+}
+
+// h[column][j] = scale[a] * (A[a][j] . e_t), t and a the column's token and its adapter; zero without an adapter and
+// for the padding ranks; in fp32 and in the two 16-bit terms.  Without a column order the blocks of rank 0 also
+// write the groups' adapters; with one, the blocks of the last y gather the columns' rows of e.
+// One block per (8 consecutive columns, 4 ranks): its 8 warps split D, each lane reads 16 bytes of the
 // four rows of A and of every token of a run that shares an adapter, and the 32 sums are joined
 // in shared memory in warp order (no atomics: the same bits every run).
 constexpr int SHRINK_TOK = 8, SHRINK_RANK = 4, SHRINK_WARPS = 8;
@@ -341,10 +652,18 @@ struct ShrinkParams {
     const void* ids;
     int ids_i64;
     int n_adapters, rank, T;
+    const int* col_token;  // null: column = token
+    const int* n_col_dev;
+    void* e_cols;          // with col_token: [column][ld_cols], the rows of e in column order, zero padded
+    long long ld_cols;
+    int rank_blocks;       // blocks in y that compute; with col_token one more copies
     long long D;
     int vec;  // 16-byte loads are possible for every row
     float* h;
     int ldh;
+    void* h16;          // [T][h16_pitch(rank)] in the 16-bit type of e, or null: every group is mixed
+    int* group;         // [ceil(T / 16)]
+    int* group_bad;     // [ceil(T / 16)], zero before the launch
 };
 
 // 16 bytes of a row, `left` of whose elements remain (zeros past them); vec: loaded at once
@@ -364,16 +683,54 @@ adapter_shrink_kernel(const ShrinkParams p) {
     constexpr int VE = 16 / int(sizeof(T));
     __shared__ float part[SHRINK_WARPS][SHRINK_TOK * SHRINK_RANK];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tok0 = blockIdx.x * SHRINK_TOK, rank0 = blockIdx.y * SHRINK_RANK;
-    const int ntok = min(SHRINK_TOK, p.T - tok0);
-    int ids[SHRINK_TOK];
+    const int tok0 = blockIdx.x * SHRINK_TOK, rank0 = blockIdx.y * SHRINK_RANK;  // tok0: a column
+    pdl_launch();
+    const T* E = reinterpret_cast<const T*>(p.e);
+    int ids[SHRINK_TOK], tok[SHRINK_TOK];
+    int ntok;
+    if (p.col_token) {
+        pdl_wait();
+        ntok = min(SHRINK_TOK, *p.n_col_dev - tok0);
+        if (ntok <= 0) return;
+        const int a = p.group[tok0 / HEAD_GROUP];
 #pragma unroll
-    for (int i = 0; i < SHRINK_TOK; ++i) {
-        long long a = -1;
-        if (i < ntok)
-            a = p.ids_i64 ? reinterpret_cast<const long long*>(p.ids)[tok0 + i]
-                          : (long long)reinterpret_cast<const int*>(p.ids)[tok0 + i];
-        ids[i] = (a >= 0 && a < p.n_adapters) ? int(a) : -1;
+        for (int i = 0; i < SHRINK_TOK; ++i) {
+            tok[i] = i < ntok ? p.col_token[tok0 + i] : -1;
+            ids[i] = tok[i] >= 0 ? a : -1;
+        }
+        if (int(blockIdx.y) == p.rank_blocks) {
+            T* dst = reinterpret_cast<T*>(p.e_cols);
+            for (int i = 0; i < ntok; ++i) {
+                const int t = p.col_token[tok0 + i];
+                if (t < 0) continue;  // padding columns are never stored: whatever is there may be multiplied
+                for (long long d = threadIdx.x * VE; d < p.ld_cols; d += SHRINK_WARPS * 32 * VE)
+                    *reinterpret_cast<uint4*>(dst + (size_t)(tok0 + i) * p.ld_cols + d) =
+                        load_piece(E + (size_t)t * p.lde + d, p.D - d, p.vec != 0);
+            }
+            return;
+        }
+    } else {
+        ntok = min(SHRINK_TOK, p.T - tok0);
+        if (blockIdx.y == 0 && tok0 % HEAD_GROUP == 0 && warp == 0) {
+            const int n = min(HEAD_GROUP, p.T - tok0);
+            long long a = -1;
+            if (lane < n)
+                a = p.ids_i64 ? reinterpret_cast<const long long*>(p.ids)[tok0 + lane]
+                              : (long long)reinterpret_cast<const int*>(p.ids)[tok0 + lane];
+            const int id = (a >= 0 && a < p.n_adapters) ? int(a) : -1;
+            const int first = __shfl_sync(0xffffffffu, id, 0);
+            const bool same = __all_sync(0xffffffffu, lane >= n || id == first);
+            if (lane == 0) p.group[tok0 / HEAD_GROUP] = same && (first < 0 || p.h16) ? first : GROUP_MIXED;
+        }
+#pragma unroll
+        for (int i = 0; i < SHRINK_TOK; ++i) {
+            long long a = -1;
+            if (i < ntok)
+                a = p.ids_i64 ? reinterpret_cast<const long long*>(p.ids)[tok0 + i]
+                              : (long long)reinterpret_cast<const int*>(p.ids)[tok0 + i];
+            ids[i] = (a >= 0 && a < p.n_adapters) ? int(a) : -1;
+            tok[i] = tok0 + i;
+        }
     }
     float acc[SHRINK_TOK][SHRINK_RANK];
 #pragma unroll
@@ -381,7 +738,6 @@ adapter_shrink_kernel(const ShrinkParams p) {
 #pragma unroll
         for (int k = 0; k < SHRINK_RANK; ++k) acc[i][k] = 0.0f;
 
-    const T* E = reinterpret_cast<const T*>(p.e);
     const T* A = reinterpret_cast<const T*>(p.lora_a);
     int done = 0;  // bit i: token i is accounted for
 #pragma unroll 1
@@ -408,7 +764,7 @@ adapter_shrink_kernel(const ShrinkParams p) {
 #pragma unroll
             for (int i = 0; i < SHRINK_TOK; ++i) {
                 if (members >> i & 1) {
-                    const uint4 ev = load_piece(E + (size_t)(tok0 + i) * p.lde + d, p.D - d, p.vec != 0);
+                    const uint4 ev = load_piece(E + (size_t)tok[i] * p.lde + d, p.D - d, p.vec != 0);
                     const T* ex = reinterpret_cast<const T*>(&ev);
 #pragma unroll
                     for (int k = 0; k < SHRINK_RANK; ++k) {
@@ -449,7 +805,31 @@ adapter_shrink_kernel(const ShrinkParams p) {
         for (int j = 0; j < SHRINK_TOK; ++j)
             if (j == i) a = ids[j];
         if (a >= 0 && p.scale) sum *= p.scale[a];
-        if (i < ntok && k < p.ldh) p.h[(size_t)(tok0 + i) * p.ldh + k] = (a >= 0 && k < p.rank) ? sum : 0.0f;
+        sum = (a >= 0 && k < p.rank) ? sum : 0.0f;
+        if (i < ntok) {
+            if (k < p.ldh) p.h[(size_t)(tok0 + i) * p.ldh + k] = sum;
+            if constexpr (sizeof(T) == 2) {
+                if (p.h16) {
+                    // |x| up to 2^15: above it, or not finite, and the group goes to the fp32 path
+                    if (!(fabsf(sum) <= 32768.0f)) {
+                        p.group_bad[(tok0 + i) / HEAD_GROUP] = 1;
+                        sum = 0.0f;
+                    }
+                    T* row = reinterpret_cast<T*>(p.h16) + (size_t)(tok0 + i) * h16_pitch(p.rank);
+                    const T hi = T(sum), lo = T(sum - float(hi));
+                    if (p.rank <= 32) {
+                        if (k < 32) {
+                            row[k] = hi;
+                            row[32 + k] = lo;
+                        }
+                    } else {
+                        const int at = k / 64 * 128 + k % 64;
+                        row[at] = hi;
+                        row[at + 64] = lo;
+                    }
+                }
+            }
+        }
     }
 }
 

@@ -100,9 +100,9 @@ def test_c_entry_points_check_their_arguments():
 
     lora = dict(lora_a=ptr, lora_b=ptr, adapter_ids=ptr, n_adapters=2, rank=8)
     assert L.cce_b200_logits_workspace_bytes(logits_args()) > 0
-    # room for one padded fp32 row of inner products per token
+    # room for at least one padded fp32 row of inner products per token
     assert (L.cce_b200_logits_workspace_bytes(logits_args(n_total=1000, n_rows=1000, **lora))
-            - L.cce_b200_logits_workspace_bytes(logits_args(n_total=1000, n_rows=1000))) == 1000 * 16 * 4  # fmt: skip
+            - L.cce_b200_logits_workspace_bytes(logits_args(n_total=1000, n_rows=1000))) >= 1000 * 16 * 4  # fmt: skip
     for kw in (
         dict(e=None), dict(V=0), dict(D=0), dict(lde=15), dict(n_rows=3), dict(out_dtype=3), dict(dtype=7),
         dict(lora_a=ptr), dict(lora, rank=0), dict(lora, rank=257), dict(lora, n_adapters=0),
