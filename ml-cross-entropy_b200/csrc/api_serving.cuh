@@ -37,11 +37,12 @@ LogitsPlan plan_logits(const cce_b200_logits_args* a) {
     if (a->lora_b) {
         // TMA reads the adapters' rows: 16-byte pitch and base
         mma = a->op.dtype != CCE_DT_F32 && a->rank % 8 == 0 && (reinterpret_cast<uintptr_t>(a->lora_b) & 15) == 0;
-        // Columns ordered by adapter need up to 15 more per adapter.  They are free while the product is bound by
-        // reading the classifier (up to 256 columns) and cheaper than mixed groups up to twice the tokens.
-        const long long padded = T + (HEAD_GROUP - 1) * std::min<long long>(T, a->n_adapters + 1);
-        pl.sorted = mma && T > 1 && padded <= std::max<long long>(BN, 2 * T);
-        if (pl.sorted) pl.n_col = cdiv(padded, HEAD_GROUP) * HEAD_GROUP;
+        // Columns ordered by adapter: each run is padded by 0 to 15 columns, about half a group.  They are free while
+        // the product is bound by reading the classifier (up to 256 columns) and cheaper than mixed groups up to
+        // twice the tokens.
+        const long long runs = std::min<long long>(T, a->n_adapters + 1);
+        pl.sorted = mma && T > 1 && a->n_adapters < LAYOUT_MAX_ADAPTERS && T + HEAD_GROUP / 2 * runs <= std::max<long long>(BN, 2 * T);
+        if (pl.sorted) pl.n_col = cdiv(T + (HEAD_GROUP - 1) * runs, HEAD_GROUP) * HEAD_GROUP;  // at most
         pl.n_group = cdiv(pl.n_col, HEAD_GROUP);
     }
     // the status word and, behind it, the flags that are cleared with it
@@ -95,23 +96,27 @@ int launch_behind(K* kernel, dim3 grid, int threads, int smem, cudaStream_t st, 
 
 template <typename T>
 int launch_shrink(const ShrinkParams& sp, long long n_col, cudaStream_t st) {
-    const dim3 grid((unsigned)cdiv(n_col, SHRINK_TOK), (unsigned)(sp.rank_blocks + (sp.col_token ? 1 : 0)));
+    const dim3 grid((unsigned)cdiv(n_col, SHRINK_TOK), (unsigned)(sp.rank_blocks + (sp.col_token ? SHRINK_TOK : 0)));
     return launch_behind(adapter_shrink_kernel<T>, grid, SHRINK_WARPS * 32, 0, st, sp.col_token != nullptr, sp);
+}
+
+// Whether the accumulators are emptied by segments: fp32 logits of a long reduction
+inline bool head_segmented(const HeadParams& hp) {
+    return hp.out_dtype == CCE_DT_F32 && cdiv(hp.n_kblk, HEAD_KSUB) > HEAD_SEGMENT;
 }
 
 // With adapters the projection may start while the shrink kernel, launched just before it, still runs.
 template <typename T>
-int launch_head(const CUtensorMap (&tm)[4], const HeadParams& hp, int grid, cudaStream_t st) {
-    const bool segmented = hp.out_dtype == CCE_DT_F32 && cdiv(hp.n_kblk, HEAD_KSUB) > HEAD_SEGMENT;
-    const auto kernel = !segmented          ? head_logits_kernel<T, 0>
+int launch_head(const HeadMaps& maps, const HeadParams& hp, int grid, cudaStream_t st) {
+    const auto kernel = !head_segmented(hp) ? head_logits_kernel<T, 0>
                         : hp.n_tok <= 64    ? head_logits_kernel<T, 1>
                         : hp.n_tok <= 128   ? head_logits_kernel<T, 2>
-                                            : head_logits_kernel<T, 4>;
-    return launch_behind(kernel, dim3(grid), HEAD_THREADS, HEAD_SMEM, st, hp.lora_b != nullptr, tm[0], tm[1], tm[2],
-                         tm[3], hp);
+                                            : head_logits_kernel<T, 3>;
+    return launch_behind(kernel, dim3(grid), HEAD_THREADS, HEAD_SMEM, st, hp.lora_b != nullptr, maps, hp);
 }
 
-// The adapters' rows of B, [n][V][rank], as a 3-D map: a box of 64 ranks x 128 classifier rows of one adapter.
+// The adapters' rows of B, [n][V][rank], as a 3-D map: a box of 16, 32 or 64 ranks x 128 classifier rows of one
+// adapter, in the swizzle of its width.
 int make_tmap_adapters(CUtensorMap* m, const void* base, int dtype, long long rank, long long V, long long n) {
     EncodeTiledFn enc = get_encode();
     if (!enc) {
@@ -120,11 +125,14 @@ int make_tmap_adapters(CUtensorMap* m, const void* base, int dtype, long long ra
     }
     cuuint64_t dims[3] = {(cuuint64_t)rank, (cuuint64_t)V, (cuuint64_t)n};
     cuuint64_t strides[2] = {(cuuint64_t)rank * 2, (cuuint64_t)(rank * V) * 2};
-    cuuint32_t box[3] = {(cuuint32_t)BK, (cuuint32_t)BM, 1};
+    const int width = AdapterPack((int)rank).a_bytes / (BM * 2);
+    cuuint32_t box[3] = {(cuuint32_t)width, (cuuint32_t)BM, 1};
     cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = enc(m, dtype == CCE_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                      3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     width == 16   ? CU_TENSOR_MAP_SWIZZLE_32B
+                     : width == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                   : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         g_last_cuda = int(r);
@@ -196,7 +204,7 @@ int cce_b200_logits(const cce_b200_logits_args* a, void* workspace, size_t works
         lp.col_token = reinterpret_cast<int*>(ws + pl.off_cols);
         lp.n_col_dev = reinterpret_cast<int*>(ws + pl.off_ncol);
         lp.group = reinterpret_cast<int*>(ws + pl.off_group);
-        adapter_layout_kernel<<<1, LAYOUT_THREADS, 0, st>>>(lp);
+        adapter_layout_kernel<<<1, LAYOUT_THREADS, (a->n_adapters + 1) * sizeof(int), st>>>(lp);
         CCE_LAUNCH_CHECK();
         sg.e = ws + pl.off_e_cols;
         sg.lde = pl.ld_cols;
@@ -240,11 +248,16 @@ int cce_b200_logits(const cce_b200_logits_args* a, void* workspace, size_t works
     hp.n_col = (int)pl.n_col;
     hp.col_token = col_token;
     hp.n_col_dev = n_col_dev;
-    const long long n_ntile = cdiv(pl.n_col, BN);
-    hp.n_tok = (int)(cdiv(cdiv(pl.n_col, n_ntile), HEAD_GROUP) * HEAD_GROUP);  // even shares of the columns
+    hp.out_dtype = a->out_dtype;
+    // A tile of 192 columns is what the registers of the segmented form hold.  Columns that only the device can
+    // count may be far fewer than the bound: there a tile has room for as many as possible.
+    const long long room = head_segmented(hp) ? 192 : BN;
+    const long long n_ntile = cdiv(pl.n_col, room);
+    hp.n_tok = n_ntile > 1 && pl.sorted ? (int)room : (int)(cdiv(cdiv(pl.n_col, n_ntile), HEAD_GROUP) * HEAD_GROUP);
+    hp.e_step = n_ntile > 1 && pl.sorted ? hp.n_tok / 2 / HEAD_E_MAPS : hp.n_tok / 2;
     hp.n_acc = hp.n_tok <= 64 ? HEAD_MAX_ACC : hp.n_tok <= 128 ? HEAD_MAX_ACC / 2 : 2;
     hp.n_vtile = (int)cdiv(op.V, 2 * BM);
-    hp.n_stage = std::min(HEAD_MAX_STAGES, HEAD_RING_BYTES / (HEAD_KSUB * (A_BYTES + hp.n_tok / 2 * BK * 2)));
+    hp.n_stage = std::min(HEAD_MAX_STAGES, HEAD_RING_BYTES / (HEAD_KSUB * (A_BYTES + (int)cdiv(hp.n_tok / 2, hp.e_step) * hp.e_step * BK * 2)));
     const int cdt = compute_dtype(&op);
     hp.idesc = make_idesc(cdt == CCE_DT_BF16 ? 1 : 0, 0, 0, 2 * BM, 0);
     hp.status = reinterpret_cast<int*>(ws);
@@ -252,7 +265,6 @@ int cce_b200_logits(const cce_b200_logits_args* a, void* workspace, size_t works
     hp.has_softcap = op.has_softcap;
     hp.softcap = op.softcap;
     hp.out = a->out;
-    hp.out_dtype = a->out_dtype;
     if (a->lora_b) {
         hp.lora_b = a->lora_b;
         hp.ids = a->adapter_ids;
@@ -265,24 +277,32 @@ int cce_b200_logits(const cce_b200_logits_args* a, void* workspace, size_t works
         hp.group = reinterpret_cast<const int*>(ws + pl.off_group);
         hp.group_bad = reinterpret_cast<const int*>(ws + pl.off_bad);
     }
-    CUtensorMap tm[4];  // classifier, tokens, adapters' B, h
-    rc = make_tmap(&tm[0], sg.c, cdt, sg.Dk, op.V, sg.ldc, BK, BM);
+    HeadMaps maps;
+    rc = make_tmap(&maps.c, sg.c, cdt, sg.Dk, op.V, sg.ldc, BK, BM);
     if (rc) return rc;
-    rc = make_tmap(&tm[1], sg.e, cdt, sg.Dk, pl.n_col, sg.lde, BK, hp.n_tok / 2);
-    if (rc) return rc;
-    tm[2] = tm[3] = tm[1];
-    if (pl.pitch16) {
-        rc = make_tmap_adapters(&tm[2], a->lora_b, cdt, a->rank, op.V, a->n_adapters);
+    for (int i = 0; i < HEAD_E_MAPS; ++i) {
+        if (i > 0 && hp.e_step == hp.n_tok / 2) {
+            maps.e[i] = maps.e[0];
+            continue;
+        }
+        rc = make_tmap(&maps.e[i], sg.e, cdt, sg.Dk, pl.n_col, sg.lde, BK, (i + 1) * hp.e_step);
         if (rc) return rc;
-        rc = make_tmap(&tm[3], ws + pl.off_h16, cdt, pl.pitch16, pl.n_col, pl.pitch16, BK, 8);
+    }
+    maps.b = maps.h8 = maps.h32 = maps.c;
+    if (pl.pitch16) {
+        rc = make_tmap_adapters(&maps.b, a->lora_b, cdt, a->rank, op.V, a->n_adapters);
+        if (rc) return rc;
+        rc = make_tmap(&maps.h8, ws + pl.off_h16, cdt, pl.pitch16, pl.n_col, pl.pitch16, BK, 8);
+        if (rc) return rc;
+        rc = make_tmap(&maps.h32, ws + pl.off_h16, cdt, pl.pitch16, pl.n_col, pl.pitch16, BK, 32);
         if (rc) return rc;
     }
     const long long n_items = (long long)hp.n_vtile * n_ntile;
     if (n_items >= (1LL << 30)) return CCE_ERR_ARG;
     const int grid = 2 * (int)std::min<long long>(dev->sms / 2, n_items);
-    if (op.dtype == CCE_DT_F32) return launch_head<float>(tm, hp, grid, st);
-    if (op.dtype == CCE_DT_BF16) return launch_head<__nv_bfloat16>(tm, hp, grid, st);
-    return launch_head<__half>(tm, hp, grid, st);
+    if (op.dtype == CCE_DT_F32) return launch_head<float>(maps, hp, grid, st);
+    if (op.dtype == CCE_DT_BF16) return launch_head<__nv_bfloat16>(maps, hp, grid, st);
+    return launch_head<__half>(maps, hp, grid, st);
 }
 
 int cce_b200_sample(const cce_b200_sample_args* a, void* stream) {

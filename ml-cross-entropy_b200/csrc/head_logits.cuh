@@ -34,7 +34,7 @@ constexpr int HEAD_THREADS = 64 + 32 * HEAD_EPI_WARPS;
 constexpr int HEAD_KSUB = 2;                   // 64-element K sub-blocks per ring stage
 constexpr int HEAD_MAX_STAGES = 8;
 constexpr int HEAD_SMEM = 227 * 1024;          // everything: the ring decides how many bytes are in flight
-constexpr int HEAD_RING_BYTES = HEAD_SMEM - 1024 /*align slack*/ - 512 /*barriers*/;
+constexpr int HEAD_RING_BYTES = HEAD_SMEM - 1024 /*align slack*/ - 1024 /*barriers, runs*/;
 constexpr int HEAD_GROUP = 16;                 // tokens that share one decision about their adapters
 constexpr int ADAPTER_RANK_PAD = 16;           // fp32 rows of h are padded to this many ranks with zeros
 constexpr int GROUP_NONE = -1, GROUP_MIXED = -2;
@@ -42,7 +42,7 @@ constexpr int HEAD_MAX_ACC = 8;
 // fp32 logits: the tensor core truncates every addition, so a sum over all of D drifts (2.4e-6 of the logits'
 // norm at D = 2304).  The accumulator is therefore emptied every HEAD_SEGMENT stages into fp32 registers,
 // which add with rounding (2e-7).  16-bit logits are rounded far above the drift and take the sum in one piece.
-constexpr int HEAD_SEGMENT = 2;
+constexpr int HEAD_SEGMENT = 4;
 
 struct HeadParams {
     int T, V;          // tokens, classifier rows
@@ -51,6 +51,7 @@ struct HeadParams {
     int n_col;         // columns: T, or with col_token an upper bound of *n_col_dev
     int n_vtile;       // classifier tiles of 256 rows
     int n_stage;
+    int e_step;        // the token maps' boxes have e_step, 2 e_step, .. rows; the smallest that holds half a tile is used
     int n_acc;         // accumulators in TMEM: 512 columns in n_acc parts of at least n_tok
     const int* col_token;  // null (column = token), or [n_col]: the token of every column, -1 for padding
     const int* n_col_dev;
@@ -72,6 +73,14 @@ struct HeadParams {
     int ldh;
     const int* group;    // [ceil(columns / 16)]: the adapter of a group, GROUP_NONE or GROUP_MIXED
     const int* group_bad;  // likewise; non-zero: h does not fit the 16-bit type, treat as mixed
+};
+
+constexpr int HEAD_E_MAPS = 4;
+struct HeadMaps {
+    CUtensorMap c;               // classifier: 64 x 128 rows
+    CUtensorMap e[HEAD_E_MAPS];  // tokens: 64 x (i + 1) e_step rows
+    CUtensorMap b;               // adapters' B
+    CUtensorMap h8, h32;         // 16-bit h: 64 x 8 and 64 x 32 rows
 };
 
 // The column tiles of a launch, from the number of columns that the device knows.
@@ -99,23 +108,70 @@ __device__ __forceinline__ int group_adapter(const HeadParams& p, int g) {
     return a >= 0 && p.group_bad[g] ? GROUP_MIXED : a;
 }
 
-// The runs of neighbouring groups of a column tile that share an adapter: f(adapter, first column, columns) for each.
-// The producers of both CTAs and the MMA issuer call this and see the same sequence.  f returns false to stop.
-template <typename F>
-__device__ __forceinline__ bool walk_runs(const HeadParams& p, const HeadTiles& tiles, int col0, F f) {
+// A run of neighbouring groups of a column tile that share an adapter.
+struct Run {
+    int adapter;
+    short first, cols;  // within the tile
+};
+constexpr int HEAD_MAX_RUNS = BN / HEAD_GROUP;
+
+// The runs of the tile that starts at column col0, found by a whole warp (one group per lane) and left in shared
+// memory; returns their number.  The producers of both CTAs and the MMA issuer find the same.
+__device__ __forceinline__ int find_runs(const HeadParams& p, const HeadTiles& tiles, int col0, Run* runs) {
+    const int lane = threadIdx.x & 31;
     const int g0 = col0 / HEAD_GROUP;
-    const int g1 = (min(tiles.n_col, col0 + tiles.n_tok) + HEAD_GROUP - 1) / HEAD_GROUP;
-    int a = GROUP_NONE, first = g0;
-    for (int g = g0; g <= g1; ++g) {
-        const int b = g < g1 ? group_adapter(p, g) : GROUP_NONE;
-        if (g == g1 || b != a) {
-            if (a >= 0 && !f(a, (first - g0) * HEAD_GROUP, (g - first) * HEAD_GROUP)) return false;
-            a = b;
-            first = g;
-        }
+    const int n = (min(tiles.n_col, col0 + tiles.n_tok) + HEAD_GROUP - 1) / HEAD_GROUP - g0;  // at most 16
+    const int a = lane < n ? group_adapter(p, g0 + lane) : GROUP_NONE;
+    const int before = __shfl_up_sync(0xffffffffu, a, 1);
+    const bool change = lane == 0 || before != a || lane == n;
+    const unsigned changes = __ballot_sync(0xffffffffu, change);
+    const bool start = change && a >= 0;
+    const unsigned starts = __ballot_sync(0xffffffffu, start);
+    __syncwarp();
+    if (start) {
+        const int end = __ffs(changes & ~((2u << lane) - 1)) - 1;  // there is one: lane n
+        runs[__popc(starts & ((1u << lane) - 1))] = Run{a, short(lane * HEAD_GROUP), short((end - lane) * HEAD_GROUP)};
     }
-    return true;
+    __syncwarp();
+    return __popc(starts);
 }
+
+// How the adapters' second product uses the ring: an entry is one run x up to 64 ranks; its rows of B take
+// 128 x (32, 64 or 128) bytes, in the swizzle of that width, so that 8, 4 or 2 entries share a stage.
+struct AdapterPack {
+    int a_bytes, max_entries;
+    uint32_t layout, sbo;  // of the descriptor: swizzle type, distance of 8-row groups
+    __host__ __device__ explicit AdapterPack(int rank) {
+        const int width = rank <= 16 ? 16 : rank <= 32 ? 32 : 64;
+        a_bytes = BM * width * 2;
+        max_entries = HEAD_KSUB * A_BYTES / a_bytes;
+        layout = width == 16 ? 6 : width == 32 ? 4 : 2;
+        sbo = 8 * width * 2;
+    }
+    // open() begins a stage, entry(i, row, run, r0) is its i-th entry with its columns' rows of h from `row` on (of this
+    // CTA's half), close() ends it; open returns false to stop.
+    template <typename Open, typename Entry, typename Close>
+    __device__ __forceinline__ bool walk(const Run* runs, int n_runs, int rank, int rows, Open open, Entry entry,
+                                         Close close) const {
+        int i = 0, row = 0;
+        for (int k = 0; k < n_runs; ++k) {
+            const Run run = runs[k];
+            const int half = run.cols / 2;
+            for (int r0 = 0; r0 < rank; r0 += BK) {
+                if (i > 0 && (i == max_entries || row + half > rows)) {
+                    close();
+                    i = row = 0;
+                }
+                if (i == 0 && !open()) return false;
+                entry(i, row, run, r0);
+                ++i;
+                row += half;
+            }
+        }
+        if (i > 0) close();
+        return true;
+    }
+};
 
 // 16 consecutive values of a row of B (ranks k0 .. k0+15 of `rank`; zeros past it), as they are stored
 template <typename T, bool VEC>
@@ -150,24 +206,35 @@ template <typename T, bool VEC>
 __device__ __noinline__ void add_adapters(const HeadParams& p, int v, int col0, int n_col, int my_id, int lane0,
                                           float* x) {
     const T* B = reinterpret_cast<const T*>(p.lora_b);
-    for (int k0 = 0; k0 < p.rank; k0 += ADAPTER_RANK_PAD) {
-#pragma unroll 8
-        for (int j = 0; j < HEAD_GROUP; ++j) {
-            const int a = __shfl_sync(0xffffffffu, my_id, lane0 + j);
-            BRow<T, VEC> b;
-            b.load(B + ((size_t)max(a, 0) * p.V + v) * p.rank, k0, p.rank);
-            const float4* hp = reinterpret_cast<const float4*>(p.h + (size_t)min(col0 + j, n_col - 1) * p.ldh + k0);
-            float s = 0.0f;
+    constexpr int U = 8;  // tokens at a time; their sums wait in registers, so that no store stands between the loads
+    for (int j0 = 0; j0 < HEAD_GROUP; j0 += U) {
+        int a[U];
+        float s[U];
 #pragma unroll
-            for (int q = 0; q < ADAPTER_RANK_PAD / 4; ++q) {
-                const float4 hv = hp[q];
-                s = fmaf(to_float(b.x[4 * q]), hv.x, s);
-                s = fmaf(to_float(b.x[4 * q + 1]), hv.y, s);
-                s = fmaf(to_float(b.x[4 * q + 2]), hv.z, s);
-                s = fmaf(to_float(b.x[4 * q + 3]), hv.w, s);
-            }
-            if (a >= 0) x[j] += s;
+        for (int j = 0; j < U; ++j) {
+            a[j] = __shfl_sync(0xffffffffu, my_id, lane0 + j0 + j);
+            s[j] = 0.0f;
         }
+        for (int k0 = 0; k0 < p.rank; k0 += ADAPTER_RANK_PAD) {
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                BRow<T, VEC> b;
+                b.load(B + ((size_t)max(a[j], 0) * p.V + v) * p.rank, k0, p.rank);
+                const float4* hp =
+                    reinterpret_cast<const float4*>(p.h + (size_t)min(col0 + j0 + j, n_col - 1) * p.ldh + k0);
+#pragma unroll
+                for (int q = 0; q < ADAPTER_RANK_PAD / 4; ++q) {
+                    const float4 hv = hp[q];
+                    s[j] = fmaf(to_float(b.x[4 * q]), hv.x, s[j]);
+                    s[j] = fmaf(to_float(b.x[4 * q + 1]), hv.y, s[j]);
+                    s[j] = fmaf(to_float(b.x[4 * q + 2]), hv.z, s[j]);
+                    s[j] = fmaf(to_float(b.x[4 * q + 3]), hv.w, s[j]);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+            if (a[j] >= 0) x[j0 + j] += s[j];
     }
 }
 
@@ -191,18 +258,18 @@ __device__ __forceinline__ void store_chunk(const HeadParams& p, int v, int my_t
     }
 }
 
-// bias, mixed groups, soft-cap and store of one chunk of 32 columns; v is this lane's classifier row
+// bias, mixed groups (bits 0 and 1 of `mixed`: the chunk's two), soft-cap and store of one chunk of 32 columns; v is
+// this lane's classifier row
 template <typename BT>
 __device__ __forceinline__ void finish_chunk(const HeadParams& p, const HeadTiles& tiles, int v, float bias, int c0,
-                                             int col_end, float (&x)[32]) {
+                                             int col_end, unsigned mixed, float (&x)[32]) {
     const int lane = threadIdx.x & 31;
     const int ncol = min(32, col_end - c0);
     const int my_token = lane < ncol ? (p.col_token ? p.col_token[c0 + lane] : c0 + lane) : -1;
 #pragma unroll
     for (int j = 0; j < 32; ++j) x[j] += bias;
-    if (p.lora_b) {
-        const bool m0 = group_adapter(p, c0 / HEAD_GROUP) == GROUP_MIXED;
-        const bool m1 = ncol > HEAD_GROUP && group_adapter(p, c0 / HEAD_GROUP + 1) == GROUP_MIXED;
+    {
+        const bool m0 = mixed & 1, m1 = mixed & 2;
         if (m0 || m1) {  // uniform over the warp
             const int my_id = my_token >= 0 ? adapter_of(p, my_token) : -1;
             const int row = min(v, p.V - 1);
@@ -239,17 +306,18 @@ struct HeadSmem {
     uint64_t *full, *empty, *tfull, *tempty, *tdown;
     uint32_t* tmem_base;
     volatile int* abort_flag;
+    Run* runs;  // [2][HEAD_MAX_RUNS]: producer, MMA issuer
 };
 
 // BT: element type of the adapters (and of e).  CHUNKS > 0: the accumulator is emptied every HEAD_SEGMENT stages
 // into the epilogue's registers, CHUNKS chunks of 32 columns per warp (tiles of up to 64 CHUNKS columns); 0: it is not.
 template <typename BT, int CHUNKS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HEAD_THREADS, 1)
-head_logits_kernel(const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmE,
-                   const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmH, const __grid_constant__ HeadParams p) {
+head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant__ HeadParams p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const uint32_t sub_e = p.n_tok / 2 * BK * 2;  // this CTA's half of the tokens x 64 reduction elements
+    // room for this CTA's half of the tokens x 64 reduction elements
+    const uint32_t sub_e = (p.n_tok / 2 + p.e_step - 1) / p.e_step * p.e_step * BK * 2;
     const uint32_t off_e = HEAD_KSUB * A_BYTES;   // of a stage: the token operand
     const uint32_t stage_bytes = off_e + HEAD_KSUB * sub_e;
     HeadSmem s;
@@ -262,6 +330,7 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmC, const __grid_constan
     s.tdown = s.tempty + HEAD_MAX_ACC;
     s.tmem_base = reinterpret_cast<uint32_t*>(s.tdown + 1);
     s.abort_flag = reinterpret_cast<int*>(s.tmem_base + 1);
+    s.runs = reinterpret_cast<Run*>(base + HEAD_RING_BYTES + 512);
 
     constexpr bool SEGMENTED = CHUNKS > 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -282,8 +351,7 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmC, const __grid_constan
         *s.abort_flag = 0;
         fence_barrier_init();
         fence_proxy_async();
-        tma_prefetch_desc(&tmC);
-        tma_prefetch_desc(&tmE);
+        tma_prefetch_desc(&maps.c);
     }
     if (warp == 1) {
         tmem_alloc_pair(smem_u32(s.tmem_base), TMEM_COLS);
@@ -296,8 +364,9 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmC, const __grid_constan
     tc_fence_after();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(s.tmem_base);
 
+    const AdapterPack pack(p.rank);
     if (warp == 0) {
-        if (lane == 0) {
+        {
             int stage = 0;
             uint32_t phase = 0;
             auto free_stage = [&]() -> bool {
@@ -317,21 +386,20 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmC, const __grid_constan
                 const uint32_t bar = map_to_cta(smem_u32(&s.full[stage]), 0);
                 const uint32_t sa = smem_u32(s.stages) + stage * stage_bytes;
                 for (int j = 0; j < sub_blocks(ks); ++j)
-                    tma_load_2d_pair(sa + j * A_BYTES, &tmC, bar, (ks * HEAD_KSUB + j) * BK, row);
+                    tma_load_2d_pair(sa + j * A_BYTES, &maps.c, bar, (ks * HEAD_KSUB + j) * BK, row);
             };
-            auto load_e = [&](int ks, int row) {
+            auto load_e = [&](int ks, int row, const CUtensorMap* map) {
                 const uint32_t bar = map_to_cta(smem_u32(&s.full[stage]), 0);
                 const uint32_t sb = smem_u32(s.stages) + stage * stage_bytes + off_e;
                 for (int j = 0; j < sub_blocks(ks); ++j)
-                    tma_load_2d_pair(sb + j * sub_e, &tmE, bar, (ks * HEAD_KSUB + j) * BK, row);
+                    tma_load_2d_pair(sb + j * sub_e, map, bar, (ks * HEAD_KSUB + j) * BK, row);
             };
             // The first tile's classifier rows are known before the columns are, if there is one column tile: a
             // ring of them is requested before the wait for the kernels that order the columns.
             int ahead = 0;
-            if (p.lora_b && p.n_col <= p.n_tok) {
+            if (p.lora_b && p.n_col <= p.n_tok && lane == 0) {
                 ahead = min(p.n_stage, n_kstage);
                 for (int ks = 0; ks < ahead; ++ks) {
-                    open_stage(sub_blocks(ks) * (A_BYTES + sub_e));
                     load_c(ks, pair * 2 * BM + rank * BM);
                     next_stage();
                 }
@@ -341,119 +409,138 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmC, const __grid_constan
             if (p.lora_b) pdl_wait();
             const HeadTiles tiles(p);
             const int n_items = p.n_vtile * tiles.n_ntile;
+            const int size = (tiles.n_tok / 2 + p.e_step - 1) / p.e_step;  // of the token loads, in steps
+            const CUtensorMap* map_e = &maps.e[size - 1];
+            const uint32_t e_bytes = size * p.e_step * BK * 2;
             bool ok = true;
-            for (int item = pair; ok && item < n_items; item += n_pairs) {
+            for (int item = pair; item < n_items; item += n_pairs) {
                 const int row_c = (item / tiles.n_ntile) * 2 * BM + rank * BM;
                 const int col0 = (item % tiles.n_ntile) * tiles.n_tok;
                 const int row_e = col0 + rank * (tiles.n_tok / 2);
-                for (int ks = 0; ok && ks < n_kstage; ++ks) {
-                    if (ks >= ahead) {
-                        ok = free_stage();
-                        if (!ok) break;
-                        open_stage(sub_blocks(ks) * (A_BYTES + sub_e));
-                        load_c(ks, row_c);
-                    }
-                    load_e(ks, row_e);
-                    next_stage();
-                }
-                ahead = 0;
-                if (!ok || !p.lora_b) continue;
-                ok = walk_runs(p, tiles, col0, [&](int a, int run0, int ncol) -> bool {
-                    const int half = ncol / 2;  // rows of h that this CTA supplies: a multiple of 8
-                    const int terms = p.rank <= 32 ? 1 : 2;
-                    for (int r0 = 0; r0 < p.rank; r0 += BK) {
-                        if (!free_stage()) return false;
-                        open_stage(A_BYTES + terms * half * BK * 2);
-                        const uint32_t bar = map_to_cta(smem_u32(&s.full[stage]), 0);
-                        const uint32_t sa = smem_u32(s.stages) + stage * stage_bytes;
-                        tma_load_3d_pair(sa, &tmB, bar, r0, row_c, a);
-                        for (int i = 0; i < terms; ++i)
-                            for (int y = 0; y < half; y += 8)
-                                tma_load_2d_pair(sa + off_e + i * sub_e + y * BK * 2, &tmH, bar, r0 * 2 + i * BK,
-                                                 col0 + run0 + rank * half + y);
+                const int n_runs = p.lora_b ? find_runs(p, tiles, col0, s.runs) : 0;
+                if (lane == 0) {  // one lane runs the loop over the stages
+                    for (int ks = 0; ok && ks < n_kstage; ++ks) {
+                        if (ks >= ahead) {
+                            ok = free_stage();
+                            if (!ok) break;
+                        }
+                        open_stage(sub_blocks(ks) * (A_BYTES + e_bytes));
+                        if (ks >= ahead) load_c(ks, row_c);
+                        load_e(ks, row_e, map_e);
                         next_stage();
                     }
-                    return true;
-                });
+                    ahead = 0;
+                    uint32_t bytes = 0;  // announced when the stage is complete: the loads may land before that
+                    ok = ok && pack.walk(
+                        s.runs, n_runs, p.rank, p.n_tok / 2,
+                        [&]() -> bool {
+                            bytes = 0;
+                            return free_stage();
+                        },
+                        [&](int i, int row, const Run& run, int r0) {
+                            const uint32_t bar = map_to_cta(smem_u32(&s.full[stage]), 0);
+                            const uint32_t sa = smem_u32(s.stages) + stage * stage_bytes;
+                            const int half = run.cols / 2;  // rows of h that this CTA supplies: a multiple of 8
+                            const int terms = p.rank <= 32 ? 1 : 2;
+                            tma_load_3d_pair(sa + i * pack.a_bytes, &maps.b, bar, r0, row_c, run.adapter);
+                            for (int t = 0; t < terms; ++t)
+                                for (int y = 0; y < half;) {  // few and large loads: each costs its issue
+                                    const bool large = half - y >= 32;
+                                    tma_load_2d_pair(sa + off_e + t * sub_e + (row + y) * BK * 2,
+                                                     large ? &maps.h32 : &maps.h8, bar, r0 * 2 + t * BK,
+                                                     col0 + run.first + rank * half + y);
+                                    y += large ? 32 : 8;
+                                }
+                            bytes += pack.a_bytes + terms * half * BK * 2;
+                        },
+                        [&]() {
+                            open_stage(bytes);
+                            next_stage();
+                        });
+                }
+                if (!__shfl_sync(0xffffffffu, int(ok), 0)) break;
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
             const uint64_t adesc0 = make_smem_desc(smem_u32(s.stages), 16, 1024);
             const uint32_t empty0 = smem_u32(s.empty), empty1 = map_to_cta(empty0, 1);
             const uint32_t tfull0 = smem_u32(s.tfull), tfull1 = map_to_cta(tfull0, 1);
-            // A filled stage, `issue(descriptor A, descriptor B)`, and the stage's release in both CTAs.
-            auto use = [&](auto issue) -> bool {
+            auto filled_stage = [&]() -> bool {
                 if (!mbar_wait(smem_u32(&s.full[stage]), phase, s.abort_flag, p.status, ERR_WAIT_SMEM_FULL)) return false;
                 tc_fence_after();
-                // the address field of a descriptor counts 16-byte units
-                const uint64_t ad = adesc0 + ((stage * stage_bytes) >> 4);
-                issue(ad, ad + (off_e >> 4));
+                return true;
+            };
+            auto release_stage = [&]() {  // in both CTAs, once the MMAs issued so far have read it
                 tc_commit_pair(empty0 + 8 * stage);
                 tc_commit_pair(empty1 + 8 * stage);
                 if (++stage == p.n_stage) {
                     stage = 0;
                     phase ^= 1u;
                 }
-                return true;
             };
-            constexpr int STEP = UMMA_K * 2 >> 4;  // descriptor units per MMA step
+            constexpr int STEP = UMMA_K * 2 >> 4;  // descriptor units (16 bytes) per MMA step
             if (p.lora_b) pdl_wait();
             const HeadTiles tiles(p);
             const int n_items = p.n_vtile * tiles.n_ntile;
             const uint32_t idesc = p.idesc | (uint32_t(tiles.n_tok >> 3) << 17);
+            Run* runs = s.runs + HEAD_MAX_RUNS;
             bool ok = true;
-            for (int item = pair; ok && item < n_items; item += n_pairs) {
-                uint32_t d_tmem = 0;
-                for (int ks = 0; ok && ks < n_kstage; ++ks) {
-                    const bool opens = SEGMENTED ? ks % HEAD_SEGMENT == 0 : ks == 0;
-                    if (opens) {
-                        ok = mbar_wait(smem_u32(&s.tempty[acc]), acc_phase ^ 1u, s.abort_flag, p.status,
-                                       ERR_WAIT_TMEM_EMPTY);
+            for (int item = pair; item < n_items; item += n_pairs) {
+                const int n_runs = p.lora_b ? find_runs(p, tiles, (item % tiles.n_ntile) * tiles.n_tok, runs) : 0;
+                if (lane == 0) {  // one lane issues
+                    uint32_t d_tmem = 0;
+                    for (int ks = 0; ok && ks < n_kstage; ++ks) {
+                        const bool opens = SEGMENTED ? ks % HEAD_SEGMENT == 0 : ks == 0, last = ks + 1 == n_kstage;
+                        if (opens) {
+                            ok = mbar_wait(smem_u32(&s.tempty[acc]), acc_phase ^ 1u, s.abort_flag, p.status,
+                                           ERR_WAIT_TMEM_EMPTY);
+                            if (!ok) break;
+                            tc_fence_after();
+                            d_tmem = tmem_base + acc * acc_cols;
+                        }
+                        ok = filled_stage();
                         if (!ok) break;
-                        tc_fence_after();
-                        d_tmem = tmem_base + acc * acc_cols;
-                    }
-                    const int n = min(HEAD_KSUB, p.n_kblk - ks * HEAD_KSUB);
-                    ok = use([&](uint64_t ad, uint64_t bd) {
+                        const int n = min(HEAD_KSUB, p.n_kblk - ks * HEAD_KSUB);
+                        const uint64_t ad = adesc0 + ((stage * stage_bytes) >> 4), bd = ad + (off_e >> 4);
                         for (int j = 0; j < n; ++j)
 #pragma unroll
                             for (int k = 0; k < BK / UMMA_K; ++k)
-                                tc_mma_f16_pair(d_tmem, ad + j * (A_BYTES >> 4) + k * STEP,
-                                                bd + j * (sub_e >> 4) + k * STEP, idesc, (!opens || j || k) ? 1u : 0u);
-                    });
-                    if (!ok) break;
-                    const bool last = ks + 1 == n_kstage;
-                    if (last && p.lora_b) {
-                        const int tile0 = (item % tiles.n_ntile) * tiles.n_tok;
-                        ok = walk_runs(p, tiles, tile0, [&](int, int run0, int ncol) -> bool {
-                            const uint32_t run_idesc = p.idesc | (uint32_t(ncol >> 3) << 17);
-                            const uint32_t lo = p.rank <= 32 ? 2 * STEP : sub_e >> 4;  // from the hi to the lo terms
-                            for (int r0 = 0; r0 < p.rank; r0 += BK) {
-                                const int steps = (min(BK, p.rank - r0) + UMMA_K - 1) / UMMA_K;
-                                if (!use([&](uint64_t ad, uint64_t bd) {
-                                        for (int k = 0; k < steps; ++k) {
-                                            tc_mma_f16_pair(d_tmem + run0, ad + k * STEP, bd + k * STEP, run_idesc, 1u);
-                                            tc_mma_f16_pair(d_tmem + run0, ad + k * STEP, bd + lo + k * STEP, run_idesc, 1u);
-                                        }
-                                    }))
-                                    return false;
+                                tc_mma_f16_pair(d_tmem, ad + j * (A_BYTES >> 4) + k * STEP, bd + j * (sub_e >> 4) + k * STEP,
+                                                idesc, (!opens || j || k) ? 1u : 0u);
+                        release_stage();
+                        if (last) {
+                            ok = pack.walk(
+                                runs, n_runs, p.rank, p.n_tok / 2, filled_stage,
+                                [&](int i, int row, const Run& run, int r0) {
+                                    const uint32_t run_idesc = p.idesc | (uint32_t(run.cols >> 3) << 17);
+                                    const uint32_t lo = p.rank <= 32 ? 2 * STEP : sub_e >> 4;  // from the hi to the lo terms
+                                    const uint32_t sa = smem_u32(s.stages) + stage * stage_bytes;
+                                    const uint64_t rad = (make_smem_desc(sa + i * pack.a_bytes, 16, pack.sbo) &
+                                                          ~(uint64_t(7) << 61)) | uint64_t(pack.layout) << 61;
+                                    const uint64_t rbd = make_smem_desc(sa + off_e + row * BK * 2, 16, 1024);
+                                    const int steps = (min(BK, p.rank - r0) + UMMA_K - 1) / UMMA_K;
+                                    for (int k = 0; k < steps; ++k) {
+                                        tc_mma_f16_pair(d_tmem + run.first, rad + k * STEP, rbd + k * STEP, run_idesc, 1u);
+                                        tc_mma_f16_pair(d_tmem + run.first, rad + k * STEP, rbd + lo + k * STEP, run_idesc, 1u);
+                                    }
+                                },
+                                release_stage);
+                            if (!ok) break;
+                        }
+                        if (last || (SEGMENTED && (ks + 1) % HEAD_SEGMENT == 0)) {
+                            tc_commit_pair(tfull0 + 8 * acc);
+                            tc_commit_pair(tfull1 + 8 * acc);
+                            if (++acc == p.n_acc) {
+                                acc = 0;
+                                acc_phase ^= 1u;
                             }
-                            return true;
-                        });
-                        if (!ok) break;
-                    }
-                    if (last || (SEGMENTED && (ks + 1) % HEAD_SEGMENT == 0)) {
-                        tc_commit_pair(tfull0 + 8 * acc);
-                        tc_commit_pair(tfull1 + 8 * acc);
-                        if (++acc == p.n_acc) {
-                            acc = 0;
-                            acc_phase ^= 1u;
                         }
                     }
                 }
+                if (!__shfl_sync(0xffffffffu, int(ok), 0)) break;
             }
         }
     } else {
@@ -472,6 +559,9 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmC, const __grid_constan
             const int col0 = (item % tiles.n_ntile) * tiles.n_tok;
             const int col_end = min(tiles.n_col, col0 + tiles.n_tok);
             const float bias = (p.bias && v < p.V) ? __ldg(p.bias + v) : 0.0f;
+            // bit g: group g of the tile is mixed
+            const unsigned mixed = __ballot_sync(0xffffffffu, p.lora_b && lane < HEAD_MAX_RUNS && col0 + lane * HEAD_GROUP < col_end &&
+                                                                  group_adapter(p, col0 / HEAD_GROUP + lane) == GROUP_MIXED);
             float sum[SEGMENTED ? CHUNKS : 1][32];
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c)
@@ -509,12 +599,12 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmC, const __grid_constan
                         }
 #pragma unroll
                         for (int j = 0; j < 32; ++j) x[j] = ok ? __uint_as_float(r[j]) : __int_as_float(0x7fc00000);
-                        finish_chunk<BT>(p, tiles, v, bias, c0, col_end, x);
+                        finish_chunk<BT>(p, tiles, v, bias, c0, col_end, mixed >> ((c0 - col0) / HEAD_GROUP), x);
                     }
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (ok && lane == 0) mbar_arrive_cluster(tempty0 + 8 * acc);
+                if (ok && lane == 0) mbar_arrive_cluster_relaxed(tempty0 + 8 * acc);
                 if (++acc == p.n_acc) {
                     acc = 0;
                     acc_phase ^= 1u;
@@ -533,7 +623,7 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmC, const __grid_constan
                         for (int i = 1; i < CHUNKS; ++i) s_c = c == i ? sum[i][j] : s_c;
                         x[j] = ok ? s_c : __int_as_float(0x7fc00000);
                     }
-                    finish_chunk<BT>(p, tiles, v, bias, c0, col_end, x);
+                    finish_chunk<BT>(p, tiles, v, bias, c0, col_end, mixed >> ((c0 - col0) / HEAD_GROUP), x);
                 }
             }
         }
@@ -559,10 +649,10 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmC, const __grid_constan
 }
 
 // The columns in order of their adapter: column runs of one adapter each, padded to whole groups of 16, tokens
-// without an adapter last.  One block; thread a walks all ids and places the tokens of adapters a, a + 1024, ...
-// (T steps: 0.3 us at 32 tokens, small beside the projection at thousands), so that the order is that of the tokens.
+// without an adapter last; within a run in order of the tokens.  One block: counts, starts, and then the tokens
+// 1024 at a time, the warps one after the other, so that a token's place is the number of those before it.
 constexpr int LAYOUT_THREADS = 1024;
-constexpr int LAYOUT_CHUNK = 4096;  // ids in shared memory at a time
+constexpr int LAYOUT_MAX_ADAPTERS = 8192;  // their places are in shared memory
 
 struct LayoutParams {
     const void* ids;
@@ -575,43 +665,27 @@ struct LayoutParams {
 
 __global__ void __launch_bounds__(LAYOUT_THREADS)
 adapter_layout_kernel(const LayoutParams p) {
-    __shared__ __align__(16) int ids[LAYOUT_CHUNK];
+    extern __shared__ int place[];  // [n_adapters + 1]: counts, then the next free column of every run
     __shared__ int warp_sum[32];
     __shared__ int base;
     pdl_launch();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // f(token, id) for every token in order, in the warps that have an adapter; the ids pass through shared memory
-    auto each = [&](bool active, auto f) {
-        for (int t0 = 0; t0 < p.T; t0 += LAYOUT_CHUNK) {
-            const int n = min(LAYOUT_CHUNK, p.T - t0);
-            __syncthreads();
-            for (int i = tid; i < (n + 3) / 4 * 4; i += LAYOUT_THREADS) {
-                if (i >= n) {
-                    ids[i] = -1;  // no thread's adapter
-                    continue;
-                }
-                const long long a = p.ids_i64 ? reinterpret_cast<const long long*>(p.ids)[t0 + i]
-                                              : (long long)reinterpret_cast<const int*>(p.ids)[t0 + i];
-                ids[i] = (a >= 0 && a < p.n_adapters) ? int(a) : p.n_adapters;
-            }
-            __syncthreads();
-            if (!active) continue;
-            for (int i = 0; i < n; i += 4) {
-                const int4 q = *reinterpret_cast<const int4*>(ids + i);
-                f(t0 + i, q.x);
-                f(t0 + i + 1, q.y);
-                f(t0 + i + 2, q.z);
-                f(t0 + i + 3, q.w);
-            }
-        }
+    const int n = p.n_adapters + 1;
+    auto id_of = [&](int t) -> int {
+        const long long a = p.ids_i64 ? reinterpret_cast<const long long*>(p.ids)[t]
+                                      : (long long)reinterpret_cast<const int*>(p.ids)[t];
+        return (a >= 0 && a < p.n_adapters) ? int(a) : p.n_adapters;
     };
+    for (int a = tid; a < n; a += LAYOUT_THREADS) place[a] = 0;
     if (tid == 0) base = 0;
-    for (int a0 = 0; a0 <= p.n_adapters; a0 += LAYOUT_THREADS) {
+    __syncthreads();
+    const int first_id = tid < p.T ? id_of(tid) : 0;
+    for (int t = tid; t < p.T; t += LAYOUT_THREADS) atomicAdd(&place[t == tid ? first_id : id_of(t)], 1);
+    __syncthreads();
+    for (int a0 = 0; a0 < n; a0 += LAYOUT_THREADS) {  // starts, and the padding behind every run
         const int a = a0 + tid;
-        const bool active = a0 + warp * 32 <= p.n_adapters;
-        int count = 0;
-        each(active, [&](int, int id) { count += id == a; });
-        const int padded = a <= p.n_adapters ? (count + HEAD_GROUP - 1) / HEAD_GROUP * HEAD_GROUP : 0;
+        const int count = a < n ? place[a] : 0;
+        const int padded = (count + HEAD_GROUP - 1) / HEAD_GROUP * HEAD_GROUP;
         int incl = padded;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -622,23 +696,41 @@ adapter_layout_kernel(const LayoutParams p) {
         __syncthreads();
         int first = base + incl - padded;
         for (int w = 0; w < warp; ++w) first += warp_sum[w];
-        int at = first;
-        each(active, [&](int t, int id) {
-            if (id == a && at < p.n_col) p.col_token[at++] = t;
-        });
-        for (; at < min(first + padded, p.n_col); ++at) p.col_token[at] = -1;
-        for (int g = first; g < min(first + padded, p.n_col); g += HEAD_GROUP)
-            p.group[g / HEAD_GROUP] = a < p.n_adapters ? a : GROUP_NONE;
+        if (a < n) {
+            place[a] = first;
+            for (int at = first + count; at < min(first + padded, p.n_col); ++at) p.col_token[at] = -1;
+            for (int at = first; at < min(first + padded, p.n_col); at += HEAD_GROUP)
+                p.group[at / HEAD_GROUP] = a < p.n_adapters ? a : GROUP_NONE;
+        }
         __syncthreads();
         if (tid == LAYOUT_THREADS - 1) base = first + padded;
         __syncthreads();
     }
     if (tid == 0) *p.n_col_dev = base;
+    for (int t0 = 0; t0 < p.T; t0 += LAYOUT_THREADS) {
+        const int t = t0 + tid;
+        const int id = t >= p.T ? -1 : t0 == 0 ? first_id : id_of(t);
+        const unsigned peers = __match_any_sync(0xffffffffu, id);
+        const int leader = __ffs(peers) - 1;
+        const int n_warp = min(32, (p.T - t0 + 31) / 32);
+        for (int w = 0; w < n_warp; ++w) {
+            if (warp == w) {
+                int at = 0;
+                if (lane == leader && id >= 0) {
+                    at = place[id];
+                    place[id] = at + __popc(peers);
+                }
+                at = __shfl_sync(0xffffffffu, at, leader) + __popc(peers & ((1u << lane) - 1));
+                if (id >= 0 && at < p.n_col) p.col_token[at] = t;
+            }
+            __syncthreads();
+        }
+    }
 }
 
 // h[column][j] = scale[a] * (A[a][j] . e_t), t and a the column's token and its adapter; zero without an adapter and
 // for the padding ranks; in fp32 and in the two 16-bit terms.  Without a column order the blocks of rank 0 also
-// write the groups' adapters; with one, the blocks of the last y gather the columns' rows of e.
+// write the groups' adapters; with one, the blocks of the last eight y gather the columns' rows of e, a column each.
 // One block per (8 consecutive columns, 4 ranks): its 8 warps split D, each lane reads 16 bytes of the
 // four rows of A and of every token of a run that shares an adapter, and the 32 sums are joined
 // in shared memory in warp order (no atomics: the same bits every run).
@@ -656,7 +748,7 @@ struct ShrinkParams {
     const int* n_col_dev;
     void* e_cols;          // with col_token: [column][ld_cols], the rows of e in column order, zero padded
     long long ld_cols;
-    int rank_blocks;       // blocks in y that compute; with col_token one more copies
+    int rank_blocks;       // blocks in y that compute; with col_token eight more copy
     long long D;
     int vec;  // 16-byte loads are possible for every row
     float* h;
@@ -698,15 +790,13 @@ adapter_shrink_kernel(const ShrinkParams p) {
             tok[i] = i < ntok ? p.col_token[tok0 + i] : -1;
             ids[i] = tok[i] >= 0 ? a : -1;
         }
-        if (int(blockIdx.y) == p.rank_blocks) {
-            T* dst = reinterpret_cast<T*>(p.e_cols);
-            for (int i = 0; i < ntok; ++i) {
-                const int t = p.col_token[tok0 + i];
-                if (t < 0) continue;  // padding columns are never stored: whatever is there may be multiplied
-                for (long long d = threadIdx.x * VE; d < p.ld_cols; d += SHRINK_WARPS * 32 * VE)
-                    *reinterpret_cast<uint4*>(dst + (size_t)(tok0 + i) * p.ld_cols + d) =
-                        load_piece(E + (size_t)t * p.lde + d, p.D - d, p.vec != 0);
-            }
+        if (int(blockIdx.y) >= p.rank_blocks) {
+            const int col = tok0 + blockIdx.y - p.rank_blocks;
+            const int t = col < *p.n_col_dev ? p.col_token[col] : -1;
+            if (t < 0) return;  // padding columns are never stored: whatever is there may be multiplied
+            T* dst = reinterpret_cast<T*>(p.e_cols) + (size_t)col * p.ld_cols;
+            for (long long d = threadIdx.x * VE; d < p.ld_cols; d += SHRINK_WARPS * 32 * VE)
+                *reinterpret_cast<uint4*>(dst + d) = load_piece(E + (size_t)t * p.lde + d, p.D - d, p.vec != 0);
             return;
         }
     } else {
@@ -751,7 +841,7 @@ adapter_shrink_kernel(const ShrinkParams p) {
         for (int i = 0; i < SHRINK_TOK; ++i)
             if (i < ntok && ids[i] == a) members |= 1 << i;
         done |= members;
-        if (a < 0) continue;  // uniform over the block
+        if (a < 0 || rank0 >= p.rank) continue;  // uniform over the block; padding ranks are zeros
         const T* arow[SHRINK_RANK];
 #pragma unroll
         for (int k = 0; k < SHRINK_RANK; ++k)  // ranks past the end repeat the last row; their sums are dropped
