@@ -247,20 +247,39 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { re
 template <>
 __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 
+// A predicated store.  (Written as `if`, the 32 stores of a chunk become 32 branches: 180 cycles a store.)
+__device__ __forceinline__ void store_if(float* q, float x, bool yes) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %2, 0;\n\t@p st.global.f32 [%0], %1;\n\t}" ::"l"(q), "f"(x), "r"(int(yes))
+                 : "memory");
+}
+__device__ __forceinline__ void store_if16(void* q, unsigned short x, bool yes) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %2, 0;\n\t@p st.global.u16 [%0], %1;\n\t}" ::"l"(q), "h"(x), "r"(int(yes))
+                 : "memory");
+}
+__device__ __forceinline__ void store_if(__nv_bfloat16* q, __nv_bfloat16 x, bool yes) {
+    store_if16(q, __bfloat16_as_ushort(x), yes);
+}
+__device__ __forceinline__ void store_if(__half* q, __half x, bool yes) { store_if16(q, __half_as_ushort(x), yes); }
+
 template <typename O>
 __device__ __forceinline__ void store_chunk(const HeadParams& p, int v, int my_token, const float (&x)[32]) {
     O* dst = reinterpret_cast<O*>(p.out) + v;
     const bool v_ok = v < p.V;
+    constexpr int U = 16;  // the shuffles of U columns before their stores, which keep their order
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-        const int t = __shfl_sync(0xffffffffu, my_token, j);
-        if (t >= 0 && v_ok) dst[(size_t)t * p.V] = from_float<O>(x[j]);
+    for (int j0 = 0; j0 < 32; j0 += U) {
+        int t[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) t[j] = __shfl_sync(0xffffffffu, my_token, j0 + j);
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+            store_if(dst + (long long)t[j] * p.V, from_float<O>(x[j0 + j]), t[j] >= 0 && v_ok);
     }
 }
 
 // bias, mixed groups (bits 0 and 1 of `mixed`: the chunk's two), soft-cap and store of one chunk of 32 columns; v is
 // this lane's classifier row
-template <typename BT>
+template <typename BT, bool FP32_OUT>
 __device__ __forceinline__ void finish_chunk(const HeadParams& p, const HeadTiles& tiles, int v, float bias, int c0,
                                              int col_end, unsigned mixed, float (&x)[32]) {
     const int lane = threadIdx.x & 31;
@@ -293,7 +312,7 @@ __device__ __forceinline__ void finish_chunk(const HeadParams& p, const HeadTile
 #pragma unroll
         for (int j = 0; j < 32; ++j) x[j] = apply_softcap(x[j], p.softcap, inv);
     }
-    if (p.out_dtype == 2)
+    if (FP32_OUT || p.out_dtype == 2)
         store_chunk<float>(p, v, my_token, x);
     else if (p.out_dtype == 1)
         store_chunk<__nv_bfloat16>(p, v, my_token, x);
@@ -578,14 +597,11 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
                     for (int c = 0; c < CHUNKS; ++c) {
                         const int col = half * 32 + c * 64;
                         if (col0 + col < col_end && ok) {  // uniform over the warp
+                            uint32_t r[32];
+                            tmem_ld32(taddr + col, r);
+                            tmem_ld_wait();
 #pragma unroll
-                            for (int i = 0; i < 32; i += 16) {
-                                uint32_t r[16];
-                                tmem_ld16(taddr + col + i, r);
-                                tmem_ld_wait();
-#pragma unroll
-                                for (int j = 0; j < 16; ++j) sum[c][i + j] += __uint_as_float(r[j]);
-                            }
+                            for (int j = 0; j < 32; ++j) sum[c][j] += __uint_as_float(r[j]);
                         }
                     }
                 } else {
@@ -599,7 +615,7 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
                         }
 #pragma unroll
                         for (int j = 0; j < 32; ++j) x[j] = ok ? __uint_as_float(r[j]) : __int_as_float(0x7fc00000);
-                        finish_chunk<BT>(p, tiles, v, bias, c0, col_end, mixed >> ((c0 - col0) / HEAD_GROUP), x);
+                        finish_chunk<BT, false>(p, tiles, v, bias, c0, col_end, mixed >> ((c0 - col0) / HEAD_GROUP), x);
                     }
                 }
                 tc_fence_before();
@@ -611,19 +627,15 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
                 }
             }
             if constexpr (SEGMENTED) {
-#pragma unroll 1
-                for (int c = 0; c < CHUNKS; ++c) {
+#pragma unroll
+                for (int c = 0; c < CHUNKS; ++c) {  // in place: the sums fill the registers
                     const int c0 = col0 + half * 32 + c * 64;
-                    if (c0 >= col_end) break;
-                    float x[32];
+                    if (c0 < col_end) {
+                        if (!ok)
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {  // a selection: registers cannot be indexed
-                        float s_c = sum[0][j];
-#pragma unroll
-                        for (int i = 1; i < CHUNKS; ++i) s_c = c == i ? sum[i][j] : s_c;
-                        x[j] = ok ? s_c : __int_as_float(0x7fc00000);
+                            for (int j = 0; j < 32; ++j) sum[c][j] = __int_as_float(0x7fc00000);
+                        finish_chunk<BT, true>(p, tiles, v, bias, c0, col_end, mixed >> ((c0 - col0) / HEAD_GROUP), sum[c]);
                     }
-                    finish_chunk<BT>(p, tiles, v, bias, c0, col_end, mixed >> ((c0 - col0) / HEAD_GROUP), x);
                 }
             }
         }
