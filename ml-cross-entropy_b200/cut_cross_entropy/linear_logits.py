@@ -7,6 +7,8 @@ head (same ``e``, ``c``, ``bias``, ``softcap``) when it has to answer.  The work
 
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from . import _native
@@ -16,14 +18,31 @@ MAX_RANK = 256  # CCE_B200_MAX_RANK
 
 
 def _check_no_grad(name: str, *tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or torch.inference_mode().")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or torch.inference_mode().")
 
 
-def _check_device(device: torch.device, **tensors: torch.Tensor | None) -> None:
-    for name, t in tensors.items():
+def _check_device(device: torch.device, *named: tuple[str, torch.Tensor | None]) -> None:
+    for name, t in named:
         if t is not None and t.device != device:
             raise ValueError(f"Expected {name} on {device}, got {t.device}.")
+
+
+def _on_device(device: torch.device):
+    """A context with ``device`` as the current one; nothing to do (and to pay for) when it already is."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
+    """``t`` as ``(rows, width)`` with unit column stride and rows that do not overlap; copied only if it is not."""
+    if t.dim() != 2:
+        t = t.reshape(-1, width)
+    s0, s1 = t.stride()
+    if (s1 != 1 and width != 1) or (t.size(0) > 1 and s0 < width):
+        t = t.contiguous()
+    return t
 
 
 def linear_logits(
@@ -58,7 +77,8 @@ def linear_logits(
 
     Under autocast ``e``, ``c`` and the adapters are cast to the autocast dtype first.
     """
-    _reject_dtensors(e=e, c=c, bias=bias, lora_a=lora_a, lora_b=lora_b, adapter_ids=adapter_ids)
+    if type(e) is not torch.Tensor or type(c) is not torch.Tensor:  # plain tensors are no DTensors
+        _reject_dtensors(e=e, c=c, bias=bias, lora_a=lora_a, lora_b=lora_b, adapter_ids=adapter_ids)
     _check_no_grad("linear_logits", e, c, bias, lora_a, lora_b)
     if e.dim() < 1 or c.dim() != 2 or e.size(-1) != c.size(1):
         raise ValueError(f"Expected e (..., D) and c (V, D), got {tuple(e.shape)} and {tuple(c.shape)}.")
@@ -89,48 +109,47 @@ def linear_logits(
     if not e.is_cuda:
         raise RuntimeError("cut_cross_entropy (B200 backend) needs CUDA tensors; it has no CPU path")
     scale_t = lora_scale if isinstance(lora_scale, torch.Tensor) else None
-    _check_device(e.device, c=c, bias=bias, lora_a=lora_a, lora_b=lora_b, adapter_ids=adapter_ids, lora_scale=scale_t)
+    _check_device(e.device, ("c", c), ("bias", bias), ("lora_a", lora_a), ("lora_b", lora_b),
+                  ("adapter_ids", adapter_ids), ("lora_scale", scale_t))  # fmt: skip
 
     if torch.is_autocast_enabled("cuda"):
         amp_dtype = torch.get_autocast_dtype("cuda")
         e, c = e.to(amp_dtype), c.to(amp_dtype)
         if lora_a is not None:
             lora_a, lora_b = lora_a.to(amp_dtype), lora_b.to(amp_dtype)
-    for name, t in dict(c=c, lora_a=lora_a, lora_b=lora_b).items():
-        if t is not None and t.dtype != e.dtype:
-            raise ValueError(f"Expected {name} in the dtype of e, {e.dtype}, got {t.dtype}.")
-    out_dtype = e.dtype if out_dtype is None else out_dtype
-    for what, dtype in (("e", e.dtype), ("bias", None if bias is None else bias.dtype), ("out", out_dtype)):
-        if dtype is not None and dtype not in _native._DTYPE_CODE:
-            raise NotImplementedError(f"{what} of dtype {dtype} is not supported by this backend (bf16, fp16, fp32 are)")
+    dtype = e.dtype
+    for name, t in (("c", c), ("lora_a", lora_a), ("lora_b", lora_b)):
+        if t is not None and t.dtype != dtype:
+            raise ValueError(f"Expected {name} in the dtype of e, {dtype}, got {t.dtype}.")
+    out_dtype = dtype if out_dtype is None else out_dtype
+    for what, d in (("e", dtype), ("bias", dtype if bias is None else bias.dtype), ("out", out_dtype)):
+        if d not in _native._DTYPE_CODE:
+            raise NotImplementedError(f"{what} of dtype {d} is not supported by this backend (bf16, fp16, fp32 are)")
 
-    batch_shape = e.shape[:-1]
-    out = torch.empty(*batch_shape, c.size(0), dtype=out_dtype, device=e.device)
+    D, V = e.size(-1), c.size(0)
+    out = torch.empty((*e.shape[:-1], V), dtype=out_dtype, device=e.device)
     if out.numel() == 0:
         return out
-    with torch.cuda.device(e.device):
-        e = e.reshape(-1, e.size(-1))
-        if e.stride(1) != 1 or (e.size(0) > 1 and e.stride(0) < e.size(1)):
-            e = e.contiguous()
-        if c.stride(1) != 1 or (c.size(0) > 1 and c.stride(0) < c.size(1)):
-            c = c.contiguous()
-        args = _native.LogitsArgs()
+    with _on_device(e.device):
+        e, c = _rows(e, D), _rows(c, D)
         bias = None if bias is None else bias.contiguous()
+        args = _native.LogitsArgs()
         args.op = _native.make_operands(e, c, bias, None, softcap)
         args.out, args.out_dtype = out.data_ptr(), _native._DTYPE_CODE[out_dtype]
         if lora_a is not None:
-            lora_a, lora_b, ids = lora_a.contiguous(), lora_b.contiguous(), adapter_ids.reshape(-1).contiguous()
+            lora_a, lora_b, ids = lora_a.contiguous(), lora_b.contiguous(), adapter_ids.contiguous()
             args.lora_a, args.lora_b, args.adapter_ids = lora_a.data_ptr(), lora_b.data_ptr(), ids.data_ptr()
             args.ids_dtype = _native.IDX_I64 if ids.dtype == torch.int64 else _native.IDX_I32
-            args.n_adapters, args.rank = lora_a.size(0), lora_a.size(1)
+            args.n_adapters, args.rank = n, rank
             if lora_scale is not None:
                 if scale_t is None:
-                    scale_t = torch.full((lora_a.size(0),), float(lora_scale), device=e.device)
+                    scale_t = torch.full((n,), float(lora_scale), device=e.device)
                 scale_t = scale_t.to(torch.float32).contiguous()
                 args.lora_scale = scale_t.data_ptr()
         L = _native.lib()
         ws = _native.workspace(L.cce_b200_logits_workspace_bytes(args), e.device)
         rc = L.cce_b200_logits(args, ws.data_ptr(), ws.numel(), _native.stream_ptr(e.device))
-    _native.check(rc, "cce_b200_logits")
+    if rc != 0:
+        _native.check(rc, "cce_b200_logits")
     _native.finish(ws, "cce_b200_logits")
     return out

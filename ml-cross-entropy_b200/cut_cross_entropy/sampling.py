@@ -12,22 +12,24 @@ import torch
 
 from . import _native
 from .linear_cross_entropy import _reject_dtensors
-from .linear_logits import _check_device, _check_no_grad, linear_logits
+from .linear_logits import _check_device, _check_no_grad, _on_device, _rows, linear_logits
 
 
-def _setting(name, value, batch_shape, device, dtype, lo, hi):
+def _setting(name, value, batch_shape, device, dtype, hi):
     """A per-row tensor in the kernel's dtype, or the checked number for all rows: (tensor, number)."""
     if not isinstance(value, torch.Tensor):
-        number = float(value)
-        if math.isnan(number) or not lo <= number <= hi:
-            raise ValueError(f"{name} must be in the range [{lo}, {hi}]. Got {value}.")
+        if not 0 <= value <= hi:  # NaN too
+            raise ValueError(f"{name} must be in the range [0, {hi}]. Got {value}.")
         return None, value
     if value.shape != batch_shape:
         raise ValueError(f"Expected {name} of shape {tuple(batch_shape)}, got {tuple(value.shape)}.")
-    if value.dtype == torch.bool or value.is_complex() or (dtype == torch.int64 and value.is_floating_point()):
-        raise ValueError(f"{name} of dtype {value.dtype} is not supported.")
-    _check_device(device, **{name: value})
-    return value.to(dtype).reshape(-1).contiguous(), None
+    if value.dtype != dtype:
+        if value.dtype == torch.bool or value.is_complex() or (dtype == torch.int64 and value.is_floating_point()):
+            raise ValueError(f"{name} of dtype {value.dtype} is not supported.")
+        value = value.to(dtype)
+    if value.device != device:
+        raise ValueError(f"Expected {name} on {device}, got {value.device}.")
+    return value.contiguous(), 0
 
 
 def sample_tokens(
@@ -61,54 +63,47 @@ def sample_tokens(
     The numbers in tensors are not looked at on the host: there, a temperature of 0 or less (or NaN) is greedy,
     ``top_p`` outside (0, 1) and ``min_p`` outside (0, 1] act like the nearest value inside, or like "off".
     """
-    _reject_dtensors(logits=logits, u=u)
+    if type(logits) is not torch.Tensor or type(u) is not torch.Tensor:  # plain tensors are no DTensors
+        _reject_dtensors(logits=logits, u=u)
     _check_no_grad("sample_tokens", logits)
-    if logits.dim() < 1 or u.shape != logits.shape[:-1]:
+    batch_shape = u.shape
+    if logits.dim() < 1 or batch_shape != logits.shape[:-1]:
         raise ValueError(f"Expected logits (..., V) and u (...), got {tuple(logits.shape)} and {tuple(u.shape)}.")
-    if logits.size(-1) == 0:
+    V = logits.size(-1)
+    if V == 0:
         raise ValueError("logits have no entries.")
     if not u.is_floating_point():
         raise ValueError(f"u must be a floating-point tensor. Got {u.dtype}.")
-    batch_shape, V = logits.shape[:-1], logits.size(-1)
     if isinstance(top_k, float):
         raise ValueError(f"top_k must be a whole number. Got {top_k}.")
-    dev = logits.device
-    f32 = torch.float32
-    temperature_t, temperature_n = _setting("temperature", temperature, batch_shape, dev, f32, 0.0, math.inf)
-    top_k_t, top_k_n = _setting("top_k", 0 if top_k is None else top_k, batch_shape, dev, torch.int64, 0, 2**62)
-    top_p_t, top_p_n = _setting("top_p", 1.0 if top_p is None else top_p, batch_shape, dev, f32, 0.0, 1.0)
-    min_p_t, min_p_n = _setting("min_p", 0.0 if min_p is None else min_p, batch_shape, dev, f32, 0.0, 1.0)
+    dev, f32 = logits.device, torch.float32
+    temperature_t, temperature_n = _setting("temperature", temperature, batch_shape, dev, f32, math.inf)
+    top_k_t, top_k_n = _setting("top_k", 0 if top_k is None else top_k, batch_shape, dev, torch.int64, 2**62)
+    top_p_t, top_p_n = _setting("top_p", 1.0 if top_p is None else top_p, batch_shape, dev, f32, 1.0)
+    min_p_t, min_p_n = _setting("min_p", 0.0 if min_p is None else min_p, batch_shape, dev, f32, 1.0)
     if not logits.is_cuda:
         raise RuntimeError("cut_cross_entropy (B200 backend) needs CUDA tensors; it has no CPU path")
-    _check_device(dev, u=u)
-    if logits.dtype not in _native._DTYPE_CODE:
+    _check_device(dev, ("u", u))
+    dtype = _native._DTYPE_CODE.get(logits.dtype)
+    if dtype is None:
         raise NotImplementedError(
             f"logits of dtype {logits.dtype} are not supported by this backend (bf16, fp16, fp32 are)"
         )
 
     tokens = torch.empty(batch_shape, dtype=torch.int64, device=dev)
     logprobs = torch.empty(batch_shape, dtype=f32, device=dev) if return_logprobs else None
-    with torch.cuda.device(dev):
-        rows = logits.reshape(-1, V)
-        if rows.stride(1) != 1 or (rows.size(0) > 1 and rows.stride(0) < V):
-            rows = rows.contiguous()
-        u = u.to(f32).reshape(-1).contiguous()
-        args = _native.SampleArgs()
-        args.logits, args.B, args.V = rows.data_ptr(), rows.size(0), V
-        args.ld = rows.stride(0) if rows.size(0) > 1 else V
-        args.dtype, args.u = _native._DTYPE_CODE[rows.dtype], u.data_ptr()
-        for name, t, n in (
-            ("temperature", temperature_t, temperature_n),
-            ("top_k", top_k_t, top_k_n),
-            ("top_p", top_p_t, top_p_n),
-            ("min_p", min_p_t, min_p_n),
-        ):
-            setattr(args, name, _native._ptr(t))
-            if t is None:
-                setattr(args, name + "_all", n)
-        args.tokens, args.logprobs = tokens.data_ptr(), _native._ptr(logprobs)
+    with _on_device(dev):
+        rows = _rows(logits, V)
+        u = u.to(f32).contiguous()
+        B = rows.size(0)
+        args = _native.SampleArgs(
+            rows.data_ptr(), B, V, rows.stride(0) if B > 1 else V, dtype, u.data_ptr(), _native._ptr(temperature_t),
+            _native._ptr(top_k_t), _native._ptr(top_p_t), _native._ptr(min_p_t), temperature_n, top_p_n, min_p_n, top_k_n,
+            tokens.data_ptr(), _native._ptr(logprobs),
+        )  # fmt: skip
         rc = _native.lib().cce_b200_sample(args, _native.stream_ptr(dev))
-    _native.check(rc, "cce_b200_sample")
+    if rc != 0:
+        _native.check(rc, "cce_b200_sample")
     return (tokens, logprobs) if return_logprobs else tokens
 
 
