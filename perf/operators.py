@@ -10,6 +10,7 @@
 
 from __future__ import annotations
 
+import functools
 import math
 import sys
 from pathlib import Path
@@ -220,6 +221,7 @@ def run(state):
     )  # fmt: skip
 
 
+@functools.cache
 def _package():
     path = str(Path("ml-cross-entropy_b200").resolve())
     if path not in sys.path:
