@@ -12,14 +12,21 @@
 //
 // A row is one cluster of CTAs; each keeps its slice of the row in shared memory, so the logits are read
 // from HBM once and every later pass runs on chip.  The row is never sorted as a whole.  With top-k or top-p a
-// histogram (counts; masses too for top-p alone), linear in the logit between the maximum and the 2^-40 floor,
-// finds the bin that holds the border.  If at most SMP_LIST logits lie in that bin or above it, they
-// are gathered into one CTA, sorted there, and everything else is done on that list.  Otherwise the border is
-// narrowed down by further histograms over the integer keys of its bin until it is a single value
-// (ties at that value are kept by index), and the kept weights are summed by blocks over the slices.
+// histogram of counts, linear in the logit between the maximum and the 2^-40 floor, tells where the border lies:
+// the bin of the k-th logit exactly, the bin where the mass reaches p to within the width of a bin (the exact sum of all
+// weights is formed in the same pass; exact masses per bin would need 64-bit atomics, 1.5 cycles per logit).
+//  - At most SMP_LIST logits down to the border: they are gathered into one CTA, sorted, and the rest
+//    is done on that list.
+//  - top-p with more: the logits of some bins around the estimate are gathered and sorted, the weights above them are
+//    summed exactly (by blocks, which the draw needs anyway), and the border is found, exactly, in the list.
+//  - Otherwise (a large k, thousands of equal logits, an estimate that was off): further histograms narrow the
+//    border down over the integer keys of its bin until it is a single value.
+// A cluster barrier costs 0.5 to 0.8 us, a pass over a slice of 16384 logits 1 to 3 us: the latency of a row is its
+// five to seven barriers, its throughput the fp64 weights (0.25 cycles per logit and SM) and the atomics (0.3).
 #pragma once
 #include <cooperative_groups.h>
 #include "engine.cuh"
+#include "ptx_pair.cuh"
 
 namespace cce {
 
@@ -109,8 +116,8 @@ struct SampleLayout {
         share = SMP_BINS / cluster;
         max_blk = slice / SMP_BLK + 1;
         int o = 0;
-        hist_mass = o, o += SMP_BINS * 8;  // later: two lists of SMP_LIST entries
-        hist_cnt = o, o += SMP_BINS * 4;   // later: one list of SMP_LIST entries
+        hist_mass = o, o += SMP_BINS * 8;  // also two lists of SMP_LIST entries
+        hist_cnt = o, o += SMP_BINS * 4;   // also one list of SMP_LIST entries
         own_mass = o, o += share * 8;
         own_cnt = o, o += share * 4;
         blk_mass = o, o += max_blk * 8;
@@ -126,8 +133,8 @@ struct SmpShared {
     u64 wa[SMP_WARPS], wb[SMP_WARPS];
     u64 r[4];
     float wf[SMP_WARPS];
-    float l_floor, l_min;
     uint32_t n_local, n_list, base;
+    int lo, hi, all;
 };
 
 __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
@@ -143,30 +150,69 @@ __device__ __forceinline__ u64 warp_scan_u64(u64 v, int lane) {  // inclusive
     }
     return v;
 }
-// In-place ascending sort of n (a power of two, at most 2 * SMP_THREADS) values by the whole CTA.
+// In-place ascending sort of n values (a power of two from 64 to 2 * SMP_THREADS) by the whole CTA: bitonic; the
+// steps within 64 neighbours stay in the registers of a warp (two values per lane), so that 1024 values need 10
+// steps through shared memory instead of 55.
+__device__ __forceinline__ void sort_pair(u64& a, u64& b, bool ascending) {
+    if ((a > b) == ascending) {
+        const u64 t = a;
+        a = b;
+        b = t;
+    }
+}
 __device__ __forceinline__ void bitonic_sort(u64* v, int n) {
-    for (int k = 2; k <= n; k <<= 1) {
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            __syncthreads();
-            const int t = threadIdx.x;
-            if (t < n / 2) {
-                const int a = 2 * t - (t & (j - 1)), b = a + j;
-                const u64 x = v[a], y = v[b];
-                if ((x > y) == ((a & k) == 0)) {
-                    v[a] = y;
-                    v[b] = x;
-                }
+    const int tid = threadIdx.x, lane = tid & 31, e0 = (tid >> 5) * 64 + lane;
+    const bool active = e0 < n;  // uniform over the warp
+    u64 a = 0, b = 0;
+    // the steps j = 32 .. 1 of stage k on the warp's 64 values
+    auto inner = [&](int k) {
+        for (int j = min(32, k >> 1); j > 0; j >>= 1) {
+            if (j == 32) {
+                sort_pair(a, b, (e0 & k) == 0);
+            } else {
+                const u64 pa = __shfl_xor_sync(0xffffffffu, a, j), pb = __shfl_xor_sync(0xffffffffu, b, j);
+                const bool low = (lane & j) == 0;
+                const bool up_a = (e0 & k) == 0, up_b = ((e0 + 32) & k) == 0;
+                a = ((a < pa) == (up_a == low)) ? a : pa;
+                b = ((b < pb) == (up_b == low)) ? b : pb;
             }
+        }
+    };
+    __syncthreads();
+    if (active) {
+        a = v[e0];
+        b = v[e0 + 32];
+        for (int k = 2; k <= 64; k <<= 1) inner(k);
+        v[e0] = a;
+        v[e0 + 32] = b;
+    }
+    for (int k = 128; k <= n; k <<= 1) {
+        for (int j = k >> 1; j >= 64; j >>= 1) {
+            __syncthreads();
+            if (tid < n / 2) {
+                const int i = 2 * tid - (tid & (j - 1));
+                u64 x = v[i], y = v[i + j];
+                sort_pair(x, y, (i & k) == 0);
+                v[i] = x;
+                v[i + j] = y;
+            }
+        }
+        __syncthreads();
+        if (active) {
+            a = v[e0];
+            b = v[e0 + 32];
+            inner(k);
+            v[e0] = a;
+            v[e0 + 32] = b;
         }
     }
     __syncthreads();
 }
-
-// Positions with l > above are kept, and the first n_tie (in index order) of those with l == tie.
-struct Cut {
-    float above, tie;
-    long long n_tie;
-};
+__device__ __forceinline__ int sort_size(int n) {
+    int m = 64;
+    while (m < n) m *= 2;
+    return m;
+}
 
 template <typename T>
 struct Sampler {
@@ -206,6 +252,8 @@ struct Sampler {
     }
     __device__ __forceinline__ u64* hist_mass() const { return reinterpret_cast<u64*>(dyn + lay.hist_mass); }
     __device__ __forceinline__ uint32_t* hist_cnt() const { return reinterpret_cast<uint32_t*>(dyn + lay.hist_cnt); }
+    __device__ __forceinline__ u64* own_mass() const { return reinterpret_cast<u64*>(dyn + lay.own_mass); }
+    __device__ __forceinline__ uint32_t* own_cnt() const { return reinterpret_cast<uint32_t*>(dyn + lay.own_cnt); }
     __device__ __forceinline__ u64* blk_mass() const { return reinterpret_cast<u64*>(dyn + lay.blk_mass); }
     __device__ __forceinline__ uint32_t* blk_tie() const { return reinterpret_cast<uint32_t*>(dyn + lay.blk_tie); }
 
@@ -342,7 +390,8 @@ struct Sampler {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         if (lane == 0) sm.wf[warp] = m;
-        if (size > 1) cl.sync(); else __syncthreads();  // the cluster's CTAs run: their memory may be written
+        __syncthreads();
+        if (size > 1) cluster_wait();  // the cluster's CTAs run (they arrived as they started): their memory may be written
         m = -INFINITY;
 #pragma unroll
         for (int w = 0; w < SMP_WARPS; ++w) m = fmaxf(m, sm.wf[w]);
@@ -398,24 +447,35 @@ struct Sampler {
         }
         __syncthreads();
     }
-    // Counts and masses of the bins over the cluster: this CTA's share to own_mass and own_cnt, the shares' totals
-    // to got(0, r) (mass) and got(1, r) (count) of everyone.
+    // The bins over the cluster: this CTA's share to own_cnt (and own_mass).
     __device__ __forceinline__ void merge_hist(bool with_mass) {
-        u64* mass = reinterpret_cast<u64*>(dyn + lay.own_mass);
-        uint32_t* cnt = reinterpret_cast<uint32_t*>(dyn + lay.own_cnt);
+        u64* mass = own_mass();
+        uint32_t* cnt = own_cnt();
+        for (int b = tid; b < lay.share; b += SMP_THREADS) {
+            cnt[b] = 0;
+            mass[b] = 0;
+        }
         if (size > 1) cl.sync(); else __syncthreads();  // all histograms are complete
+        const int n = lay.share * size;  // = SMP_BINS: a thread reads a few bins of other CTAs
+#pragma unroll
+        for (int i0 = 0; i0 < SMP_BINS; i0 += SMP_THREADS) {
+            const int i = i0 + tid, b = i % lay.share, r = i / lay.share;
+            if (i < n) {
+                const uint32_t c = cl.map_shared_rank(hist_cnt(), r)[rank * lay.share + b];
+                if (c) {
+                    atomicAdd(&cnt[b], c);
+                    if (with_mass) atomicAdd(&mass[b], cl.map_shared_rank(hist_mass(), r)[rank * lay.share + b]);
+                }
+            }
+        }
+        __syncthreads();
+    }
+    // the shares' totals to got(0, r) (mass) and got(1, r) (count) of everyone
+    __device__ __forceinline__ void exchange_totals() {
         u64 tm = 0, tc = 0;
         for (int b = tid; b < lay.share; b += SMP_THREADS) {
-            u64 m = 0;
-            uint32_t c = 0;
-            for (int r = 0; r < size; ++r) {
-                c += cl.map_shared_rank(hist_cnt(), r)[rank * lay.share + b];
-                if (with_mass) m += cl.map_shared_rank(hist_mass(), r)[rank * lay.share + b];
-            }
-            mass[b] = m;
-            cnt[b] = c;
-            tm += m;
-            tc += c;
+            tm += own_mass()[b];
+            tc += own_cnt()[b];
         }
         cta_sum(tm, tc);
         exchange(tm, tc);
@@ -425,11 +485,11 @@ struct Sampler {
         int owner, bin;
         u64 mass_above, cnt_above, cnt;  // above the bin, and in it
     };
-    // The bin where the running count (by_mass: mass) from the top reaches `target`, straight after merge_hist;
+    // The bin where the running count (by_mass: mass) from the top reaches `target`, straight after exchange_totals;
     // (am, ac): the mass and count above all of its bins.
     __device__ __forceinline__ Border find_border(bool by_mass, u64 target, u64 am, u64 ac) {
-        const u64* mass = reinterpret_cast<const u64*>(dyn + lay.own_mass);
-        const uint32_t* cnt = reinterpret_cast<const uint32_t*>(dyn + lay.own_cnt);
+        const u64* mass = own_mass();
+        const uint32_t* cnt = own_cnt();
         int owner = 0;
         while (owner + 1 < size && (by_mass ? am + got(0, owner) : ac + got(1, owner)) < target) {
             am += got(0, owner);
@@ -483,6 +543,24 @@ struct Sampler {
         });
         merge_hist(with_mass);
     }
+    // the counts of level 0, and the sum of this CTA's weights
+    __device__ __forceinline__ u64 level0_counts_and_sum() {
+        clear_hist(false);
+        u64 sum = 0;
+        each_of_slice([&](float l, int) {
+            if (l >= l_floor) {
+                atomicAdd(&hist_cnt()[bin0(l)], 1u);
+                sum += weight(l);
+            }
+        });
+        merge_hist(false);
+        return sum;
+    }
+    // the running sum that top-p has to reach, of the mass it is measured by
+    __device__ __forceinline__ u64 p_target(u64 mass) const {
+        const double t = ceil(fmax(top_p, 0.0) * double(mass));
+        return t < 1.0 ? 1ull : min((u64)t, mass);
+    }
 
     // The first key of [lo, hi] that fulfils a predicate which holds from some key on (hi if none before it does),
     // by all threads together
@@ -522,6 +600,7 @@ struct Sampler {
                 }
             });
             merge_hist(by_mass);
+            exchange_totals();
             bd = find_border(by_mass, target, bd.mass_above, bd.cnt_above);
             const uint32_t top = hi - (uint32_t(bd.bin) << shift);
             lo = max(lo, top - ((1u << shift) - 1));
@@ -530,40 +609,55 @@ struct Sampler {
         return Level{order_value(lo), bd.mass_above, bd.cnt_above};
     }
 
+    // A logit and its token as one number: ascending = falling logits, ties by the lower index.
+    __device__ __forceinline__ u64 rank_key(float l, long long token) const { return u64(~order_key(l)) << 32 | u64(token); }
+    static __device__ __forceinline__ float key_logit(u64 key) { return order_value(~uint32_t(key >> 32)); }
+
+    // This CTA's candidates: up to SMP_LIST, in hist_mass()[0 .. n_local).
+    __device__ __forceinline__ void collect(float l, int pos) {
+        hist_mass()[atomicAdd(&sm.n_local, 1u)] = rank_key(l, token_at(pos));
+    }
+    // They go to the list of CTA `leader`, hist_mass() + SMP_LIST there, where n_list counts them; a barrier of the
+    // cluster has to follow.
+    __device__ __forceinline__ void send_candidates(int leader) {
+        __syncthreads();
+        const uint32_t n = sm.n_local;
+        if (tid == 0 && n > 0) sm.base = atomicAdd(&cl.map_shared_rank(&sm, leader)->n_list, n);
+        __syncthreads();
+        u64* dst = cl.map_shared_rank(hist_mass() + SMP_LIST, leader) + sm.base;
+        for (uint32_t i = tid; i < n; i += SMP_THREADS) dst[i] = hist_mass()[i];
+    }
+    // In the leader, after that barrier: sorts the list and returns its length.
+    __device__ __forceinline__ int sort_candidates() {
+        u64* list = hist_mass() + SMP_LIST;
+        const int n = int(sm.n_list), m = sort_size(n);
+        for (int i = n + tid; i < m; i += SMP_THREADS) list[i] = ~0ull;
+        bitonic_sort(list, m);
+        return n;
+    }
+
     // ---- the whole rest on a list: every logit of bins 0..bin (at most SMP_LIST) goes to CTA `leader`, which sorts
     // them, applies the three prefixes and draws.  mass: of all weights (top-p without top-k).
     __device__ __forceinline__ void finish_on_list(int bin, int leader, u64 mass) {
-        u64* local = hist_mass();               // this CTA's candidates; in the leader later the weights
-        u64* list = hist_mass() + SMP_LIST;     // the leader's list: (key descending, index ascending)
-        u64* by_index = reinterpret_cast<u64*>(hist_cnt());
         each_of_slice([&](float l, int pos) {
-            if (l >= l_floor && bin0(l) <= bin)
-                local[atomicAdd(&sm.n_local, 1u)] = u64(~order_key(l)) << 32 | u64(token_at(pos));
+            if (l >= l_floor && bin0(l) <= bin) collect(l, pos);
         });
-        __syncthreads();
-        const uint32_t n_local = sm.n_local;
-        if (tid == 0 && n_local > 0) sm.base = atomicAdd(&cl.map_shared_rank(&sm, leader)->n_list, n_local);
-        __syncthreads();
-        u64* dst = cl.map_shared_rank(list, leader) + sm.base;
-        for (uint32_t i = tid; i < n_local; i += SMP_THREADS) dst[i] = local[i];
+        send_candidates(leader);
         if (size > 1) cl.sync(); else __syncthreads();
         if (rank != leader) return;
-
-        const int n = int(sm.n_list);
-        int n2 = 2;
-        while (n2 < n) n2 *= 2;
-        for (int i = n + tid; i < n2; i += SMP_THREADS) list[i] = ~0ull;
-        bitonic_sort(list, n2);
-
+        u64* const weights = hist_mass();               // in place of the leader's own candidates
+        const u64* const list = hist_mass() + SMP_LIST;
+        u64* const by_index = reinterpret_cast<u64*>(hist_cnt());
+        const int n = sort_candidates();
         const int n_k = k && k < n ? int(k) : n;
         u64 w[2];
         float l[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int j = 2 * tid + i;
-            l[i] = j < n_k ? order_value(~uint32_t(list[j] >> 32)) : -INFINITY;
+            l[i] = j < n_k ? key_logit(list[j]) : -INFINITY;
             w[i] = j < n_k ? weight(l[i]) : 0;
-            if (j < n_k) local[j] = w[i];
+            if (j < n_k) weights[j] = w[i];
         }
         u64 cum = w[0] + w[1], above_min = u64(l[0] >= l_min) + u64(l[1] >= l_min);
         cta_scan(cum, above_min);
@@ -572,150 +666,335 @@ struct Sampler {
         __syncthreads();
         int kept = max(1, int(min(u64(n_k), sm.r[1])));
         if (top_p < 1.0) {
-            const u64 s = k ? sm.r[0] : mass;
-            const double t = ceil(fmax(top_p, 0.0) * double(s));
-            const u64 target = t < 1.0 ? 1ull : min((u64)t, s);
+            const u64 target = p_target(k ? sm.r[0] : mass);
             // the first whose running sum reaches it
-            int n_p = 0;
-            n_p += __syncthreads_count(2 * tid < n_k && cum - w[1] < target);
+            int n_p = __syncthreads_count(2 * tid < n_k && cum - w[1] < target);
             n_p += __syncthreads_count(2 * tid + 1 < n_k && cum < target);
             kept = min(kept, n_p + 1);
         }
-        __syncthreads();
         // the kept weights' sum, and the kept candidates in order of their index
         if ((kept - 1) >> 1 == tid) sm.r[2] = (kept & 1) ? cum - w[1] : cum;
-        n2 = 2;
-        while (n2 < kept) n2 *= 2;
-        for (int j = tid; j < n2; j += SMP_THREADS) by_index[j] = j < kept ? (list[j] << 32 | u64(j)) : ~0ull;
-        bitonic_sort(by_index, n2);
+        const int m = sort_size(kept);
+        for (int j = tid; j < m; j += SMP_THREADS) by_index[j] = j < kept ? (list[j] << 32 | u64(j)) : ~0ull;
+        bitonic_sort(by_index, m);
         const u64 total = sm.r[2], target = draw_target(total);
         u64 v[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) v[i] = 2 * tid + i < kept ? local[uint32_t(by_index[2 * tid + i])] : 0;
+        for (int i = 0; i < 2; ++i) v[i] = 2 * tid + i < kept ? weights[uint32_t(by_index[2 * tid + i])] : 0;
         u64 run = v[0] + v[1], unused = 0;
         cta_scan(run, unused);
         if (run > target && run - v[0] - v[1] <= target) {  // one thread
             const u64 e = by_index[2 * tid + (run - v[1] > target ? 0 : 1)];
-            write((long long)(e >> 32), log_share(order_value(~uint32_t(list[uint32_t(e)] >> 32)), total));
+            write((long long)(e >> 32), log_share(key_logit(list[uint32_t(e)]), total));
         }
     }
 
-    // ---- the cut of top-k and top-p as a value and a number of ties, for borders too far down for a list
-    __device__ __forceinline__ Cut cut_by_levels(Border bd, bool by_mass, u64 k_target, u64 p_target) {
-        Cut cut{-INFINITY, 0.0f, 0};
-        u64 mass = 0;
-        if (k) {
-            if (k_target) {
-                const Level lv = descend(bd, false, k_target);
-                cut = Cut{lv.value, lv.value, (long long)(k_target - lv.cnt_above)};
+    // ---- top-p alone: where the mass reaches the target, estimated from the counts (every weight of a bin as its
+    // middle's, off by at most 0.7 %).  In every CTA: a window [lo, hi] of bins around the estimate, from the share of
+    // CTA `owner`, with at most SMP_LIST logits.  all: the logits down to hi fit the list, and reach the target for certain.
+    struct Window {
+        int owner, lo, hi;
+        bool all, none;  // none: the bin of the estimate alone is too full
+    };
+    __device__ __forceinline__ Window p_window(u64& mass, u64& target, u64 sum) {
+        u64 unused = 0;
+        cta_sum(sum, unused);
+        // the estimates, in place of the (unused) masses of the bins; all threads of one order: the same every run
+        double* est = reinterpret_cast<double*>(own_mass());
+        const double step = -2.0 / double(bin_scale) * weight.scale * (1.0 / SMP_TABLE);  // log2 of a weight per bin
+        const double unit = exp2(double(p.frac_bits));
+        double tm = 0.0;
+        u64 tc = 0;
+        const int per = max(1, lay.share / SMP_THREADS), b0 = tid * per;
+        for (int i = 0; i < per && b0 + i < lay.share; ++i) {
+            const int b = rank * lay.share + b0 + i;
+            const uint32_t c = own_cnt()[b0 + i];
+            const double e = c ? double(c) * unit * double(ex2f(float((double(b) + 0.5) * step))) : 0.0;
+            est[b0 + i] = e;
+            tm += e;
+            tc += c;
+        }
+        // inclusive scans over the threads
+        u64 em = u64(tm), ec = tc;
+        const u64 em_own = em;
+        cta_scan(em, ec);
+        if (tid == SMP_THREADS - 1) {
+            sm.r[0] = em;
+            sm.r[1] = ec;
+        }
+        __syncthreads();
+        exchange(sm.r[0], sm.r[1], sum);
+        mass = 0;
+        for (int r = 0; r < size; ++r) mass += got(2, r);
+        target = p_target(mass);
+        int owner = 0;
+        u64 am = 0, ac = 0, bm = 0, bc = 0;  // estimate and count above share r; those of the owner
+        for (int r = 0, found = 0; r < size; ++r) {
+            if (got(1, r) > 0 && !found) {  // never an empty share
+                owner = r;
+                bm = am;
+                bc = ac;
+                found = am + got(0, r) >= target;
             }
-            if (!(top_p < 1.0)) return cut;
-            // the counts alone led here: now the masses, of the top-k and of every bin
-            u64 s = 0, unused = 0;
+            am += got(0, r);
+            ac += got(1, r);
+        }
+        __syncthreads();
+        if (tid == 0) {
+            sm.lo = sm.all = lay.share;
+            sm.hi = -1;
+        }
+        if (tid == SMP_THREADS - 1) sm.r[3] = ~0ull;  // the bin of the estimate and the count above it
+        __syncthreads();
+        if (rank == owner) {
+            // the thread whose bins cross the target; the last one with a count if the estimate falls short
+            const u64 begin = bm + em - em_own;
+            const bool crosses = begin < target && target <= bm + em;
+            if (crosses || (bm + sm.r[0] < target && ec == sm.r[1] && tc > 0)) {
+                double run = double(begin);
+                u64 c = bc + ec - tc;
+                int at = b0;
+                for (int i = 0; i < per && b0 + i < lay.share; ++i) {
+                    at = b0 + i;
+                    run += est[at];
+                    if (run >= double(target) || (!crosses && c + own_cnt()[at] == bc + ec)) break;
+                    if (i + 1 < per && b0 + i + 1 < lay.share) c += own_cnt()[at];
+                }
+                sm.r[3] = u64(at) << 40 | c;
+            }
+        }
+        __syncthreads();
+        if (rank == owner) {
+            const int at = int(sm.r[3] >> 40);
+            const u64 c_at = sm.r[3] & 0xffffffffffull;           // count above the bin
+            const u64 n_at = sm.r[3] == ~0ull ? ~0ull : own_cnt()[at];
+            const u64 room = n_at < SMP_LIST ? (SMP_LIST - n_at) / 2 : 0;
+            if (n_at <= SMP_LIST) {
+                u64 c = bc + ec - tc;
+                double run = double(bm + em - em_own);
+                for (int i = 0; i < per && b0 + i < lay.share; ++i) {  // (c, c + n]: the logits of this bin
+                    const int b = b0 + i;
+                    const u64 n = own_cnt()[b];
+                    run += est[b];
+                    if (b <= at && c_at - c <= room) atomicMin(&sm.lo, b);
+                    if (b >= at && c + n - c_at - n_at <= room) {
+                        atomicMax(&sm.hi, b);
+                        if (c + n <= SMP_LIST && (c + n == ac || run * 0.98 >= double(target))) atomicMin(&sm.all, b);
+                    }
+                    c += n;
+                }
+            }
+        }
+        __syncthreads();
+        // sm.all: a bin down to which everything fits the list and reaches the target
+        exchange(u64(owner * lay.share + sm.lo), u64(sm.hi < 0 ? 0 : owner * lay.share + sm.hi + 1),
+                 u64(sm.all == lay.share ? 0 : owner * lay.share + sm.all + 1));
+        const int hi = int(got(1, owner)) - 1, all = int(got(2, owner)) - 1;
+        return Window{owner, int(got(0, owner)), all >= 0 ? all : hi, all >= 0, hi < 0};
+    }
+
+    // The exact border of top-p in the window.  Leaves the kept weights by blocks in blk_mass; the key of the last
+    // kept logit, or 0 when the window missed the border.
+    __device__ __forceinline__ u64 cut_in_window(const Window& win, u64 target) {
+        u64 above = 0, unused = 0;
+        for (int b = warp; b < n_blk; b += SMP_WARPS) {
+            u64 bm = 0;
+            each(b, [&](float l, int pos) {
+                if (l >= l_floor) {
+                    const int bin = bin0(l);
+                    if (bin < win.lo) {
+                        const u64 w = weight(l);
+                        above += w;
+                        if (l >= l_min) bm += w;
+                    } else if (bin <= win.hi) {
+                        collect(l, pos);
+                    }
+                }
+            });
+            bm = warp_sum_u64(bm);
+            if (lane == 0) blk_mass()[b] = bm;
+        }
+        cta_sum(above, unused);
+        send_candidates(win.owner);
+        exchange(above);
+        above = 0;
+        for (int r = 0; r < size; ++r) above += got(0, r);
+        if (rank == win.owner) {
+            const int n = sort_candidates();
+            const u64* const list = hist_mass() + SMP_LIST;
+            u64 w[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) w[i] = 2 * tid + i < n ? weight(key_logit(list[2 * tid + i])) : 0;
+            u64 cum = w[0] + w[1];
+            cta_scan(cum, unused);
+            if (tid == 0) sm.r[0] = 0;
+            __syncthreads();
+            const u64 end = above + cum, begin = end - w[0] - w[1];
+            if (begin < target && target <= end)  // one thread, if the border is here
+                sm.r[0] = list[2 * tid + (begin + w[0] >= target ? 0 : 1)];
+            __syncthreads();
+        }
+        exchange(sm.r[0]);
+        const u64 cut = got(0, win.owner);
+        if (cut) {
+            // this CTA's kept candidates join their blocks (its own list may have been sorted into the leader's: it is
+            // still here, the leader's copy is the other half)
+            for (uint32_t i = tid; i < sm.n_local; i += SMP_THREADS) {
+                const u64 key = hist_mass()[i];
+                const float l = key_logit(key);
+                if (key <= cut && l >= l_min)
+                    atomicAdd(&blk_mass()[int((long long)(key & 0xffffffffu) - start + phase) / SMP_BLK], weight(l));
+            }
+        }
+        __syncthreads();
+        return cut;
+    }
+
+    // ---- the key of the last kept logit by narrowing histograms, for borders that no list holds
+    __device__ __forceinline__ u64 cut_by_levels(bool top_k_cuts, const Border& k_border, u64 k_target) {
+        Level lv{-INFINITY, 0, 0};
+        long long n_tie = 0;  // how many of the logits equal to lv.value are kept
+        if (top_k_cuts) {
+            lv = descend(k_border, false, k_target);
+            n_tie = (long long)(k_target - lv.cnt_above);
+        }
+        if (top_p < 1.0) {
+            // the masses, of the top-k and of every bin
+            u64 s = 0, unused = 0, mass = 0;
             each_of_slice([&](float l, int) {
-                if (l > cut.above && l >= l_floor) s += weight(l);
+                if (l > lv.value && l >= l_floor) s += weight(l);
             });
             cta_sum(s, unused);
             exchange(s);
             for (int r = 0; r < size; ++r) mass += got(0, r);
-            if (cut.n_tie > 0) mass += u64(cut.n_tie) * weight(cut.tie);
-            const double t = ceil(fmax(top_p, 0.0) * double(mass));
-            p_target = t < 1.0 ? 1ull : min((u64)t, mass);
+            if (n_tie > 0) mass += u64(n_tie) * weight(lv.value);
+            const u64 target = p_target(mass);
             level0(true);
-            bd = find_border(true, p_target, 0, 0);
+            exchange_totals();
+            const Level lp = descend(find_border(true, target, 0, 0), true, target);
+            const u64 w = weight(lp.value);
+            long long need = (long long)((target - lp.mass_above + w - 1) / w);  // the mass above is short of the target
+            if (n_tie > 0 && lp.value == lv.value) need = min(need, n_tie);
+            lv = lp;
+            n_tie = need;
         }
-        const Level lv = descend(bd, true, p_target);
-        const u64 w = weight(lv.value);
-        long long need = (long long)((p_target - lv.mass_above + w - 1) / w);  // the mass above is short of the target
-        if (cut.n_tie > 0 && lv.value == cut.tie) need = min(need, cut.n_tie);
-        return Cut{lv.value, lv.value, need};
+        if (n_tie == 0) return ~0ull;
+        // the index of the n_tie-th of the equal logits
+        u64 mine = 0, unused = 0;
+        __syncthreads();
+        for (int b = warp; b < n_blk; b += SMP_WARPS) {
+            uint32_t t = 0;
+            each(b, [&](float l, int) { t += l == lv.value; });
+            t = __reduce_add_sync(0xffffffffu, t);
+            if (lane == 0) {
+                blk_tie()[b] = t;
+                mine += t;
+            }
+        }
+        cta_sum(mine, unused);
+        exchange(mine);
+        u64 before = 0;
+        for (int r = 0; r < rank; ++r) before += got(0, r);
+        u64 left = u64(n_tie) > before ? u64(n_tie) - before : 0;  // 1-based within this CTA
+        if (tid == 0) sm.r[0] = 0;
+        __syncthreads();
+        if (warp == 0 && left > 0 && left <= mine) {
+            for (int b0 = 0; b0 < n_blk; b0 += 32) {
+                const u64 t = b0 + lane < n_blk ? blk_tie()[b0 + lane] : 0;
+                const u64 incl = warp_scan_u64(t, lane);
+                const unsigned hit = __ballot_sync(0xffffffffu, incl >= left);
+                if (!hit) {
+                    left -= __shfl_sync(0xffffffffu, incl, 31);
+                    continue;
+                }
+                const int f = __ffs(hit) - 1;
+                left -= __shfl_sync(0xffffffffu, incl - t, f);
+                const int pos0 = (b0 + f) * SMP_BLK + lane * (SMP_BLK / 32);
+                const T* x = reinterpret_cast<const T*>(data) + pos0;
+                u64 n = 0;
+                for (int i = 0; i < SMP_BLK / 32; ++i) n += float(x[i]) == lv.value;
+                const u64 n_incl = warp_scan_u64(n, lane);
+                if (n_incl >= left && n_incl - n < left) {
+                    u64 seen = n_incl - n;
+                    for (int i = 0; i < SMP_BLK / 32; ++i)
+                        if (float(x[i]) == lv.value && ++seen == left) sm.r[0] = rank_key(lv.value, token_at(pos0 + i));
+                }
+                break;
+            }
+        }
+        __syncthreads();
+        exchange(sm.r[0]);
+        u64 cut = 0;
+        for (int r = 0; r < size; ++r) cut = max(cut, got(0, r));
+        return cut;
     }
 
-    // ---- the draw over the slices: kept weights by blocks, ties counted apart
-    __device__ __forceinline__ void draw(Cut cut) {
-        if (cut.n_tie > 0 && cut.tie < l_min) cut.n_tie = 0;
-        cut.above = fmaxf(cut.above, just_below(l_min));
-        const bool ties = cut.n_tie > 0;
-        u64 sum_m = 0, sum_t = 0;
+    // A logit is kept when it is not below min-p's and its key not behind the cut.
+    __device__ __forceinline__ bool is_kept(float l, int pos, u64 cut, float cut_l) const {
+        return l >= l_min && (l > cut_l || (l == cut_l && rank_key(l, token_at(pos)) <= cut));
+    }
+    static __device__ __forceinline__ float cut_logit(u64 cut) { return cut == ~0ull ? -INFINITY : key_logit(cut); }
+    // the kept weights by blocks
+    __device__ __forceinline__ void sum_blocks(u64 cut) {
+        const float cut_l = cut_logit(cut);
+        __syncthreads();
         for (int b = warp; b < n_blk; b += SMP_WARPS) {
             u64 bm = 0;
-            uint32_t bt = 0;
-            each(b, [&](float l, int) {
-                if (l > cut.above) bm += weight(l);
-                if (ties && l == cut.tie) ++bt;
+            each(b, [&](float l, int pos) {
+                if (is_kept(l, pos, cut, cut_l)) bm += weight(l);
             });
             bm = warp_sum_u64(bm);
-            if (ties) bt = __reduce_add_sync(0xffffffffu, bt);
-            if (lane == 0) {
-                blk_mass()[b] = bm;
-                blk_tie()[b] = bt;
-                sum_m += bm;
-                sum_t += bt;
-            }
+            if (lane == 0) blk_mass()[b] = bm;
         }
-        cta_sum(sum_m, sum_t);
-        exchange(sum_m, sum_t);
+        __syncthreads();
+    }
 
-        // which CTA, which block, which position
-        const u64 w_tie = ties ? weight(cut.tie) : 0;
-        u64 total = 0, before = 0, mine = 0, ties_left = u64(cut.n_tie), my_ties = 0;
+    // ---- the draw over the slices, from the kept weights by blocks: which CTA, which block, which position
+    __device__ __forceinline__ void draw(u64 cut) {
+        u64 mine = 0, unused = 0;
+        for (int b = tid; b < n_blk; b += SMP_THREADS) mine += blk_mass()[b];
+        cta_sum(mine, unused);
+        exchange(mine);
+        u64 total = 0, before = 0;
         for (int r = 0; r < size; ++r) {
-            const u64 t = min(got(1, r), ties_left);
-            const u64 m = got(0, r) + t * w_tie;
-            if (r == rank) {
-                before = total;
-                mine = m;
-                my_ties = ties_left;
-            }
-            total += m;
-            ties_left -= t;
+            if (r < rank) before += got(0, r);
+            total += got(0, r);
         }
         u64 target = draw_target(total);
         if (target < before || target >= before + mine || warp != 0) return;  // the owner's first warp goes on
         target -= before;
+        const float cut_l = cut_logit(cut);
         for (int b0 = 0; b0 < n_blk; b0 += 32) {
-            const int b = b0 + lane;
-            const u64 t = b < n_blk && ties ? blk_tie()[b] : 0;
-            const u64 t_incl = warp_scan_u64(t, lane), t_excl = t_incl - t;
-            const u64 left = my_ties > t_excl ? my_ties - t_excl : 0;  // ties that this block may still keep
-            const u64 m = (b < n_blk ? blk_mass()[b] : 0) + min(t, left) * w_tie;
+            const u64 m = b0 + lane < n_blk ? blk_mass()[b0 + lane] : 0;
             const u64 m_incl = warp_scan_u64(m, lane);
             const unsigned hit = __ballot_sync(0xffffffffu, m_incl > target);
             if (!hit) {
                 target -= __shfl_sync(0xffffffffu, m_incl, 31);
-                const u64 seen = __shfl_sync(0xffffffffu, t_incl, 31);
-                my_ties = my_ties > seen ? my_ties - seen : 0;
                 continue;
             }
             const int f = __ffs(hit) - 1;
             target -= __shfl_sync(0xffffffffu, m_incl - m, f);
-            my_ties = __shfl_sync(0xffffffffu, left, f);
             // inside block b0 + f every lane takes 16 consecutive positions
             const int pos0 = (b0 + f) * SMP_BLK + lane * (SMP_BLK / 32);
             const T* x = reinterpret_cast<const T*>(data) + pos0;
-            u64 lt = 0;
-            for (int i = 0; i < SMP_BLK / 32; ++i) lt += ties && float(x[i]) == cut.tie;
-            const u64 lt_excl = warp_scan_u64(lt, lane) - lt;
-            const u64 lane_ties = my_ties > lt_excl ? my_ties - lt_excl : 0;
-            // the running sum over the lane's kept positions; returns the first that exceeds the target, or -1
-            auto walk = [&](u64& run, bool stop) -> int {
-                u64 seen = 0;
-                for (int i = 0; i < SMP_BLK / 32; ++i) {
-                    const float l = float(x[i]);
-                    if (l > cut.above) run += weight(l);
-                    else if (ties && l == cut.tie && seen++ < lane_ties) run += w_tie;
-                    if (stop && run > target) return i;
-                }
-                return -1;
-            };
             u64 lm = 0;
-            walk(lm, false);
+#pragma unroll 4
+            for (int i = 0; i < SMP_BLK / 32; ++i) {
+                const float l = float(x[i]);
+                if (is_kept(l, pos0 + i, cut, cut_l)) lm += weight(l);
+            }
             const u64 incl = warp_scan_u64(lm, lane);
             const unsigned lane_hit = __ballot_sync(0xffffffffu, incl > target);
             if (lane == __ffs(lane_hit) - 1) {
                 u64 run = incl - lm;
-                const int i = walk(run, true);
-                write(token_at(pos0 + i), log_share(float(x[i]), total));
+                for (int i = 0; i < SMP_BLK / 32; ++i) {
+                    const float l = float(x[i]);
+                    if (is_kept(l, pos0 + i, cut, cut_l)) run += weight(l);
+                    if (run > target) {
+                        write(token_at(pos0 + i), log_share(l, total));
+                        break;
+                    }
+                }
             }
             break;
         }
@@ -724,6 +1003,8 @@ struct Sampler {
     __device__ __forceinline__ void run() {
         if (tid < SMP_TABLE) sm.table[tid] = exp2(double(tid) / SMP_TABLE);
         if (tid == 0) sm.n_local = sm.n_list = sm.base = 0;
+        __syncthreads();
+        if (size > 1) cluster_arrive();
         // the row's settings (the same in every thread, so the branches are uniform over the cluster)
         temp = p.temperature ? double(p.temperature[row]) : p.temperature_all;
         k = p.top_k ? p.top_k[row] : p.top_k_all;
@@ -746,44 +1027,45 @@ struct Sampler {
         weight.scale = SMP_TABLE * k2;
         weight.table = sm.table;
         weight.frac = p.frac_bits;
-        if (warp == 0) {
-            const double x = lane == 1 && min_p > 0.0 ? fmax(SMP_FLOOR_LOG2, log2(fmin(min_p, 1.0))) : SMP_FLOOR_LOG2;
-            const float l = lowest_with(x, k2);
-            if (lane == 0) sm.l_floor = l;
-            if (lane == 1) sm.l_min = l;
-        }
-        __syncthreads();
-        l_floor = sm.l_floor;
-        l_min = sm.l_min;
+        l_floor = l_min = lowest_with(SMP_FLOOR_LOG2, k2);
+        if (min_p > 0.0) l_min = fmaxf(l_floor, lowest_with(fmax(SMP_FLOOR_LOG2, log2(fmin(min_p, 1.0))), k2));
         const bool want_p = top_p < 1.0;
         if (!k && !want_p) {
-            draw(Cut{-INFINITY, 0.0f, 0});
+            sum_blocks(~0ull);
+            draw(~0ull);
             return;
         }
         bin_scale = fminf(float(SMP_BINS) / (0.5f * mx - 0.5f * l_floor), 1e30f);
-        const bool by_mass = !k;  // top-k comes first: its counts decide
-        level0(by_mass);
-        u64 mass = 0, cnt = 0;
-        for (int r = 0; r < size; ++r) {
-            mass += got(0, r);
-            cnt += got(1, r);
-        }
-        u64 target;
-        if (by_mass) {
-            const double t = ceil(fmax(top_p, 0.0) * double(mass));
-            target = t < 1.0 ? 1ull : min((u64)t, mass);
+        u64 cut;
+        if (k) {  // top-k comes first, and is exact in the counts
+            level0(false);
+            exchange_totals();
+            u64 cnt = 0;
+            for (int r = 0; r < size; ++r) cnt += got(1, r);
+            const u64 target = min(u64(k), cnt);
+            const Border bd = find_border(false, target, 0, 0);
+            if (bd.cnt_above + bd.cnt <= SMP_LIST) {
+                finish_on_list(bd.bin, bd.owner, 0);
+                return;
+            }
+            cut = cut_by_levels(u64(k) < cnt, bd, target);
         } else {
-            target = min(u64(k), cnt);
+            const u64 sum = level0_counts_and_sum();
+            u64 mass, target;
+            const Window win = p_window(mass, target, sum);
+            if (win.all) {
+                finish_on_list(win.hi, win.owner, mass);
+                return;
+            }
+            cut = win.none ? 0 : cut_in_window(win, target);
+            if (cut) {
+                draw(cut);
+                return;
+            }
+            cut = cut_by_levels(false, Border{}, 0);
         }
-        const Border bd = find_border(by_mass, target, 0, 0);
-        if (bd.cnt_above + bd.cnt <= SMP_LIST) {
-            finish_on_list(bd.bin, bd.owner, mass);
-            return;
-        }
-        if (by_mass)
-            draw(cut_by_levels(bd, true, 0, target));
-        else
-            draw(cut_by_levels(bd, false, u64(k) < cnt ? u64(k) : 0, 0));
+        sum_blocks(cut);
+        draw(cut);
     }
 };
 
