@@ -331,7 +331,8 @@ int cce_b200_logits(const cce_b200_logits_args* a, void* workspace, size_t works
  * A setting is an array with one value per row, or (array NULL) the *_all value for every row; top_k <= 0
  * or >= V, top_p >= 1 and min_p <= 0 switch a filter off.  Sums are exact (64-bit fixed point), so the result
  * does not depend on the launch.  V is bounded by the shared memory of sixteen SMs (CCE_ERR_TOO_LARGE above
- * 2^20, or about 780 000 fp32 logits).  No workspace. */
+ * 2^20, or about 780 000 fp32 logits).  The workspace (256-byte aligned) carries no status word: these
+ * kernels wait for nothing but the hardware's barriers. */
 typedef struct cce_b200_sample_args {
     const void* logits;  /* [B][V], row stride ld elements */
     int64_t B, V, ld;
@@ -348,7 +349,8 @@ typedef struct cce_b200_sample_args {
     int64_t* tokens;     /* [B] */
     float* logprobs;     /* [B] or NULL */
 } cce_b200_sample_args;
-int cce_b200_sample(const cce_b200_sample_args* a, void* stream);
+size_t cce_b200_sample_workspace_bytes(const cce_b200_sample_args* a);
+int cce_b200_sample(const cce_b200_sample_args* a, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Synchronises `stream` and returns CCE_OK or CCE_ERR_KERNEL_WAIT; the raw word goes to *word.
  * Without this read an abandoned wait still shows: the log-sum-exp (hence the loss) and dE of that

@@ -16,6 +16,7 @@
 #include "engine_pair.cuh"
 #include "head_logits.cuh"
 #include "sample.cuh"
+#include "sample_stream.cuh"
 #include "small_kernels.cuh"
 
 using namespace cce;

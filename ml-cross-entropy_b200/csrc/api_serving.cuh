@@ -141,26 +141,96 @@ int make_tmap_adapters(CUtensorMap* m, const void* base, int dtype, long long ra
     return CCE_OK;
 }
 
-template <typename T>
-int launch_sample(const SampleParams& sp, int cluster, int smem, long long B, cudaStream_t st) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(B * cluster));
-    cfg.blockDim = dim3(SMP_THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, sample_kernel<T>, sp);
-    CCE_LAUNCH_CHECK();
+// Positions per CTA for a row of V logits over `cluster` CTAs: whole blocks.
+inline int sample_slice(long long V, int cluster) { return int(cdiv(cdiv(V, cluster), SMP_BLK) * SMP_BLK); }
+
+struct SamplePlan {
+    int cluster, slice, smem;  // of sample_kernel
+    bool stream, filters;      // sample_stream.cuh's kernels; with top-k or top-p
+    int n_chunk;
+    size_t off_max, off_sum, off_blk, off_hist, off_list, total;
+};
+
+int plan_sample(const cce_b200_sample_args* a, SamplePlan* out) {
+    if (!a || a->B < 0 || a->V <= 0 || a->ld < a->V) return CCE_ERR_ARG;
+    if (a->dtype != CCE_DT_F16 && a->dtype != CCE_DT_BF16 && a->dtype != CCE_DT_F32) return CCE_ERR_ARG;
+    SamplePlan pl = {};
+    const int elem = a->dtype == CCE_DT_F32 ? 4 : 2;
+    if (a->V > (1 << 20)) return CCE_ERR_TOO_LARGE;  // the weights keep at least 42 bits
+    // CTAs per row.  Few rows: short slices (1 x 256000 fp32: 22.5 us with 16384 positions, 24.6 with 32768);
+    // many rows: fewer, longer ones, whose fixed cost is paid less often (512 x 152064: 803 us against 1360).
+    const int longest = a->B >= 32 ? 32768 : 16384;
+    pl.cluster = 1;
+    while (pl.cluster < SMP_MAX_CLUSTER && sample_slice(a->V, pl.cluster) > longest) pl.cluster *= 2;
+    pl.slice = sample_slice(a->V, pl.cluster);
+    pl.smem = SampleLayout(pl.cluster, pl.slice, elem).bytes;
+    if (pl.smem > SMP_SMEM) return CCE_ERR_TOO_LARGE;
+    if (a->B * pl.cluster >= (1LL << 31)) return CCE_ERR_ARG;
+    pl.filters = a->top_k || a->top_p || a->top_k_all > 0 || a->top_p_all < 1.0;
+    static const long long kStream = getenv("STREAM") ? atoll(getenv("STREAM")) : (8LL << 20);
+    pl.stream = a->B * a->V >= kStream;
+    pl.total = 256;
+    if (pl.stream) {
+        pl.n_chunk = (int)cdiv(a->V + 16 / elem - 1, STR_CHUNK);
+        if (a->B * pl.n_chunk >= (1LL << 31)) return CCE_ERR_ARG;
+        size_t off = align_up((size_t)a->B * sizeof(RowState), 256);
+        auto take = [&](size_t bytes) {
+            const size_t at = off;
+            off = align_up(off + bytes, 256);
+            return at;
+        };
+        const size_t chunks = (size_t)a->B * pl.n_chunk;
+        pl.off_max = take(chunks * sizeof(float));
+        pl.off_sum = take(chunks * sizeof(u64));
+        pl.off_blk = take(chunks * STR_BLOCKS * sizeof(u64));
+        pl.off_hist = take(pl.filters ? (size_t)a->B * SMP_BINS * sizeof(uint32_t) : 0);
+        pl.off_list = take(pl.filters ? (size_t)a->B * SMP_LIST * sizeof(u64) : 0);
+        pl.total = off;
+    }
+    *out = pl;
     return CCE_OK;
 }
 
-// Positions per CTA for a row of V logits over `cluster` CTAs: whole blocks.
-inline int sample_slice(long long V, int cluster) { return int(cdiv(cdiv(V, cluster), SMP_BLK) * SMP_BLK); }
+template <typename T>
+int launch_sample(const SampleParams& sp, const SamplePlan& pl, long long B, char* ws, cudaStream_t st) {
+    RowState* only = nullptr;
+    if (pl.stream) {
+        StreamBuffers b = {};
+        b.state = reinterpret_cast<RowState*>(ws);
+        b.chunk_max = reinterpret_cast<float*>(ws + pl.off_max);
+        b.chunk_sum = reinterpret_cast<u64*>(ws + pl.off_sum);
+        b.blk_mass = reinterpret_cast<u64*>(ws + pl.off_blk);
+        b.hist = pl.filters ? reinterpret_cast<uint32_t*>(ws + pl.off_hist) : nullptr;
+        b.list = reinterpret_cast<u64*>(ws + pl.off_list);
+        b.n_chunk = pl.n_chunk;
+        const dim3 chunks((unsigned)(B * pl.n_chunk)), rows((unsigned)B);
+        const int draw_smem = (3 * SMP_LIST + pl.n_chunk * STR_BLOCKS) * (int)sizeof(u64);
+        int rc = launch_behind(row_max_kernel<T>, chunks, SMP_THREADS, 0, st, false, sp, b);
+        if (!rc && !pl.filters) rc = launch_behind(row_stats_kernel<T, false>, chunks, SMP_THREADS, 0, st, true, sp, b);
+        if (!rc && pl.filters) rc = launch_behind(row_stats_kernel<T, true>, chunks, SMP_THREADS, 0, st, true, sp, b);
+        if (!rc && pl.filters) rc = launch_behind(row_plan_kernel, rows, SMP_THREADS, 0, st, true, sp, b);
+        if (!rc && pl.filters) rc = launch_behind(row_pass_kernel<T>, chunks, SMP_THREADS, 0, st, true, sp, b);
+        if (!rc) rc = launch_behind(row_draw_kernel<T>, rows, SMP_THREADS, draw_smem, st, true, sp, b);
+        if (rc || !pl.filters) return rc;
+        only = b.state;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(B * pl.cluster));
+    cfg.blockDim = dim3(SMP_THREADS);
+    cfg.dynamicSmemBytes = pl.smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = pl.cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = only ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, sample_kernel<T>, sp, (const RowState*)only);
+    CCE_LAUNCH_CHECK();
+    return CCE_OK;
+}
 
 }  // namespace
 
@@ -305,26 +375,24 @@ int cce_b200_logits(const cce_b200_logits_args* a, void* workspace, size_t works
     return launch_head<__half>(maps, hp, grid, st);
 }
 
-int cce_b200_sample(const cce_b200_sample_args* a, void* stream) {
-    if (!a || a->B < 0 || a->V <= 0 || a->ld < a->V) return CCE_ERR_ARG;
-    if (a->dtype != CCE_DT_F16 && a->dtype != CCE_DT_BF16 && a->dtype != CCE_DT_F32) return CCE_ERR_ARG;
-    if (a->B == 0) return CCE_OK;
-    if (!a->logits || !a->u || !a->tokens) return CCE_ERR_ARG;
-    const int elem = a->dtype == CCE_DT_F32 ? 4 : 2;
-    if (reinterpret_cast<uintptr_t>(a->logits) % elem) return CCE_ERR_ALIGN;
-    DeviceInfo* dev;
-    int rc = device_info(&dev);
+size_t cce_b200_sample_workspace_bytes(const cce_b200_sample_args* a) {
+    SamplePlan pl;
+    return plan_sample(a, &pl) ? 0 : pl.total;
+}
+
+int cce_b200_sample(const cce_b200_sample_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+    SamplePlan pl;
+    int rc = plan_sample(a, &pl);
     if (rc) return rc;
-    // CTAs per row.  Few rows: short slices (1 x 256000 fp32: 22.5 us with 16384 positions, 24.6 with 32768);
-    // many rows: fewer, longer ones, whose fixed cost is paid less often (512 x 152064: 803 us against 1360).
-    int cluster = 1;
-    const int longest = a->B >= 32 ? 32768 : 16384;
-    if (a->V > (1 << 20)) return CCE_ERR_TOO_LARGE;  // the weights keep at least 42 bits
-    while (cluster < SMP_MAX_CLUSTER && sample_slice(a->V, cluster) > longest) cluster *= 2;
-    const int slice = sample_slice(a->V, cluster);
-    const SampleLayout lay(cluster, slice, elem);
-    if (lay.bytes > SMP_SMEM) return CCE_ERR_TOO_LARGE;
-    if (a->B * cluster >= (1LL << 31)) return CCE_ERR_ARG;
+    if (a->B == 0) return CCE_OK;
+    if (!a->logits || !a->u || !a->tokens || !workspace) return CCE_ERR_ARG;
+    if (workspace_bytes < pl.total) return CCE_ERR_WORKSPACE;
+    if ((reinterpret_cast<uintptr_t>(workspace) & 255) ||
+        reinterpret_cast<uintptr_t>(a->logits) % (a->dtype == CCE_DT_F32 ? 4 : 2))
+        return CCE_ERR_ALIGN;
+    DeviceInfo* dev;
+    rc = device_info(&dev);
+    if (rc) return rc;
     SampleParams sp = {};
     sp.logits = a->logits;
     sp.ld = a->ld;
@@ -340,14 +408,15 @@ int cce_b200_sample(const cce_b200_sample_args* a, void* stream) {
     sp.min_p_all = a->min_p_all;
     sp.tokens = reinterpret_cast<long long*>(a->tokens);
     sp.logprobs = a->logprobs;
-    sp.slice = slice;
+    sp.slice = pl.slice;
     int log2v = 0;
     while ((1LL << log2v) < a->V) ++log2v;
     sp.frac_bits = std::min(50, 62 - log2v);  // V weights of at most 1 << frac_bits stay below 2^63
+    char* ws = reinterpret_cast<char*>(workspace);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (a->dtype == CCE_DT_F32) return launch_sample<float>(sp, cluster, lay.bytes, a->B, st);
-    if (a->dtype == CCE_DT_BF16) return launch_sample<__nv_bfloat16>(sp, cluster, lay.bytes, a->B, st);
-    return launch_sample<__half>(sp, cluster, lay.bytes, a->B, st);
+    if (a->dtype == CCE_DT_F32) return launch_sample<float>(sp, pl, a->B, ws, st);
+    if (a->dtype == CCE_DT_BF16) return launch_sample<__nv_bfloat16>(sp, pl, a->B, ws, st);
+    return launch_sample<__half>(sp, pl, a->B, ws, st);
 }
 
 }  // extern "C"

@@ -100,9 +100,6 @@ __host__ __device__ inline int h16_pitch(int rank) { return rank <= 32 ? 64 : (r
 template <typename T>
 __device__ __forceinline__ float to_float(T x) { return float(x); }
 
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 __device__ __forceinline__ int group_adapter(const HeadParams& p, int g) {
     const int a = p.group[g];
     return a >= 0 && p.group_bad[g] ? GROUP_MIXED : a;

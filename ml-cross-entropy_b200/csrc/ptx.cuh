@@ -13,6 +13,11 @@
 
 namespace cce {
 
+// Programmatic dependent launch: wait for the kernel before this one in the stream (whose writes are then visible), and
+// allow the next one to start.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }

@@ -127,11 +127,15 @@ struct SampleLayout {
     }
 };
 
-struct SmpShared {
+// Shared memory of a CTA's sums and scans.
+struct CtaScratch {
     double table[SMP_TABLE];
-    u64 x[2][4][SMP_MAX_CLUSTER];  // exchange slots, written by the whole cluster
     u64 wa[SMP_WARPS], wb[SMP_WARPS];
     u64 r[4];
+};
+
+struct SmpShared : CtaScratch {
+    u64 x[2][4][SMP_MAX_CLUSTER];  // exchange slots, written by the whole cluster
     float wf[SMP_WARPS];
     uint32_t n_local, n_list, base;
     int lo, hi, all;
@@ -214,40 +218,211 @@ __device__ __forceinline__ int sort_size(int n) {
     return m;
 }
 
+// How the kernels of sample_stream.cuh go on with a row.
+enum RowMode { ROW_DONE, ROW_GREEDY, ROW_SUM, ROW_LIST, ROW_WINDOW, ROW_BY_CLUSTER };
+struct RowState {
+    int mode;
+    int lo, hi;        // window of bins; ROW_LIST: bins 0..hi
+    unsigned first;    // ROW_GREEDY: the lowest index of the largest logits
+    unsigned n_list;
+    u64 mass, target;  // top-p alone: all weights, and the running sum to reach
+};
+
+// What a row's kernels share: its settings, its thresholds, and the arithmetic on them.
+struct RowBase {
+    const SampleParams& p;
+    CtaScratch& sc;
+    long long row;
+    int tid, warp, lane;
+    float mx, l_floor, l_min, bin_scale;
+    double temp, top_p;
+    float u;
+    long long k;  // 0: off
+    WeightFn weight;
+
+    __device__ __forceinline__ RowBase(const SampleParams& p_, CtaScratch& sc_, long long row_) : p(p_), sc(sc_), row(row_) {
+        tid = threadIdx.x;
+        warp = tid >> 5;
+        lane = tid & 31;
+        // the same in every thread, so that the branches on them are uniform
+        temp = p.temperature ? double(p.temperature[row]) : p.temperature_all;
+        k = p.top_k ? p.top_k[row] : p.top_k_all;
+        top_p = p.top_p ? double(p.top_p[row]) : p.top_p_all;
+        u = p.u[row];
+        if (k <= 0 || k >= p.V) k = 0;
+    }
+    __device__ __forceinline__ bool greedy_row() const { return !(temp > 0.0) || k == 1; }
+    __device__ __forceinline__ void make_table() {
+        if (tid < SMP_TABLE) sc.table[tid] = exp2(double(tid) / SMP_TABLE);
+    }
+    // from the row's maximum (above -inf): the weights and the thresholds
+    __device__ __forceinline__ void prepare(float m) {
+        mx = m + 0.0f;
+        const double min_p = p.min_p ? double(p.min_p[row]) : p.min_p_all;
+        const double k2 = 1.4426950408889634074 / temp;  // exponents of 2 per unit of logit
+        weight.m = double(mx);
+        weight.peak = mx;
+        weight.scale = SMP_TABLE * k2;
+        weight.table = sc.table;
+        weight.frac = p.frac_bits;
+        l_floor = l_min = lowest_with(SMP_FLOOR_LOG2, k2);
+        if (min_p > 0.0) l_min = fmaxf(l_floor, lowest_with(fmax(SMP_FLOOR_LOG2, log2(fmin(min_p, 1.0))), k2));
+        bin_scale = fminf(float(SMP_BINS) / (0.5f * mx - 0.5f * l_floor), 1e30f);
+    }
+    // The smallest logit whose weight is at least 2^x (x <= 0): a first guess, then the neighbours.  A weight
+    // that rounds to 1 in fp64, exp(z) with z >= -2^-54, counts as 1.
+    __device__ __forceinline__ float lowest_with(double x, double k2) const {
+        if (isinf(mx)) return mx;
+        x = fmin(x, -8.0e-17);  // -2^-54 log2(e)
+        float g = float(double(mx) + x / k2);
+        if (!(g > SMP_LOWEST)) g = SMP_LOWEST;
+        for (int it = 0; it < 4 && g < mx && (double(g) - double(mx)) * k2 < x; ++it) g = order_value(order_key(g) + 1);
+        for (int it = 0; it < 4 && g > SMP_LOWEST; ++it) {
+            const float below = just_below(g);
+            if ((double(below) - double(mx)) * k2 < x) break;
+            g = below;
+        }
+        return g;
+    }
+
+    // ---- histogram level 0: bins linear in the logit, bin 0 at the maximum (halves: the difference of two floats
+    // may overflow).  The bin falls, or stays, as the logit grows.
+    __device__ __forceinline__ int bin0(float l) const {
+        return min(SMP_BINS - 1, int((0.5f * mx - 0.5f * l) * bin_scale));
+    }
+    // the running sum that top-p has to reach, of the mass it is measured by
+    __device__ __forceinline__ u64 p_target(u64 mass) const {
+        const double t = ceil(fmax(top_p, 0.0) * double(mass));
+        return t < 1.0 ? 1ull : min((u64)t, mass);
+    }
+
+    __device__ __forceinline__ void write(long long token, float logprob) const {
+        p.tokens[row] = token;
+        if (p.logprobs) p.logprobs[row] = logprob;
+    }
+    // log of a kept logit's share of the kept weights
+    __device__ __forceinline__ float log_share(float l, u64 total) const {
+        const double y = l == mx ? 0.0 : (double(l) - double(mx)) / temp;
+        return float(y - log(double(total) * exp2(-double(p.frac_bits))));
+    }
+    // the running sum that the drawn token is the first to exceed
+    __device__ __forceinline__ u64 draw_target(u64 total) const {
+        const double x = double(u) * double(total);
+        if (!(x > 0.0)) return 0;
+        return x >= double(total) ? total - 1 : min((u64)x, total - 1);
+    }
+
+    // sum of two values over the CTA's threads, in every thread
+    __device__ __forceinline__ void cta_sum(u64& a, u64& b) {
+        a = warp_sum_u64(a);
+        b = warp_sum_u64(b);
+        __syncthreads();
+        if (lane == 0) {
+            sc.wa[warp] = a;
+            sc.wb[warp] = b;
+        }
+        __syncthreads();
+        a = b = 0;
+#pragma unroll
+        for (int w = 0; w < SMP_WARPS; ++w) {
+            a += sc.wa[w];
+            b += sc.wb[w];
+        }
+    }
+    // inclusive scans of two values over the CTA's threads
+    __device__ __forceinline__ void cta_scan(u64& a, u64& b) {
+        a = warp_scan_u64(a, lane);
+        b = warp_scan_u64(b, lane);
+        __syncthreads();
+        if (lane == 31) {
+            sc.wa[warp] = a;
+            sc.wb[warp] = b;
+        }
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) {
+            a += sc.wa[w];
+            b += sc.wb[w];
+        }
+    }
+
+    // A logit and its token as one number: ascending = falling logits, ties by the lower index.
+    __device__ __forceinline__ u64 rank_key(float l, long long token) const { return u64(~order_key(l)) << 32 | u64(token); }
+    static __device__ __forceinline__ float key_logit(u64 key) { return order_value(~uint32_t(key >> 32)); }
+
+    // A logit is kept when it is not below min-p's and its key not behind the cut.
+    __device__ __forceinline__ bool is_kept(float l, long long token, u64 cut, float cut_l) const {
+        return l >= l_min && (l > cut_l || (l == cut_l && rank_key(l, token) <= cut));
+    }
+    static __device__ __forceinline__ float cut_logit(u64 cut) { return cut == ~0ull ? -INFINITY : key_logit(cut); }
+
+    // The rest of a row on the sorted list of its n largest logits (all that any prefix can keep; list in shared memory,
+    // like the two others of SMP_LIST entries): applies the three prefixes and draws.  mass: of all weights, for top-p
+    // without top-k.
+    __device__ __forceinline__ void draw_from_list(const u64* list, int n, u64* weights, u64* by_index, u64 mass) {
+        const int n_k = k && k < n ? int(k) : n;
+        u64 w[2];
+        float l[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int j = 2 * tid + i;
+            l[i] = j < n_k ? key_logit(list[j]) : -INFINITY;
+            w[i] = j < n_k ? weight(l[i]) : 0;
+            if (j < n_k) weights[j] = w[i];
+        }
+        u64 cum = w[0] + w[1], above_min = u64(l[0] >= l_min) + u64(l[1] >= l_min);
+        cta_scan(cum, above_min);
+        if (2 * tid < n_k && 2 * tid + 2 >= n_k) sc.r[0] = cum;  // sum over the first k
+        if (tid == SMP_THREADS - 1) sc.r[1] = above_min;
+        __syncthreads();
+        int kept = max(1, int(min(u64(n_k), sc.r[1])));
+        if (top_p < 1.0) {
+            const u64 target = p_target(k ? sc.r[0] : mass);
+            // the first whose running sum reaches it
+            int n_p = __syncthreads_count(2 * tid < n_k && cum - w[1] < target);
+            n_p += __syncthreads_count(2 * tid + 1 < n_k && cum < target);
+            kept = min(kept, n_p + 1);
+        }
+        // the kept weights' sum, and the kept candidates in order of their index
+        if ((kept - 1) >> 1 == tid) sc.r[2] = (kept & 1) ? cum - w[1] : cum;
+        const int m = sort_size(kept);
+        for (int j = tid; j < m; j += SMP_THREADS) by_index[j] = j < kept ? (list[j] << 32 | u64(j)) : ~0ull;
+        bitonic_sort(by_index, m);
+        const u64 total = sc.r[2], target = draw_target(total);
+        u64 v[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) v[i] = 2 * tid + i < kept ? weights[uint32_t(by_index[2 * tid + i])] : 0;
+        u64 run = v[0] + v[1], unused = 0;
+        cta_scan(run, unused);
+        if (run > target && run - v[0] - v[1] <= target) {  // one thread
+            const u64 e = by_index[2 * tid + (run - v[1] > target ? 0 : 1)];
+            write((long long)(e >> 32), log_share(key_logit(list[uint32_t(e)]), total));
+        }
+    }
+
+};
+
 template <typename T>
-struct Sampler {
+struct Sampler : RowBase {
     static constexpr int VE = 16 / int(sizeof(T));
     static constexpr int CHUNKS = SMP_BLK / VE / 32;  // 16-byte chunks per lane and block
 
-    const SampleParams& p;
     SmpShared& sm;
     uint8_t* dyn;
     SampleLayout lay;
     cooperative_groups::cluster_group cl;
     int rank, size, buf = 0;
-    long long row;
-    int tid, warp, lane;
     // the slice: positions are counted from the 16-byte boundary at or below its first element, so that whole
     // 16-byte pieces of global memory land on 16-byte pieces of shared memory at any alignment; positions
     // outside the slice hold -inf
     uint4* data;
     long long start;
     int phase, n_blk;
-    float mx, l_floor, l_min, bin_scale;
-    double temp, top_p;
-    float u;
-    long long k;
-    WeightFn weight;
 
-    __device__ __forceinline__ Sampler(const SampleParams& p_, SmpShared& sm_, uint8_t* dyn_)
-        : p(p_), sm(sm_), dyn(dyn_), lay(int(cooperative_groups::this_cluster().num_blocks()), p_.slice, int(sizeof(T))),
+    __device__ __forceinline__ Sampler(const SampleParams& p_, SmpShared& sm_, uint8_t* dyn_, int cluster)
+        : RowBase(p_, sm_, blockIdx.x / cluster), sm(sm_), dyn(dyn_), lay(cluster, p_.slice, int(sizeof(T))),
           cl(cooperative_groups::this_cluster()) {
         rank = int(cl.block_rank());
-        size = int(cl.num_blocks());
-        row = blockIdx.x / size;
-        tid = threadIdx.x;
-        warp = tid >> 5;
-        lane = tid & 31;
+        size = cluster;
         data = reinterpret_cast<uint4*>(dyn + lay.data);
     }
     __device__ __forceinline__ u64* hist_mass() const { return reinterpret_cast<u64*>(dyn + lay.hist_mass); }
@@ -301,55 +476,6 @@ struct Sampler {
         cl.sync();
     }
     __device__ __forceinline__ u64 got(int i, int r) const { return sm.x[buf][i][r]; }
-    // sum of two values over the CTA's threads, in every thread
-    __device__ __forceinline__ void cta_sum(u64& a, u64& b) {
-        a = warp_sum_u64(a);
-        b = warp_sum_u64(b);
-        __syncthreads();
-        if (lane == 0) {
-            sm.wa[warp] = a;
-            sm.wb[warp] = b;
-        }
-        __syncthreads();
-        a = b = 0;
-#pragma unroll
-        for (int w = 0; w < SMP_WARPS; ++w) {
-            a += sm.wa[w];
-            b += sm.wb[w];
-        }
-    }
-    // inclusive scans of two values over the CTA's threads
-    __device__ __forceinline__ void cta_scan(u64& a, u64& b) {
-        a = warp_scan_u64(a, lane);
-        b = warp_scan_u64(b, lane);
-        __syncthreads();
-        if (lane == 31) {
-            sm.wa[warp] = a;
-            sm.wb[warp] = b;
-        }
-        __syncthreads();
-        for (int w = 0; w < warp; ++w) {
-            a += sm.wa[w];
-            b += sm.wb[w];
-        }
-    }
-
-    __device__ __forceinline__ void write(long long token, float logprob) const {
-        p.tokens[row] = token;
-        if (p.logprobs) p.logprobs[row] = logprob;
-    }
-    // log of a kept logit's share of the kept weights
-    __device__ __forceinline__ float log_share(float l, u64 total) const {
-        const double y = l == mx ? 0.0 : (double(l) - double(mx)) / temp;
-        return float(y - log(double(total) * exp2(-double(p.frac_bits))));
-    }
-    // the running sum that the drawn token is the first to exceed
-    __device__ __forceinline__ u64 draw_target(u64 total) const {
-        const double x = double(u) * double(total);
-        if (!(x > 0.0)) return 0;
-        return x >= double(total) ? total - 1 : min((u64)x, total - 1);
-    }
-
     // ---- the slice to shared memory, and the row's maximum
     __device__ __forceinline__ void load() {
         start = (long long)rank * p.slice;
@@ -419,27 +545,6 @@ struct Sampler {
         }
     }
 
-    // The smallest logit whose weight is at least 2^x (x <= 0): a first guess, then the neighbours.  A weight
-    // that rounds to 1 in fp64, exp(z) with z >= -2^-54, counts as 1.
-    __device__ __forceinline__ float lowest_with(double x, double k2) const {
-        if (isinf(mx)) return mx;
-        x = fmin(x, -8.0e-17);  // -2^-54 log2(e)
-        float g = float(double(mx) + x / k2);
-        if (!(g > SMP_LOWEST)) g = SMP_LOWEST;
-        for (int it = 0; it < 4 && g < mx && (double(g) - double(mx)) * k2 < x; ++it) g = order_value(order_key(g) + 1);
-        for (int it = 0; it < 4 && g > SMP_LOWEST; ++it) {
-            const float below = just_below(g);
-            if ((double(below) - double(mx)) * k2 < x) break;
-            g = below;
-        }
-        return g;
-    }
-
-    // ---- histogram level 0: bins linear in the logit, bin 0 at the maximum (halves: the difference of two floats
-    // may overflow).  The bin falls, or stays, as the logit grows.
-    __device__ __forceinline__ int bin0(float l) const {
-        return min(SMP_BINS - 1, int((0.5f * mx - 0.5f * l) * bin_scale));
-    }
     __device__ __forceinline__ void clear_hist(bool mass) {
         for (int b = tid; b < SMP_BINS; b += SMP_THREADS) {
             hist_cnt()[b] = 0;
@@ -556,12 +661,6 @@ struct Sampler {
         merge_hist(false);
         return sum;
     }
-    // the running sum that top-p has to reach, of the mass it is measured by
-    __device__ __forceinline__ u64 p_target(u64 mass) const {
-        const double t = ceil(fmax(top_p, 0.0) * double(mass));
-        return t < 1.0 ? 1ull : min((u64)t, mass);
-    }
-
     // The first key of [lo, hi] that fulfils a predicate which holds from some key on (hi if none before it does),
     // by all threads together
     template <typename F>
@@ -609,10 +708,6 @@ struct Sampler {
         return Level{order_value(lo), bd.mass_above, bd.cnt_above};
     }
 
-    // A logit and its token as one number: ascending = falling logits, ties by the lower index.
-    __device__ __forceinline__ u64 rank_key(float l, long long token) const { return u64(~order_key(l)) << 32 | u64(token); }
-    static __device__ __forceinline__ float key_logit(u64 key) { return order_value(~uint32_t(key >> 32)); }
-
     // This CTA's candidates: up to SMP_LIST, in hist_mass()[0 .. n_local).
     __device__ __forceinline__ void collect(float l, int pos) {
         hist_mass()[atomicAdd(&sm.n_local, 1u)] = rank_key(l, token_at(pos));
@@ -645,48 +740,8 @@ struct Sampler {
         send_candidates(leader);
         if (size > 1) cl.sync(); else __syncthreads();
         if (rank != leader) return;
-        u64* const weights = hist_mass();               // in place of the leader's own candidates
-        const u64* const list = hist_mass() + SMP_LIST;
-        u64* const by_index = reinterpret_cast<u64*>(hist_cnt());
         const int n = sort_candidates();
-        const int n_k = k && k < n ? int(k) : n;
-        u64 w[2];
-        float l[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int j = 2 * tid + i;
-            l[i] = j < n_k ? key_logit(list[j]) : -INFINITY;
-            w[i] = j < n_k ? weight(l[i]) : 0;
-            if (j < n_k) weights[j] = w[i];
-        }
-        u64 cum = w[0] + w[1], above_min = u64(l[0] >= l_min) + u64(l[1] >= l_min);
-        cta_scan(cum, above_min);
-        if (2 * tid < n_k && 2 * tid + 2 >= n_k) sm.r[0] = cum;  // sum over the first k
-        if (tid == SMP_THREADS - 1) sm.r[1] = above_min;
-        __syncthreads();
-        int kept = max(1, int(min(u64(n_k), sm.r[1])));
-        if (top_p < 1.0) {
-            const u64 target = p_target(k ? sm.r[0] : mass);
-            // the first whose running sum reaches it
-            int n_p = __syncthreads_count(2 * tid < n_k && cum - w[1] < target);
-            n_p += __syncthreads_count(2 * tid + 1 < n_k && cum < target);
-            kept = min(kept, n_p + 1);
-        }
-        // the kept weights' sum, and the kept candidates in order of their index
-        if ((kept - 1) >> 1 == tid) sm.r[2] = (kept & 1) ? cum - w[1] : cum;
-        const int m = sort_size(kept);
-        for (int j = tid; j < m; j += SMP_THREADS) by_index[j] = j < kept ? (list[j] << 32 | u64(j)) : ~0ull;
-        bitonic_sort(by_index, m);
-        const u64 total = sm.r[2], target = draw_target(total);
-        u64 v[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) v[i] = 2 * tid + i < kept ? weights[uint32_t(by_index[2 * tid + i])] : 0;
-        u64 run = v[0] + v[1], unused = 0;
-        cta_scan(run, unused);
-        if (run > target && run - v[0] - v[1] <= target) {  // one thread
-            const u64 e = by_index[2 * tid + (run - v[1] > target ? 0 : 1)];
-            write((long long)(e >> 32), log_share(key_logit(list[uint32_t(e)]), total));
-        }
+        draw_from_list(hist_mass() + SMP_LIST, n, hist_mass(), reinterpret_cast<u64*>(hist_cnt()), mass);
     }
 
     // ---- top-p alone: where the mass reaches the target, estimated from the counts (every weight of a bin as its
@@ -929,11 +984,6 @@ struct Sampler {
         return cut;
     }
 
-    // A logit is kept when it is not below min-p's and its key not behind the cut.
-    __device__ __forceinline__ bool is_kept(float l, int pos, u64 cut, float cut_l) const {
-        return l >= l_min && (l > cut_l || (l == cut_l && rank_key(l, token_at(pos)) <= cut));
-    }
-    static __device__ __forceinline__ float cut_logit(u64 cut) { return cut == ~0ull ? -INFINITY : key_logit(cut); }
     // the kept weights by blocks
     __device__ __forceinline__ void sum_blocks(u64 cut) {
         const float cut_l = cut_logit(cut);
@@ -941,7 +991,7 @@ struct Sampler {
         for (int b = warp; b < n_blk; b += SMP_WARPS) {
             u64 bm = 0;
             each(b, [&](float l, int pos) {
-                if (is_kept(l, pos, cut, cut_l)) bm += weight(l);
+                if (is_kept(l, token_at(pos), cut, cut_l)) bm += weight(l);
             });
             bm = warp_sum_u64(bm);
             if (lane == 0) blk_mass()[b] = bm;
@@ -981,7 +1031,7 @@ struct Sampler {
 #pragma unroll 4
             for (int i = 0; i < SMP_BLK / 32; ++i) {
                 const float l = float(x[i]);
-                if (is_kept(l, pos0 + i, cut, cut_l)) lm += weight(l);
+                if (is_kept(l, token_at(pos0 + i), cut, cut_l)) lm += weight(l);
             }
             const u64 incl = warp_scan_u64(lm, lane);
             const unsigned lane_hit = __ballot_sync(0xffffffffu, incl > target);
@@ -989,7 +1039,7 @@ struct Sampler {
                 u64 run = incl - lm;
                 for (int i = 0; i < SMP_BLK / 32; ++i) {
                     const float l = float(x[i]);
-                    if (is_kept(l, pos0 + i, cut, cut_l)) run += weight(l);
+                    if (is_kept(l, token_at(pos0 + i), cut, cut_l)) run += weight(l);
                     if (run > target) {
                         write(token_at(pos0 + i), log_share(l, total));
                         break;
@@ -1001,41 +1051,26 @@ struct Sampler {
     }
 
     __device__ __forceinline__ void run() {
-        if (tid < SMP_TABLE) sm.table[tid] = exp2(double(tid) / SMP_TABLE);
+        make_table();
         if (tid == 0) sm.n_local = sm.n_list = sm.base = 0;
         __syncthreads();
         if (size > 1) cluster_arrive();
-        // the row's settings (the same in every thread, so the branches are uniform over the cluster)
-        temp = p.temperature ? double(p.temperature[row]) : p.temperature_all;
-        k = p.top_k ? p.top_k[row] : p.top_k_all;
-        top_p = p.top_p ? double(p.top_p[row]) : p.top_p_all;
-        const double min_p = p.min_p ? double(p.min_p[row]) : p.min_p_all;
-        u = p.u[row];
-        if (k <= 0 || k >= p.V) k = 0;
         load();
         if (!(mx > -INFINITY)) {  // nothing to draw from
             if (rank == 0 && tid == 0) write(-1, -INFINITY);
             return;
         }
-        if (!(temp > 0.0) || k == 1) {
+        if (greedy_row()) {
             greedy();
             return;
         }
-        const double k2 = 1.4426950408889634074 / temp;  // exponents of 2 per unit of logit
-        weight.m = double(mx);
-        weight.peak = mx;
-        weight.scale = SMP_TABLE * k2;
-        weight.table = sm.table;
-        weight.frac = p.frac_bits;
-        l_floor = l_min = lowest_with(SMP_FLOOR_LOG2, k2);
-        if (min_p > 0.0) l_min = fmaxf(l_floor, lowest_with(fmax(SMP_FLOOR_LOG2, log2(fmin(min_p, 1.0))), k2));
+        prepare(mx);
         const bool want_p = top_p < 1.0;
         if (!k && !want_p) {
             sum_blocks(~0ull);
             draw(~0ull);
             return;
         }
-        bin_scale = fminf(float(SMP_BINS) / (0.5f * mx - 0.5f * l_floor), 1e30f);
         u64 cut;
         if (k) {  // top-k comes first, and is exact in the counts
             level0(false);
@@ -1069,12 +1104,18 @@ struct Sampler {
     }
 };
 
+// only: null, or the rows' states, of which those in ROW_BY_CLUSTER are sampled
 template <typename T>
 __global__ void __launch_bounds__(SMP_THREADS, 2)
-sample_kernel(const SampleParams p) {
+sample_kernel(const SampleParams p, const RowState* only) {
     extern __shared__ __align__(16) uint8_t dyn[];
     __shared__ SmpShared sm;
-    Sampler<T> s(p, sm, dyn);
+    const int cluster = int(cooperative_groups::this_cluster().num_blocks());
+    if (only) {
+        pdl_wait();
+        if (only[blockIdx.x / cluster].mode != ROW_BY_CLUSTER) return;
+    }
+    Sampler<T> s(p, sm, dyn, cluster);
     s.run();
 }
 

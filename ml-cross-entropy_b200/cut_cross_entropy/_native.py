@@ -48,6 +48,7 @@ EXPORTS = (
     "cce_b200_de_peer_scatter",
     "cce_b200_logits_workspace_bytes",
     "cce_b200_logits",
+    "cce_b200_sample_workspace_bytes",
     "cce_b200_sample",
     "cce_b200_gemm",
     "cce_b200_read_status",
@@ -239,7 +240,9 @@ def lib() -> ctypes.CDLL:
     L.cce_b200_logits.restype = c_int32
     L.cce_b200_logits.argtypes = [POINTER(LogitsArgs), c_void_p, c_size_t, c_void_p]
     L.cce_b200_sample.restype = c_int32
-    L.cce_b200_sample.argtypes = [POINTER(SampleArgs), c_void_p]
+    L.cce_b200_sample.argtypes = [POINTER(SampleArgs), c_void_p, c_size_t, c_void_p]
+    L.cce_b200_sample_workspace_bytes.restype = c_size_t
+    L.cce_b200_sample_workspace_bytes.argtypes = [POINTER(SampleArgs)]
     L.cce_b200_gemm.restype = c_int32
     L.cce_b200_gemm.argtypes = [
         c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,

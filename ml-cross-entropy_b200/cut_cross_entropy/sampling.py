@@ -101,7 +101,9 @@ def sample_tokens(
             _native._ptr(top_k_t), _native._ptr(top_p_t), _native._ptr(min_p_t), temperature_n, top_p_n, min_p_n, top_k_n,
             tokens.data_ptr(), _native._ptr(logprobs),
         )  # fmt: skip
-        rc = _native.lib().cce_b200_sample(args, _native.stream_ptr(dev))
+        L = _native.lib()
+        ws = _native.workspace(L.cce_b200_sample_workspace_bytes(args), dev)
+        rc = L.cce_b200_sample(args, ws.data_ptr(), ws.numel(), _native.stream_ptr(dev))
     if rc != 0:
         _native.check(rc, "cce_b200_sample")
     return (tokens, logprobs) if return_logprobs else tokens

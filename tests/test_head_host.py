@@ -82,11 +82,13 @@ def test_c_entry_points_check_their_arguments():
     L = _native.lib()
     bad = -1  # CCE_ERR_ARG
     assert L.cce_b200_logits(None, None, 0, None) == bad
-    assert L.cce_b200_sample(None, None) == bad
+    assert L.cce_b200_sample(None, None, 0, None) == bad
+    assert L.cce_b200_sample_workspace_bytes(None) == 0
     assert L.cce_b200_logits_workspace_bytes(None) == 0
 
-    buf = ctypes.create_string_buffer(64)
-    ptr = ctypes.addressof(buf)
+    buf = ctypes.create_string_buffer(1024)
+    ptr = ctypes.addressof(buf) // 16 * 16 + 16
+    aligned = (ctypes.addressof(buf) + 255) // 256 * 256  # as a workspace has to be
 
     def logits_args(**kw):
         a = _native.LogitsArgs()
@@ -123,9 +125,13 @@ def test_c_entry_points_check_their_arguments():
         return a
 
     for kw in (dict(logits=None), dict(u=None), dict(tokens=None), dict(V=0), dict(B=-1), dict(ld=9), dict(dtype=3)):
-        assert L.cce_b200_sample(sample_args(**kw), None) == bad, kw
-    assert L.cce_b200_sample(sample_args(logits=ptr + 2), None) == -2  # CCE_ERR_ALIGN
-    assert L.cce_b200_sample(sample_args(B=0, logits=None), None) == 0
+        assert L.cce_b200_sample(sample_args(**kw), aligned, 1 << 40, None) == bad, kw
+    assert L.cce_b200_sample(sample_args(logits=ptr + 2), aligned, 1 << 40, None) == -2  # CCE_ERR_ALIGN
+    assert L.cce_b200_sample(sample_args(), None, 0, None) == bad
+    assert L.cce_b200_sample(sample_args(), aligned, 0, None) == -3
+    assert L.cce_b200_sample(sample_args(), aligned + 8, 1 << 40, None) == -2
+    assert L.cce_b200_sample(sample_args(V=2**20 + 1, ld=2**21), aligned, 1 << 40, None) == -7  # CCE_ERR_TOO_LARGE
+    assert L.cce_b200_sample(sample_args(B=0, logits=None), None, 0, None) == 0
 
 
 def test_struct_sizes_match_the_header(tmp_path):
