@@ -215,7 +215,8 @@ int launch_sample(const SampleParams& sp, const SamplePlan& pl, long long B, cha
         only = b.state;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(B * pl.cluster));
+    // behind the streaming kernels few rows are left, if any
+    cfg.gridDim = dim3((unsigned)((only ? std::min<long long>(B, 16) : B) * pl.cluster));
     cfg.blockDim = dim3(SMP_THREADS);
     cfg.dynamicSmemBytes = pl.smem;
     cfg.stream = st;
@@ -227,7 +228,7 @@ int launch_sample(const SampleParams& sp, const SamplePlan& pl, long long B, cha
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = only ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, sample_kernel<T>, sp, (const RowState*)only);
+    cudaLaunchKernelEx(&cfg, sample_kernel<T>, sp, (const RowState*)only, B);
     CCE_LAUNCH_CHECK();
     return CCE_OK;
 }

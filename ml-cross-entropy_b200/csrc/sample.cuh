@@ -77,33 +77,32 @@ __device__ __forceinline__ float just_below(float x) {
 }
 
 // 2^frac * exp((l - m) / T) rounded to an integer.  Table-driven (P. T. P. Tang, ACM TOMS 15(2), 1989):
-// (l - m) * 64 log2(e) / T = 64 n + j + r with |r| <= 1/2, so the weight is 2^n * 2^(j/64) * e^z with
-// z = r ln2 / 64, |z| < 0.0055, and four terms of the Taylor series leave a relative error of
-// z^5/120 < 4e-14, below the rounding to 2^-43.  The product is added to 2^52, whose low bits then
-// hold the rounded integer.  Nine fp64 operations: they bound the passes that need every weight.
-constexpr int SMP_TABLE = 64;
+// (l - m) * 16 log2(e) / T = 16 n + j + r with |r| <= 1/2, so the weight is 2^n * 2^(j/16) * e^z with
+// z = r ln2 / 16, |z| < 0.022, and five terms of the Taylor series leave a relative error of
+// z^6/720 < 1.5e-13, about the rounding to 2^-43.  The product is added to 2^52, whose low bits then
+// hold the rounded integer.  16 entries of 8 bytes are what the 32 banks serve at once, whichever the lanes ask for
+// (64 entries, with one term less, were slower).  Ten fp64 operations of the twenty instructions: they bound the
+// passes that need every weight.
+constexpr int SMP_TABLE = 16;
 struct WeightFn {
-    double m, scale;      // maximum, 64 * log2(e) / T
-    const double* table;  // shared memory: 2^(j/64)
-    int frac;
-    float peak;           // m as it is stored
+    double m, scale;      // maximum (the largest finite number for an infinite one), 16 * log2(e) / T
+    const double* table;  // shared memory: 2^(frac + j/16)
     __device__ __forceinline__ u64 operator()(float l) const {
-        constexpr double c = 0.010830424696249145;    // ln2 / 64
+        constexpr double c = 0.043321698784996581;    // ln2 / 16
         constexpr double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
-        const double d = double(l) - m;
+        const double d = double(fminf(l, -SMP_LOWEST)) - m;
         const double t = fma(d, scale, magic);
         const int i = __double2loint(t);
         const double r = fma(d, scale, magic - t);
-        double e = fma(r, c * c * c * c / 24.0, c * c * c / 6.0);
+        double e = fma(r, c * c * c * c * c / 120.0, c * c * c * c / 24.0);
+        e = fma(e, r, c * c * c / 6.0);
         e = fma(e, r, c * c / 2.0);
         e = fma(e, r, c);
         e = fma(e, r, 1.0);
         const double tab = table[i & (SMP_TABLE - 1)];
-        const double scaled =
-            __hiloint2double(__double2hiint(tab) + ((i >> 6) + frac) * (1 << 20), __double2loint(tab));
+        const double scaled = __hiloint2double(__double2hiint(tab) + (i & ~(SMP_TABLE - 1)) * (1 << 16), __double2loint(tab));
         const double w = fma(e, scaled, 4503599627370496.0);  // 2^52
-        const u64 q = (u64)__double_as_longlong(w) & 0xfffffffffffffull;
-        return l == peak ? 1ull << frac : q;  // exact, also where the maximum is infinite
+        return (u64)__double_as_longlong(w) & 0xfffffffffffffull;
     }
 };
 
@@ -222,7 +221,7 @@ __device__ __forceinline__ int sort_size(int n) {
 enum RowMode { ROW_DONE, ROW_GREEDY, ROW_SUM, ROW_LIST, ROW_WINDOW, ROW_BY_CLUSTER };
 struct RowState {
     int mode;
-    int lo, hi;        // window of bins; ROW_LIST: bins 0..hi
+    float above, last;  // ROW_WINDOW: the logits > above lie above the window, those >= last in it; ROW_LIST: those >= last
     unsigned first;    // ROW_GREEDY: the lowest index of the largest logits
     unsigned n_list;
     u64 mass, target;  // top-p alone: all weights, and the running sum to reach
@@ -253,18 +252,16 @@ struct RowBase {
     }
     __device__ __forceinline__ bool greedy_row() const { return !(temp > 0.0) || k == 1; }
     __device__ __forceinline__ void make_table() {
-        if (tid < SMP_TABLE) sc.table[tid] = exp2(double(tid) / SMP_TABLE);
+        if (tid < SMP_TABLE) sc.table[tid] = exp2(double(tid) / SMP_TABLE + double(p.frac_bits));
     }
     // from the row's maximum (above -inf): the weights and the thresholds
     __device__ __forceinline__ void prepare(float m) {
         mx = m + 0.0f;
         const double min_p = p.min_p ? double(p.min_p[row]) : p.min_p_all;
         const double k2 = 1.4426950408889634074 / temp;  // exponents of 2 per unit of logit
-        weight.m = double(mx);
-        weight.peak = mx;
+        weight.m = double(fminf(mx, -SMP_LOWEST));
         weight.scale = SMP_TABLE * k2;
         weight.table = sc.table;
-        weight.frac = p.frac_bits;
         l_floor = l_min = lowest_with(SMP_FLOOR_LOG2, k2);
         if (min_p > 0.0) l_min = fmaxf(l_floor, lowest_with(fmax(SMP_FLOOR_LOG2, log2(fmin(min_p, 1.0))), k2));
         bin_scale = fminf(float(SMP_BINS) / (0.5f * mx - 0.5f * l_floor), 1e30f);
@@ -289,6 +286,26 @@ struct RowBase {
     // may overflow).  The bin falls, or stays, as the logit grows.
     __device__ __forceinline__ int bin0(float l) const {
         return min(SMP_BINS - 1, int((0.5f * mx - 0.5f * l) * bin_scale));
+    }
+    // The first key of [lo, hi] that fulfils a predicate which holds from some key on (hi if none before it does),
+    // by all threads together
+    template <typename F>
+    __device__ __forceinline__ uint32_t first_key(uint32_t lo, uint32_t hi, F pred) {
+        while (lo < hi) {
+            const uint32_t step = (hi - lo) / SMP_THREADS + 1;
+            const u64 at = u64(lo) + u64(tid) * step;
+            const int below = __syncthreads_count(at < hi && !pred(uint32_t(at)));
+            if (below == 0) return lo;
+            const u64 next = u64(lo) + u64(below) * step;
+            lo = lo + uint32_t(below - 1) * step + 1;
+            hi = next < hi ? uint32_t(next) : hi;
+        }
+        return lo;
+    }
+
+    // The smallest logit of bins 0..bin, by all threads together
+    __device__ __forceinline__ float lowest_of_bins(int bin) {
+        return order_value(first_key(order_key(l_floor), order_key(mx), [&](uint32_t q) { return bin0(order_value(q)) <= bin; }));
     }
     // the running sum that top-p has to reach, of the mass it is measured by
     __device__ __forceinline__ u64 p_target(u64 mass) const {
@@ -418,8 +435,8 @@ struct Sampler : RowBase {
     long long start;
     int phase, n_blk;
 
-    __device__ __forceinline__ Sampler(const SampleParams& p_, SmpShared& sm_, uint8_t* dyn_, int cluster)
-        : RowBase(p_, sm_, blockIdx.x / cluster), sm(sm_), dyn(dyn_), lay(cluster, p_.slice, int(sizeof(T))),
+    __device__ __forceinline__ Sampler(const SampleParams& p_, SmpShared& sm_, uint8_t* dyn_, long long row_, int cluster)
+        : RowBase(p_, sm_, row_), sm(sm_), dyn(dyn_), lay(cluster, p_.slice, int(sizeof(T))),
           cl(cooperative_groups::this_cluster()) {
         rank = int(cl.block_rank());
         size = cluster;
@@ -661,22 +678,6 @@ struct Sampler : RowBase {
         merge_hist(false);
         return sum;
     }
-    // The first key of [lo, hi] that fulfils a predicate which holds from some key on (hi if none before it does),
-    // by all threads together
-    template <typename F>
-    __device__ __forceinline__ uint32_t first_key(uint32_t lo, uint32_t hi, F pred) {
-        while (lo < hi) {
-            const uint32_t step = (hi - lo) / SMP_THREADS + 1;
-            const u64 at = u64(lo) + u64(tid) * step;
-            const int below = __syncthreads_count(at < hi && !pred(uint32_t(at)));
-            if (below == 0) return lo;
-            const u64 next = u64(lo) + u64(below) * step;
-            lo = lo + uint32_t(below - 1) * step + 1;
-            hi = next < hi ? uint32_t(next) : hi;
-        }
-        return lo;
-    }
-
     // From a level-0 border down to one value: that value, and the count and mass above it.
     struct Level {
         float value;
@@ -780,8 +781,15 @@ struct Sampler : RowBase {
         __syncthreads();
         exchange(sm.r[0], sm.r[1], sum);
         mass = 0;
-        for (int r = 0; r < size; ++r) mass += got(2, r);
+        u64 est_all = 0;
+        for (int r = 0; r < size; ++r) {
+            mass += got(2, r);
+            est_all += got(0, r);
+        }
         target = p_target(mass);
+        // Measured from the tail, whose many logits' estimates are good, not from the few largest: their error is the
+        // difference of the sums.
+        const u64 goal = est_all > mass - target ? est_all - (mass - target) : 1;
         int owner = 0;
         u64 am = 0, ac = 0, bm = 0, bc = 0;  // estimate and count above share r; those of the owner
         for (int r = 0, found = 0; r < size; ++r) {
@@ -789,7 +797,7 @@ struct Sampler : RowBase {
                 owner = r;
                 bm = am;
                 bc = ac;
-                found = am + got(0, r) >= target;
+                found = am + got(0, r) >= goal;
             }
             am += got(0, r);
             ac += got(1, r);
@@ -804,15 +812,15 @@ struct Sampler : RowBase {
         if (rank == owner) {
             // the thread whose bins cross the target; the last one with a count if the estimate falls short
             const u64 begin = bm + em - em_own;
-            const bool crosses = begin < target && target <= bm + em;
-            if (crosses || (bm + sm.r[0] < target && ec == sm.r[1] && tc > 0)) {
+            const bool crosses = begin < goal && goal <= bm + em;
+            if (crosses || (bm + sm.r[0] < goal && ec == sm.r[1] && tc > 0)) {
                 double run = double(begin);
                 u64 c = bc + ec - tc;
                 int at = b0;
                 for (int i = 0; i < per && b0 + i < lay.share; ++i) {
                     at = b0 + i;
                     run += est[at];
-                    if (run >= double(target) || (!crosses && c + own_cnt()[at] == bc + ec)) break;
+                    if (run >= double(goal) || (!crosses && c + own_cnt()[at] == bc + ec)) break;
                     if (i + 1 < per && b0 + i + 1 < lay.share) c += own_cnt()[at];
                 }
                 sm.r[3] = u64(at) << 40 | c;
@@ -1104,19 +1112,38 @@ struct Sampler : RowBase {
     }
 };
 
-// only: null, or the rows' states, of which those in ROW_BY_CLUSTER are sampled
+// The rows of a call, one per cluster; or (only: their states) those in ROW_BY_CLUSTER, dealt to the clusters of a small
+// grid.
 template <typename T>
 __global__ void __launch_bounds__(SMP_THREADS, 2)
-sample_kernel(const SampleParams p, const RowState* only) {
+sample_kernel(const SampleParams p, const RowState* only, long long B) {
     extern __shared__ __align__(16) uint8_t dyn[];
     __shared__ SmpShared sm;
-    const int cluster = int(cooperative_groups::this_cluster().num_blocks());
-    if (only) {
-        pdl_wait();
-        if (only[blockIdx.x / cluster].mode != ROW_BY_CLUSTER) return;
+    __shared__ uint32_t todo[SMP_WARPS];
+    const cooperative_groups::cluster_group cl = cooperative_groups::this_cluster();
+    const int cluster = int(cl.num_blocks());
+    if (!only) {
+        Sampler<T> s(p, sm, dyn, blockIdx.x / cluster, cluster);
+        s.run();
+        return;
     }
-    Sampler<T> s(p, sm, dyn, cluster);
-    s.run();
+    pdl_wait();
+    const long long n_cluster = gridDim.x / cluster, first = blockIdx.x / cluster;
+    for (long long r0 = first; r0 < B; r0 += n_cluster * SMP_THREADS) {
+        // bit t of the list: row r0 + t * n_cluster; the same in all CTAs of the cluster
+        const long long mine = r0 + threadIdx.x * n_cluster;
+        const unsigned bits = __ballot_sync(0xffffffffu, mine < B && only[mine].mode == ROW_BY_CLUSTER);
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) todo[threadIdx.x >> 5] = bits;
+        __syncthreads();
+        for (int t = 0; t < SMP_THREADS; ++t) {
+            if (!todo[t >> 5]) t |= 31;
+            if (!(todo[t >> 5] >> (t & 31) & 1)) continue;
+            Sampler<T> s(p, sm, dyn, r0 + t * n_cluster, cluster);
+            s.run();
+            if (cluster > 1) cl.sync(); else __syncthreads();  // before the next row takes the shared memory
+        }
+    }
 }
 
 }  // namespace cce

@@ -101,7 +101,7 @@ row_max_kernel(const SampleParams p, const StreamBuffers b) {
 #pragma unroll
         for (int w = 0; w < SMP_WARPS; ++w) m = fmaxf(m, wf[w]);
         b.chunk_max[row * b.n_chunk + chunk] = m;
-        if (chunk == 0) b.state[row] = RowState{ROW_SUM, 0, 0, 0xffffffffu, 0, 0, 0};
+        if (chunk == 0) b.state[row] = RowState{ROW_SUM, 0.0f, 0.0f, 0xffffffffu, 0, 0, 0};
     }
 }
 
@@ -220,10 +220,13 @@ row_plan_kernel(const SampleParams p, const StreamBuffers b) {
         const u64 n_all = sc.r[1];
         st.mass = mass;
         st.target = r.k ? min(u64(r.k), n_all) : r.p_target(mass);
+        // top-p alone: the estimates are measured from the tail, whose many logits make them good, not from the few largest
+        const u64 rest = mass - st.target;
+        const u64 goal = r.k ? st.target : sc.r[0] > rest ? sc.r[0] - rest : 1;
         // the thread whose bins hold the border; for an estimate that falls short, the last one with a count
         const u64 c0 = ec - tc, e0 = em - em_own;
-        const bool mine = r.k ? c0 < st.target && st.target <= ec
-                              : (e0 < st.target && st.target <= em) || (sc.r[0] < st.target && ec == n_all && tc > 0);
+        const bool mine = r.k ? c0 < goal && goal <= ec
+                              : (e0 < goal && goal <= em) || (sc.r[0] < goal && ec == n_all && tc > 0);
         if (mine) {
             u64 c = c0;
             double run = double(e0);
@@ -231,7 +234,7 @@ row_plan_kernel(const SampleParams p, const StreamBuffers b) {
             u64 above = 0;
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
-                if (cnt[i] && (bin < 0 || !(r.k ? c >= st.target : run >= double(st.target)))) {
+                if (cnt[i] && (bin < 0 || !(r.k ? c >= goal : run >= double(goal)))) {
                     bin = r.tid * PER + i;  // the last bin with a count before the target is reached
                     above = c;
                 }
@@ -247,7 +250,7 @@ row_plan_kernel(const SampleParams p, const StreamBuffers b) {
             st.mode = ROW_BY_CLUSTER;
         } else if (r.k) {
             st.mode = at_above + n_at <= SMP_LIST ? ROW_LIST : ROW_BY_CLUSTER;
-            st.hi = at_bin;
+            hi = at_bin;
         } else {
             const u64 room = (SMP_LIST - n_at) / 2;
             u64 c = c0;
@@ -264,13 +267,14 @@ row_plan_kernel(const SampleParams p, const StreamBuffers b) {
                 c += cnt[i];
             }
             __syncthreads();
-            st.lo = lo;
-            st.hi = hi;
-            st.mode = ROW_WINDOW;
-            if (all < SMP_BINS) {
-                st.mode = ROW_LIST;
-                st.hi = all;
-            }
+            st.mode = all < SMP_BINS ? ROW_LIST : ROW_WINDOW;
+            if (all < SMP_BINS) hi = all;  // by every thread alike
+        }
+        __syncthreads();
+        if (st.mode == ROW_LIST || st.mode == ROW_WINDOW) {
+            st.last = r.lowest_of_bins(hi);
+            // (a window that begins with bin 0 has nothing above it)
+            st.above = st.mode == ROW_LIST || lo == 0 ? INFINITY : just_below(r.lowest_of_bins(lo - 1));
         }
     }
     if (r.tid == 0) b.state[row] = st;
@@ -318,20 +322,18 @@ row_pass_kernel(const SampleParams p, const StreamBuffers b) {
             };
             if (st.mode == ROW_LIST) {
                 rs.each(block, r.lane, [&](float l, long long pos) {
-                    if (l >= r.l_floor && r.bin0(l) <= st.hi) collect(l, pos);
+                    if (l >= st.last) collect(l, pos);
                 });
             } else {
-                const bool window = st.mode == ROW_WINDOW;
+                const float edge = st.mode == ROW_WINDOW ? st.above : just_below(r.l_floor);  // ROW_SUM: all is above
+                const float last = st.mode == ROW_WINDOW ? st.last : INFINITY;
                 rs.each(block, r.lane, [&](float l, long long pos) {
-                    if (l >= r.l_floor) {
-                        const int bin = window ? r.bin0(l) : -1;
-                        if (bin < st.lo) {
-                            const u64 w = r.weight(l);
-                            above += w;
-                            if (l >= r.l_min) bm += w;
-                        } else if (bin <= st.hi) {
-                            collect(l, pos);
-                        }
+                    if (l > edge) {
+                        const u64 w = r.weight(l);
+                        above += w;
+                        if (l >= r.l_min) bm += w;
+                    } else if (l >= last) {
+                        collect(l, pos);
                     }
                 });
                 bm = warp_sum_u64(bm);
@@ -350,7 +352,7 @@ row_pass_kernel(const SampleParams p, const StreamBuffers b) {
 
 // One CTA per row.  Dynamic shared memory: three lists of SMP_LIST keys, then the blocks' masses.
 template <typename T>
-__global__ void __launch_bounds__(SMP_THREADS)
+__global__ void __launch_bounds__(SMP_THREADS, 2)
 row_draw_kernel(const SampleParams p, const StreamBuffers b) {
     extern __shared__ __align__(16) uint8_t dyn[];
     __shared__ CtaScratch sc;
