@@ -81,12 +81,13 @@ __device__ __forceinline__ float just_below(float x) {
 // z = r ln2 / 16, |z| < 0.022, and five terms of the Taylor series leave a relative error of
 // z^6/720 < 1.5e-13, about the rounding to 2^-43.  The product is added to 2^52, whose low bits then
 // hold the rounded integer.  16 entries of 8 bytes are what the 32 banks serve at once, whichever the lanes ask for
-// (64 entries, with one term less, were slower).  Ten fp64 operations of the twenty instructions: they bound the
-// passes that need every weight.
+// (64 entries, with one term less, were slower).  A pass over every weight is bound by issuing its instructions, ten of
+// them fp64: sum_weights below has no branch per logit, which took them from 51 to about 25.
 constexpr int SMP_TABLE = 16;
 struct WeightFn {
-    double m, scale;      // maximum (the largest finite number for an infinite one), 16 * log2(e) / T
-    const double* table;  // shared memory: 2^(frac + j/16)
+    double m, scale;  // maximum (the largest finite number for an infinite one), 16 * log2(e) / T
+    uint32_t table;   // shared memory: 2^(frac + j/16)
+    // for m - l beyond the floor (or NaN, -inf) the result means nothing
     __device__ __forceinline__ u64 operator()(float l) const {
         constexpr double c = 0.043321698784996581;    // ln2 / 16
         constexpr double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
@@ -99,10 +100,27 @@ struct WeightFn {
         e = fma(e, r, c * c / 2.0);
         e = fma(e, r, c);
         e = fma(e, r, 1.0);
-        const double tab = table[i & (SMP_TABLE - 1)];
-        const double scaled = __hiloint2double(__double2hiint(tab) + (i & ~(SMP_TABLE - 1)) * (1 << 16), __double2loint(tab));
+        double tab;
+        asm("ld.shared.f64 %0, [%1];" : "=d"(tab) : "r"(table + ((i << 3) & ((SMP_TABLE - 1) << 3))));
+        const double scaled = __hiloint2double(__double2hiint(tab) + ((i << 16) & 0xfff00000), __double2loint(tab));
         const double w = fma(e, scaled, 4503599627370496.0);  // 2^52
         return (u64)__double_as_longlong(w) & 0xfffffffffffffull;
+    }
+    // sum of the weights of those of n logits that are at least `from`; a warp together
+    template <int N>
+    __device__ __forceinline__ u64 sum_weights(const float (&l)[N], float from) const {
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) any |= l[i] >= from;
+        u64 s = 0;
+        if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const u64 w = (*this)(l[i]);
+                s += l[i] >= from ? w : 0;
+            }
+        }
+        return s;
     }
 };
 
@@ -221,7 +239,8 @@ __device__ __forceinline__ int sort_size(int n) {
 enum RowMode { ROW_DONE, ROW_GREEDY, ROW_SUM, ROW_LIST, ROW_WINDOW, ROW_BY_CLUSTER };
 struct RowState {
     int mode;
-    float above, last;  // ROW_WINDOW: the logits > above lie above the window, those >= last in it; ROW_LIST: those >= last
+    float edge, last;   // ROW_WINDOW: the logits from edge on lie above the window, those from last on in it; ROW_LIST: those
+                        // from last on
     unsigned first;    // ROW_GREEDY: the lowest index of the largest logits
     unsigned n_list;
     u64 mass, target;  // top-p alone: all weights, and the running sum to reach
@@ -261,7 +280,7 @@ struct RowBase {
         const double k2 = 1.4426950408889634074 / temp;  // exponents of 2 per unit of logit
         weight.m = double(fminf(mx, -SMP_LOWEST));
         weight.scale = SMP_TABLE * k2;
-        weight.table = sc.table;
+        weight.table = smem_u32(sc.table);
         l_floor = l_min = lowest_with(SMP_FLOOR_LOG2, k2);
         if (min_p > 0.0) l_min = fmaxf(l_floor, lowest_with(fmax(SMP_FLOOR_LOG2, log2(fmin(min_p, 1.0))), k2));
         bin_scale = fminf(float(SMP_BINS) / (0.5f * mx - 0.5f * l_floor), 1e30f);
@@ -459,6 +478,20 @@ struct Sampler : RowBase {
             const T* x = reinterpret_cast<const T*>(&w);
 #pragma unroll
             for (int i = 0; i < VE; ++i) f(float(x[i]), q * VE + i);
+        }
+    }
+    // f(logits of a 16-byte piece, first position), likewise
+    template <typename F>
+    __device__ __forceinline__ void each_piece(int b, F f) const {
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            const int q = (b * CHUNKS + c) * 32 + lane;
+            const uint4 w = data[q];
+            const T* x = reinterpret_cast<const T*>(&w);
+            float l[VE];
+#pragma unroll
+            for (int i = 0; i < VE; ++i) l[i] = float(x[i]);
+            f(l, q * VE);
         }
     }
     // this warp's blocks of the slice
@@ -669,12 +702,13 @@ struct Sampler : RowBase {
     __device__ __forceinline__ u64 level0_counts_and_sum() {
         clear_hist(false);
         u64 sum = 0;
-        each_of_slice([&](float l, int) {
-            if (l >= l_floor) {
-                atomicAdd(&hist_cnt()[bin0(l)], 1u);
-                sum += weight(l);
-            }
-        });
+        for (int b = warp; b < n_blk; b += SMP_WARPS)
+            each_piece(b, [&](const float (&l)[VE], int) {
+#pragma unroll
+                for (int i = 0; i < VE; ++i)
+                    if (l[i] >= l_floor) atomicAdd(&hist_cnt()[bin0(l[i])], 1u);
+                sum += weight.sum_weights(l, l_floor);
+            });
         merge_hist(false);
         return sum;
     }
@@ -859,20 +893,19 @@ struct Sampler : RowBase {
     // The exact border of top-p in the window.  Leaves the kept weights by blocks in blk_mass; the key of the last
     // kept logit, or 0 when the window missed the border.
     __device__ __forceinline__ u64 cut_in_window(const Window& win, u64 target) {
+        // the logits from `edge` on lie above the window, those from `last` on in it
+        const float edge = win.lo == 0 ? INFINITY : lowest_of_bins(win.lo - 1), last = lowest_of_bins(win.hi);
+        const float min_edge = fmaxf(edge, l_min);
         u64 above = 0, unused = 0;
         for (int b = warp; b < n_blk; b += SMP_WARPS) {
             u64 bm = 0;
-            each(b, [&](float l, int pos) {
-                if (l >= l_floor) {
-                    const int bin = bin0(l);
-                    if (bin < win.lo) {
-                        const u64 w = weight(l);
-                        above += w;
-                        if (l >= l_min) bm += w;
-                    } else if (bin <= win.hi) {
-                        collect(l, pos);
-                    }
-                }
+            each_piece(b, [&](const float (&l)[VE], int pos) {
+                const u64 w = weight.sum_weights(l, edge);
+                above += w;
+                bm += min_edge > edge ? weight.sum_weights(l, min_edge) : w;
+#pragma unroll
+                for (int i = 0; i < VE; ++i)
+                    if (l[i] < edge && l[i] >= last) collect(l[i], pos + i);
             });
             bm = warp_sum_u64(bm);
             if (lane == 0) blk_mass()[b] = bm;
@@ -998,9 +1031,13 @@ struct Sampler : RowBase {
         __syncthreads();
         for (int b = warp; b < n_blk; b += SMP_WARPS) {
             u64 bm = 0;
-            each(b, [&](float l, int pos) {
-                if (is_kept(l, token_at(pos), cut, cut_l)) bm += weight(l);
-            });
+            if (cut == ~0ull) {
+                each_piece(b, [&](const float (&l)[VE], int) { bm += weight.sum_weights(l, l_min); });
+            } else {
+                each(b, [&](float l, int pos) {
+                    if (is_kept(l, token_at(pos), cut, cut_l)) bm += weight(l);
+                });
+            }
             bm = warp_sum_u64(bm);
             if (lane == 0) blk_mass()[b] = bm;
         }

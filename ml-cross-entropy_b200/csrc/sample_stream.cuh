@@ -62,18 +62,28 @@ struct RowStream {
         return pos >= phase && pos < phase + V ? float(base[pos]) : -INFINITY;
     }
     __device__ __forceinline__ bool holds(long long block) const { return block * SMP_BLK < phase + V; }
-    // f(l, position) for every position of a block, a warp together
+    // f(logits of a 16-byte piece, first position) for the pieces of a block, a warp together
     template <typename F>
-    __device__ __forceinline__ void each(long long block, int lane, F f) const {
+    __device__ __forceinline__ void each_piece(long long block, int lane, F f) const {
         uint4 w[CHUNKS];
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) w[c] = piece((block * CHUNKS + c) * 32 + lane);
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             const T* x = reinterpret_cast<const T*>(&w[c]);
+            float l[VE];
 #pragma unroll
-            for (int i = 0; i < VE; ++i) f(float(x[i]), ((block * CHUNKS + c) * 32 + lane) * VE + i);
+            for (int i = 0; i < VE; ++i) l[i] = float(x[i]);
+            f(l, ((block * CHUNKS + c) * 32 + lane) * VE);
         }
+    }
+    // f(l, position) for every position of a block, likewise
+    template <typename F>
+    __device__ __forceinline__ void each(long long block, int lane, F f) const {
+        each_piece(block, lane, [&](const float (&l)[VE], long long pos) {
+#pragma unroll
+            for (int i = 0; i < VE; ++i) f(l[i], pos + i);
+        });
     }
 };
 
@@ -144,14 +154,14 @@ row_stats_kernel(const SampleParams p, const StreamBuffers b) {
             continue;
         }
         u64 bm = 0;
-        rs.each(block, r.lane, [&](float l, long long) {
+        rs.each_piece(block, r.lane, [&](const float (&l)[RowStream<T>::VE], long long) {
             if (FILTERS) {
-                if (l >= r.l_floor) {
-                    atomicAdd(&hist[r.bin0(l)], 1u);
-                    if (want_sum) sum += r.weight(l);
-                }
-            } else if (l >= r.l_min) {
-                bm += r.weight(l);
+#pragma unroll
+                for (int j = 0; j < RowStream<T>::VE; ++j)
+                    if (l[j] >= r.l_floor) atomicAdd(&hist[r.bin0(l[j])], 1u);
+                if (want_sum) sum += r.weight.sum_weights(l, r.l_floor);
+            } else {
+                bm += r.weight.sum_weights(l, r.l_min);
             }
         });
         if (!FILTERS) {
@@ -274,7 +284,7 @@ row_plan_kernel(const SampleParams p, const StreamBuffers b) {
         if (st.mode == ROW_LIST || st.mode == ROW_WINDOW) {
             st.last = r.lowest_of_bins(hi);
             // (a window that begins with bin 0 has nothing above it)
-            st.above = st.mode == ROW_LIST || lo == 0 ? INFINITY : just_below(r.lowest_of_bins(lo - 1));
+            st.edge = st.mode == ROW_LIST || lo == 0 ? INFINITY : r.lowest_of_bins(lo - 1);
         }
     }
     if (r.tid == 0) b.state[row] = st;
@@ -325,16 +335,16 @@ row_pass_kernel(const SampleParams p, const StreamBuffers b) {
                     if (l >= st.last) collect(l, pos);
                 });
             } else {
-                const float edge = st.mode == ROW_WINDOW ? st.above : just_below(r.l_floor);  // ROW_SUM: all is above
+                const float edge = st.mode == ROW_WINDOW ? st.edge : r.l_floor;  // ROW_SUM: all is above
                 const float last = st.mode == ROW_WINDOW ? st.last : INFINITY;
-                rs.each(block, r.lane, [&](float l, long long pos) {
-                    if (l > edge) {
-                        const u64 w = r.weight(l);
-                        above += w;
-                        if (l >= r.l_min) bm += w;
-                    } else if (l >= last) {
-                        collect(l, pos);
-                    }
+                const float min_edge = fmaxf(edge, r.l_min);
+                rs.each_piece(block, r.lane, [&](const float (&l)[RowStream<T>::VE], long long pos) {
+                    const u64 w = r.weight.sum_weights(l, edge);
+                    above += w;
+                    bm += min_edge > edge ? r.weight.sum_weights(l, min_edge) : w;
+#pragma unroll
+                    for (int j = 0; j < RowStream<T>::VE; ++j)
+                        if (l[j] < edge && l[j] >= last) collect(l[j], pos + j);
                 });
                 bm = warp_sum_u64(bm);
             }
