@@ -412,7 +412,8 @@ int cce_b200_sample(const cce_b200_sample_args* a, void* workspace, size_t works
     sp.slice = pl.slice;
     int log2v = 0;
     while ((1LL << log2v) < a->V) ++log2v;
-    sp.frac_bits = std::min(50, 62 - log2v);  // V weights of at most 1 << frac_bits stay below 2^63
+    // V weights of at most 1 << frac_bits stay below 2^63
+    sp.frac_bits = std::min(SMP_MAX_FRAC, 62 - log2v);
     char* ws = reinterpret_cast<char*>(workspace);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (a->dtype == CCE_DT_F32) return launch_sample<float>(sp, pl, a->B, ws, st);

@@ -6,7 +6,7 @@
 //   token = the first kept v, in order of v, whose running sum of weights exceeds u * (sum kept)
 //
 // With 2^18 tokens of a flat distribution the running sums are 4e-6 apart, so fp32 sums would move
-// the draw.  The weights are evaluated in fp64 and rounded to fixed point (a unit of 2^-50..2^-43 of the
+// the draw.  The weights are evaluated in fp64 and rounded to fixed point (a unit of 2^-46..2^-42 of the
 // largest, so that V of them fit 63 bits): integer sums are exact in any order, hence the token
 // depends neither on the split of the row nor on the order of the atomics below.
 //
@@ -80,15 +80,22 @@ __device__ __forceinline__ float just_below(float x) {
 // (l - m) * 16 log2(e) / T = 16 n + j + r with |r| <= 1/2, so the weight is 2^n * 2^(j/16) * e^z with
 // z = r ln2 / 16, |z| < 0.022, and five terms of the Taylor series leave a relative error of
 // z^6/720 < 1.5e-13, about the rounding to 2^-43.  The product is added to 2^52, whose low bits then
-// hold the rounded integer.  16 entries of 8 bytes are what the 32 banks serve at once, whichever the lanes ask for
-// (64 entries, with one term less, were slower).  A pass over every weight is bound by issuing its instructions, ten of
-// them fp64: sum_weights below has no branch per logit, which took them from 51 to about 25.
+// hold the rounded integer.  16 entries of 8 bytes are what the 32 banks serve at once, whichever the lanes ask for.
+// The exponent n reaches the table's value by one addition: i << 16 is n << 20 plus j << 16, and the entry of j has
+// that taken off.  A pass over every weight is bound by issuing its instructions (51 per logit with a branch for each and
+// 64-bit integer sums, about 22 as below): the sums are kept in fp64, exact while 128 weights of at most 2^46 meet.
 constexpr int SMP_TABLE = 16;
+constexpr int SMP_MAX_FRAC = 46;
 struct WeightFn {
     double m, scale;  // maximum (the largest finite number for an infinite one), 16 * log2(e) / T
-    uint32_t table;   // shared memory: 2^(frac + j/16)
-    // for m - l beyond the floor (or NaN, -inf) the result means nothing
-    __device__ __forceinline__ u64 operator()(float l) const {
+    uint32_t table;   // shared memory, see fill_table
+    // 2^(frac + j/16), less j << 16 in its high word
+    static __device__ __forceinline__ double entry(int j, int frac) {
+        const double x = exp2(double(j) / SMP_TABLE + double(frac));
+        return __hiloint2double(__double2hiint(x) - (j << 16), __double2loint(x));
+    }
+    // the rounded weight + 2^52; for m - l beyond the floor (or NaN, -inf) the result means nothing
+    __device__ __forceinline__ double raised(float l) const {
         constexpr double c = 0.043321698784996581;    // ln2 / 16
         constexpr double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
         const double d = double(fminf(l, -SMP_LOWEST)) - m;
@@ -102,25 +109,25 @@ struct WeightFn {
         e = fma(e, r, 1.0);
         double tab;
         asm("ld.shared.f64 %0, [%1];" : "=d"(tab) : "r"(table + ((i << 3) & ((SMP_TABLE - 1) << 3))));
-        const double scaled = __hiloint2double(__double2hiint(tab) + ((i << 16) & 0xfff00000), __double2loint(tab));
-        const double w = fma(e, scaled, 4503599627370496.0);  // 2^52
-        return (u64)__double_as_longlong(w) & 0xfffffffffffffull;
+        const double scaled = __hiloint2double(__double2hiint(tab) + i * (1 << 16), __double2loint(tab));
+        return fma(e, scaled, 4503599627370496.0);
     }
-    // sum of the weights of those of n logits that are at least `from`; a warp together
+    __device__ __forceinline__ u64 operator()(float l) const {
+        return (u64)__double_as_longlong(raised(l)) & 0xfffffffffffffull;
+    }
+    // adds the weights of those of N logits that are at least `from` to sum; a warp together
     template <int N>
-    __device__ __forceinline__ u64 sum_weights(const float (&l)[N], float from) const {
+    __device__ __forceinline__ void sum_weights(const float (&l)[N], float from, double& sum) const {
         bool any = false;
 #pragma unroll
         for (int i = 0; i < N; ++i) any |= l[i] >= from;
-        u64 s = 0;
         if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const u64 w = (*this)(l[i]);
-                s += l[i] >= from ? w : 0;
+                const double w = raised(l[i]) - 4503599627370496.0;
+                asm("{\n\t.reg .pred p;\n\tsetp.ge.f32 p, %2, %3;\n\t@p add.rn.f64 %0, %0, %1;\n\t}" : "+d"(sum) : "d"(w), "f"(l[i]), "f"(from));
             }
         }
-        return s;
     }
 };
 
@@ -271,7 +278,7 @@ struct RowBase {
     }
     __device__ __forceinline__ bool greedy_row() const { return !(temp > 0.0) || k == 1; }
     __device__ __forceinline__ void make_table() {
-        if (tid < SMP_TABLE) sc.table[tid] = exp2(double(tid) / SMP_TABLE + double(p.frac_bits));
+        if (tid < SMP_TABLE) sc.table[tid] = WeightFn::entry(tid, p.frac_bits);
     }
     // from the row's maximum (above -inf): the weights and the thresholds
     __device__ __forceinline__ void prepare(float m) {
@@ -701,16 +708,16 @@ struct Sampler : RowBase {
     // the counts of level 0, and the sum of this CTA's weights
     __device__ __forceinline__ u64 level0_counts_and_sum() {
         clear_hist(false);
-        u64 sum = 0;
+        double sum = 0.0;
         for (int b = warp; b < n_blk; b += SMP_WARPS)
             each_piece(b, [&](const float (&l)[VE], int) {
 #pragma unroll
                 for (int i = 0; i < VE; ++i)
                     if (l[i] >= l_floor) atomicAdd(&hist_cnt()[bin0(l[i])], 1u);
-                sum += weight.sum_weights(l, l_floor);
+                weight.sum_weights(l, l_floor, sum);
             });
         merge_hist(false);
-        return sum;
+        return u64(sum);
     }
     // From a level-0 border down to one value: that value, and the count and mass above it.
     struct Level {
@@ -896,20 +903,21 @@ struct Sampler : RowBase {
         // the logits from `edge` on lie above the window, those from `last` on in it
         const float edge = win.lo == 0 ? INFINITY : lowest_of_bins(win.lo - 1), last = lowest_of_bins(win.hi);
         const float min_edge = fmaxf(edge, l_min);
-        u64 above = 0, unused = 0;
+        double above_d = 0.0;
         for (int b = warp; b < n_blk; b += SMP_WARPS) {
-            u64 bm = 0;
+            double bm = 0.0, bw = 0.0;
             each_piece(b, [&](const float (&l)[VE], int pos) {
-                const u64 w = weight.sum_weights(l, edge);
-                above += w;
-                bm += min_edge > edge ? weight.sum_weights(l, min_edge) : w;
+                weight.sum_weights(l, edge, bw);
+                if (min_edge > edge) weight.sum_weights(l, min_edge, bm);
 #pragma unroll
                 for (int i = 0; i < VE; ++i)
                     if (l[i] < edge && l[i] >= last) collect(l[i], pos + i);
             });
-            bm = warp_sum_u64(bm);
-            if (lane == 0) blk_mass()[b] = bm;
+            above_d += bw;
+            const u64 kept = warp_sum_u64(u64(min_edge > edge ? bm : bw));
+            if (lane == 0) blk_mass()[b] = kept;
         }
+        u64 above = u64(above_d), unused = 0;
         cta_sum(above, unused);
         send_candidates(win.owner);
         exchange(above);
@@ -1032,7 +1040,9 @@ struct Sampler : RowBase {
         for (int b = warp; b < n_blk; b += SMP_WARPS) {
             u64 bm = 0;
             if (cut == ~0ull) {
-                each_piece(b, [&](const float (&l)[VE], int) { bm += weight.sum_weights(l, l_min); });
+                double sum = 0.0;
+                each_piece(b, [&](const float (&l)[VE], int) { weight.sum_weights(l, l_min, sum); });
+                bm = u64(sum);
             } else {
                 each(b, [&](float l, int pos) {
                     if (is_kept(l, token_at(pos), cut, cut_l)) bm += weight(l);

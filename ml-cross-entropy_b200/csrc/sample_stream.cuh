@@ -145,7 +145,7 @@ row_stats_kernel(const SampleParams p, const StreamBuffers b) {
     if (!(m > -INFINITY) || r.greedy_row()) return;
     r.prepare(m);
     __syncthreads();
-    u64 sum = 0, unused = 0;
+    double sum_d = 0.0;
     const bool want_sum = !r.k;
     for (int i = r.warp; i < STR_BLOCKS; i += SMP_WARPS) {
         const long long block = (long long)chunk * STR_BLOCKS + i;
@@ -153,23 +153,24 @@ row_stats_kernel(const SampleParams p, const StreamBuffers b) {
             if (!FILTERS && r.lane == 0) b.blk_mass[(row * b.n_chunk + chunk) * STR_BLOCKS + i] = 0;
             continue;
         }
-        u64 bm = 0;
+        double bm = 0.0;
         rs.each_piece(block, r.lane, [&](const float (&l)[RowStream<T>::VE], long long) {
             if (FILTERS) {
 #pragma unroll
                 for (int j = 0; j < RowStream<T>::VE; ++j)
                     if (l[j] >= r.l_floor) atomicAdd(&hist[r.bin0(l[j])], 1u);
-                if (want_sum) sum += r.weight.sum_weights(l, r.l_floor);
+                if (want_sum) r.weight.sum_weights(l, r.l_floor, sum_d);
             } else {
-                bm += r.weight.sum_weights(l, r.l_min);
+                r.weight.sum_weights(l, r.l_min, bm);
             }
         });
         if (!FILTERS) {
-            bm = warp_sum_u64(bm);
-            if (r.lane == 0) b.blk_mass[(row * b.n_chunk + chunk) * STR_BLOCKS + i] = bm;
+            const u64 kept = warp_sum_u64(u64(bm));
+            if (r.lane == 0) b.blk_mass[(row * b.n_chunk + chunk) * STR_BLOCKS + i] = kept;
         }
     }
     if (!FILTERS) return;
+    u64 sum = u64(sum_d), unused = 0;
     r.cta_sum(sum, unused);  // a barrier: the counts are complete
     if (r.tid == 0) b.chunk_sum[row * b.n_chunk + chunk] = sum;
     for (int i = r.tid; i < SMP_BINS; i += SMP_THREADS)
@@ -322,10 +323,10 @@ row_pass_kernel(const SampleParams p, const StreamBuffers b) {
     }
     r.prepare(m);
     __syncthreads();
-    u64 above = 0, unused = 0;
+    double above_d = 0.0;
     for (int i = r.warp; i < STR_BLOCKS; i += SMP_WARPS) {
         const long long block = (long long)chunk * STR_BLOCKS + i;
-        u64 bm = 0;
+        u64 kept = 0;
         if (rs.holds(block)) {
             auto collect = [&](float l, long long pos) {
                 local[atomicAdd(&n_local, 1u)] = r.rank_key(l, pos - rs.phase);
@@ -338,19 +339,21 @@ row_pass_kernel(const SampleParams p, const StreamBuffers b) {
                 const float edge = st.mode == ROW_WINDOW ? st.edge : r.l_floor;  // ROW_SUM: all is above
                 const float last = st.mode == ROW_WINDOW ? st.last : INFINITY;
                 const float min_edge = fmaxf(edge, r.l_min);
+                double bm = 0.0, bw = 0.0;
                 rs.each_piece(block, r.lane, [&](const float (&l)[RowStream<T>::VE], long long pos) {
-                    const u64 w = r.weight.sum_weights(l, edge);
-                    above += w;
-                    bm += min_edge > edge ? r.weight.sum_weights(l, min_edge) : w;
+                    r.weight.sum_weights(l, edge, bw);
+                    if (min_edge > edge) r.weight.sum_weights(l, min_edge, bm);
 #pragma unroll
                     for (int j = 0; j < RowStream<T>::VE; ++j)
                         if (l[j] < edge && l[j] >= last) collect(l[j], pos + j);
                 });
-                bm = warp_sum_u64(bm);
+                above_d += bw;
+                kept = warp_sum_u64(u64(min_edge > edge ? bm : bw));
             }
         }
-        if (r.lane == 0) b.blk_mass[(row * b.n_chunk + chunk) * STR_BLOCKS + i] = bm;
+        if (r.lane == 0) b.blk_mass[(row * b.n_chunk + chunk) * STR_BLOCKS + i] = kept;
     }
+    u64 above = u64(above_d), unused = 0;
     r.cta_sum(above, unused);
     if (r.tid == 0) {
         b.chunk_sum[row * b.n_chunk + chunk] = above;
