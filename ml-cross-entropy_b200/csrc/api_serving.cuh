@@ -206,6 +206,8 @@ int launch_sample(const SampleParams& sp, const SamplePlan& pl, long long B, cha
         const dim3 chunks((unsigned)(B * pl.n_chunk)), rows((unsigned)B);
         const int draw_smem = (3 * SMP_LIST + pl.n_chunk * STR_BLOCKS) * (int)sizeof(u64);
         int rc = launch_behind(row_max_kernel<T>, chunks, SMP_THREADS, 0, st, false, sp, b);
+        if (!rc)
+            rc = launch_behind(row_prepare_kernel, dim3((unsigned)cdiv(B, PREP_WARPS)), 32 * PREP_WARPS, 0, st, true, sp, b, B);
         if (!rc && !pl.filters) rc = launch_behind(row_stats_kernel<T, false>, chunks, SMP_THREADS, 0, st, true, sp, b);
         if (!rc && pl.filters) rc = launch_behind(row_stats_kernel<T, true>, chunks, SMP_THREADS, 0, st, true, sp, b);
         if (!rc && pl.filters) rc = launch_behind(row_plan_kernel, rows, SMP_THREADS, 0, st, true, sp, b);
@@ -414,6 +416,7 @@ int cce_b200_sample(const cce_b200_sample_args* a, void* workspace, size_t works
     while ((1LL << log2v) < a->V) ++log2v;
     // V weights of at most 1 << frac_bits stay below 2^63
     sp.frac_bits = std::min(SMP_MAX_FRAC, 62 - log2v);
+    for (int j = 0; j < SMP_TABLE; ++j) sp.table[j] = WeightFn::entry(j, sp.frac_bits);
     char* ws = reinterpret_cast<char*>(workspace);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (a->dtype == CCE_DT_F32) return launch_sample<float>(sp, pl, a->B, ws, st);

@@ -40,6 +40,9 @@ constexpr int SMP_SMEM = 224 * 1024; // dynamic shared memory at most: of the 22
 constexpr double SMP_FLOOR_LOG2 = -40.0;
 constexpr float SMP_LOWEST = -3.402823466e38f;
 
+constexpr int SMP_TABLE = 16;
+constexpr int SMP_MAX_FRAC = 46;
+
 // A setting is an array with a value per row, or one value for all rows.
 struct SampleParams {
     const void* logits;
@@ -58,6 +61,7 @@ struct SampleParams {
     float* logprobs;      // [B] or null
     int slice;            // positions per CTA: a multiple of SMP_BLK
     int frac_bits;        // weight 1 = 1 << frac_bits
+    double table[SMP_TABLE];  // see WeightFn
 };
 
 typedef unsigned long long u64;
@@ -84,15 +88,18 @@ __device__ __forceinline__ float just_below(float x) {
 // The exponent n reaches the table's value by one addition: i << 16 is n << 20 plus j << 16, and the entry of j has
 // that taken off.  A pass over every weight is bound by issuing its instructions (51 per logit with a branch for each and
 // 64-bit integer sums, about 22 as below): the sums are kept in fp64, exact while 128 weights of at most 2^46 meet.
-constexpr int SMP_TABLE = 16;
-constexpr int SMP_MAX_FRAC = 46;
 struct WeightFn {
     double m, scale;  // maximum (the largest finite number for an infinite one), 16 * log2(e) / T
-    uint32_t table;   // shared memory, see fill_table
-    // 2^(frac + j/16), less j << 16 in its high word
-    static __device__ __forceinline__ double entry(int j, int frac) {
+    uint32_t table;   // shared memory: SampleParams::table
+    // its entry j, on the host: 2^(frac + j/16), less j << 16 in its high word
+    static double entry(int j, int frac) {
         const double x = exp2(double(j) / SMP_TABLE + double(frac));
-        return __hiloint2double(__double2hiint(x) - (j << 16), __double2loint(x));
+        long long b;
+        memcpy(&b, &x, 8);
+        b -= (long long)j << 48;
+        double y;
+        memcpy(&y, &b, 8);
+        return y;
     }
     // the rounded weight + 2^52; for m - l beyond the floor (or NaN, -inf) the result means nothing
     __device__ __forceinline__ double raised(float l) const {
@@ -251,6 +258,9 @@ struct RowState {
     unsigned first;    // ROW_GREEDY: the lowest index of the largest logits
     unsigned n_list;
     u64 mass, target;  // top-p alone: all weights, and the running sum to reach
+    // RowBase::prepare's results
+    double scale;
+    float mx, l_floor, l_min, bin_scale;
 };
 
 // What a row's kernels share: its settings, its thresholds, and the arithmetic on them.
@@ -278,19 +288,31 @@ struct RowBase {
     }
     __device__ __forceinline__ bool greedy_row() const { return !(temp > 0.0) || k == 1; }
     __device__ __forceinline__ void make_table() {
-        if (tid < SMP_TABLE) sc.table[tid] = WeightFn::entry(tid, p.frac_bits);
+        if (tid < SMP_TABLE) sc.table[tid] = p.table[tid];
     }
     // from the row's maximum (above -inf): the weights and the thresholds
     __device__ __forceinline__ void prepare(float m) {
         mx = m + 0.0f;
         const double min_p = p.min_p ? double(p.min_p[row]) : p.min_p_all;
         const double k2 = 1.4426950408889634074 / temp;  // exponents of 2 per unit of logit
-        weight.m = double(fminf(mx, -SMP_LOWEST));
         weight.scale = SMP_TABLE * k2;
-        weight.table = smem_u32(sc.table);
+        set_weight();
         l_floor = l_min = lowest_with(SMP_FLOOR_LOG2, k2);
         if (min_p > 0.0) l_min = fmaxf(l_floor, lowest_with(fmax(SMP_FLOOR_LOG2, log2(fmin(min_p, 1.0))), k2));
         bin_scale = fminf(float(SMP_BINS) / (0.5f * mx - 0.5f * l_floor), 1e30f);
+    }
+    __device__ __forceinline__ void set_weight() {
+        weight.m = double(fminf(mx, -SMP_LOWEST));
+        weight.table = smem_u32(sc.table);
+    }
+    // the same as another kernel left it
+    __device__ __forceinline__ void prepare(const RowState& st) {
+        mx = st.mx;
+        l_floor = st.l_floor;
+        l_min = st.l_min;
+        bin_scale = st.bin_scale;
+        weight.scale = st.scale;
+        set_weight();
     }
     // The smallest logit whose weight is at least 2^x (x <= 0): a first guess, then the neighbours.  A weight
     // that rounds to 1 in fp64, exp(z) with z >= -2^-54, counts as 1.

@@ -6,10 +6,11 @@
 // weights cost (0.25 cycles per logit and SM), and what a barrier did is the end of a kernel.  Below some tens of
 // megabytes the launches cost more than the barriers (api_serving.cuh has the rule).
 //
-//   row_max_kernel     the largest logit of every chunk; clears the row's state
+//   row_max_kernel     the largest logit of every chunk
+//   row_prepare_kernel per row (a warp): its maximum and thresholds, and whether there is anything to do (RowMode)
 //   row_stats_kernel   counts by bin and, for top-p alone, the exact sum of the weights; without any filter: the
 //                      weights by blocks of 512 positions
-//   row_plan_kernel    per row: which logits are needed in order (RowMode)
+//   row_plan_kernel    per row with a filter: which logits are needed in order
 //   row_pass_kernel    gathers them, and sums the kept weights by blocks where not everything is gathered
 //   row_draw_kernel    per row: the border among the gathered, the draw
 //   sample_kernel      the rows that no list holds (ROW_BY_CLUSTER)
@@ -111,18 +112,37 @@ row_max_kernel(const SampleParams p, const StreamBuffers b) {
 #pragma unroll
         for (int w = 0; w < SMP_WARPS; ++w) m = fmaxf(m, wf[w]);
         b.chunk_max[row * b.n_chunk + chunk] = m;
-        if (chunk == 0) b.state[row] = RowState{ROW_SUM, 0.0f, 0.0f, 0xffffffffu, 0, 0, 0};
     }
 }
 
-// the row's maximum from its chunks', in every thread
-__device__ __forceinline__ float stream_max(const StreamBuffers& b, long long row) {
-    const int lane = threadIdx.x & 31;
+// A warp per row.
+constexpr int PREP_WARPS = 4;
+__global__ void __launch_bounds__(32 * PREP_WARPS)
+row_prepare_kernel(const SampleParams p, const StreamBuffers b, long long B) {
+    __shared__ CtaScratch sc;  // unused by what is called here
+    pdl_launch();
+    const long long row = (long long)blockIdx.x * PREP_WARPS + (threadIdx.x >> 5);
+    pdl_wait();
+    if (row >= B) return;
+    RowBase r(p, sc, row);
     float m = -INFINITY;
-    for (int i = lane; i < b.n_chunk; i += 32) m = fmaxf(m, b.chunk_max[row * b.n_chunk + i]);
+    for (int i = r.lane; i < b.n_chunk; i += 32) m = fmaxf(m, b.chunk_max[row * b.n_chunk + i]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    return m;
+    if (r.lane != 0) return;
+    RowState st = {};
+    st.mode = !(m > -INFINITY) ? ROW_DONE : r.greedy_row() ? ROW_GREEDY : r.k || r.top_p < 1.0 ? ROW_LIST : ROW_SUM;
+    st.first = 0xffffffffu;
+    st.mx = m;
+    if (st.mode == ROW_LIST || st.mode == ROW_SUM) {
+        r.prepare(m);
+        st.scale = r.weight.scale;
+        st.mx = r.mx;
+        st.l_floor = r.l_floor;
+        st.l_min = r.l_min;
+        st.bin_scale = r.bin_scale;
+    }
+    b.state[row] = st;
 }
 
 // FILTERS: some row may have top-k or top-p
@@ -140,10 +160,9 @@ row_stats_kernel(const SampleParams p, const StreamBuffers b) {
         for (int i = r.tid; i < SMP_BINS; i += SMP_THREADS) hist[i] = 0;
     const RowStream<T> rs(p, row);
     pdl_wait();
-    if (FILTERS && !r.k && !(r.top_p < 1.0)) return;
-    const float m = stream_max(b, row);
-    if (!(m > -INFINITY) || r.greedy_row()) return;
-    r.prepare(m);
+    const RowState st = b.state[row];
+    if (st.mode != (FILTERS ? ROW_LIST : ROW_SUM)) return;
+    r.prepare(st);
     __syncthreads();
     double sum_d = 0.0;
     const bool want_sum = !r.k;
@@ -192,16 +211,9 @@ row_plan_kernel(const SampleParams p, const StreamBuffers b) {
         hi = at_bin = -1;
     }
     pdl_wait();
-    const float m = stream_max(b, row);
     RowState st = b.state[row];
-    if (!(m > -INFINITY)) {
-        st.mode = ROW_DONE;
-    } else if (r.greedy_row()) {
-        st.mode = ROW_GREEDY;
-    } else if (!r.k && !(r.top_p < 1.0)) {
-        st.mode = ROW_SUM;
-    } else {
-        r.prepare(m);
+    if (st.mode == ROW_LIST) {
+        r.prepare(st);
         uint32_t cnt[PER];
         double est[PER];
         const double step = -2.0 / double(r.bin_scale) * r.weight.scale * (1.0 / SMP_TABLE);  // log2 of a weight per bin
@@ -307,21 +319,20 @@ row_pass_kernel(const SampleParams p, const StreamBuffers b) {
     pdl_wait();
     const RowState st = b.state[row];
     if (st.mode == ROW_DONE || st.mode == ROW_BY_CLUSTER) return;
-    const float m = stream_max(b, row);
     if (st.mode == ROW_GREEDY) {
         unsigned best = 0xffffffffu;
         for (int i = r.warp; i < STR_BLOCKS; i += SMP_WARPS) {
             const long long block = (long long)chunk * STR_BLOCKS + i;
             if (rs.holds(block))
                 rs.each(block, r.lane, [&](float l, long long pos) {
-                    if (l == m) best = min(best, unsigned(pos - rs.phase));
+                    if (l == st.mx) best = min(best, unsigned(pos - rs.phase));
                 });
         }
         best = __reduce_min_sync(0xffffffffu, best);
         if (r.lane == 0 && best != 0xffffffffu) atomicMin(&b.state[row].first, best);
         return;
     }
-    r.prepare(m);
+    r.prepare(st);
     __syncthreads();
     double above_d = 0.0;
     for (int i = r.warp; i < STR_BLOCKS; i += SMP_WARPS) {
@@ -378,9 +389,8 @@ row_draw_kernel(const SampleParams p, const StreamBuffers b) {
     if (r.tid == 0) sc.r[0] = 0;
     pdl_wait();
     const RowState st = b.state[row];
-    const float m = stream_max(b, row);
     if (st.mode == ROW_BY_CLUSTER) return;
-    if (!(m > -INFINITY)) {
+    if (st.mode == ROW_DONE) {
         if (r.tid == 0) r.write(-1, -INFINITY);
         return;
     }
@@ -388,7 +398,7 @@ row_draw_kernel(const SampleParams p, const StreamBuffers b) {
         if (r.tid == 0) r.write((long long)st.first, 0.0f);
         return;
     }
-    r.prepare(m);
+    r.prepare(st);
     __syncthreads();
     const int n_blk = b.n_chunk * STR_BLOCKS;
     u64 cut = ~0ull;
