@@ -147,7 +147,7 @@ row_prepare_kernel(const SampleParams p, const StreamBuffers b, long long B) {
 
 // FILTERS: some row may have top-k or top-p
 template <typename T, bool FILTERS>
-__global__ void __launch_bounds__(SMP_THREADS, 2)
+__global__ void __launch_bounds__(SMP_THREADS, 3)
 row_stats_kernel(const SampleParams p, const StreamBuffers b) {
     __shared__ CtaScratch sc;
     __shared__ uint32_t hist[FILTERS ? SMP_BINS : 1];
@@ -304,7 +304,7 @@ row_plan_kernel(const SampleParams p, const StreamBuffers b) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(SMP_THREADS, 2)
+__global__ void __launch_bounds__(SMP_THREADS, 3)
 row_pass_kernel(const SampleParams p, const StreamBuffers b) {
     __shared__ CtaScratch sc;
     __shared__ u64 local[SMP_LIST];
