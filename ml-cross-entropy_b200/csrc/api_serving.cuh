@@ -167,8 +167,10 @@ int plan_sample(const cce_b200_sample_args* a, SamplePlan* out) {
     if (pl.smem > SMP_SMEM) return CCE_ERR_TOO_LARGE;
     if (a->B * pl.cluster >= (1LL << 31)) return CCE_ERR_ARG;
     pl.filters = a->top_k || a->top_p || a->top_k_all > 0 || a->top_p_all < 1.0;
-    static const long long kStream = getenv("STREAM") ? atoll(getenv("STREAM")) : (8LL << 20);
-    pl.stream = a->B * a->V >= kStream;
+    // From 32 MB of logits on the streaming kernels win: fp32, no filters / top-p / top-k and top-p, 64 x 128000: 41 / 84 /
+    // 55 us against one cluster per row's 41 / 109 / 55, 128 x 256000: 92 / 182 / 121 against 133 / 334 / 162; bf16,
+    // 64 x 128000: 37 / 80 / 53 against 31 / 72 / 39, 128 x 128000: 51 / 109 / 72 against 51 / 127 / 64.
+    pl.stream = a->B * a->V * elem >= (32LL << 20);
     pl.total = 256;
     if (pl.stream) {
         pl.n_chunk = (int)cdiv(a->V + 16 / elem - 1, STR_CHUNK);
@@ -183,7 +185,7 @@ int plan_sample(const cce_b200_sample_args* a, SamplePlan* out) {
         pl.off_max = take(chunks * sizeof(float));
         pl.off_sum = take(chunks * sizeof(u64));
         pl.off_blk = take(chunks * STR_BLOCKS * sizeof(u64));
-        pl.off_hist = take(pl.filters ? (size_t)a->B * SMP_BINS * sizeof(uint32_t) : 0);
+        pl.off_hist = take(pl.filters ? (size_t)a->B * STR_BINS * sizeof(uint32_t) : 0);
         pl.off_list = take(pl.filters ? (size_t)a->B * SMP_LIST * sizeof(u64) : 0);
         pl.total = off;
     }
@@ -217,8 +219,8 @@ int launch_sample(const SampleParams& sp, const SamplePlan& pl, long long B, cha
         only = b.state;
     }
     cudaLaunchConfig_t cfg = {};
-    // behind the streaming kernels few rows are left, if any
-    cfg.gridDim = dim3((unsigned)((only ? std::min<long long>(B, 16) : B) * pl.cluster));
+    // behind the streaming kernels few rows are left, if any: what the GPU holds at a time
+    cfg.gridDim = dim3((unsigned)((only ? std::min<long long>(B, 256 / pl.cluster) : B) * pl.cluster));
     cfg.blockDim = dim3(SMP_THREADS);
     cfg.dynamicSmemBytes = pl.smem;
     cfg.stream = st;

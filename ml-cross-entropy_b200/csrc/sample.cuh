@@ -168,7 +168,7 @@ struct CtaScratch {
 struct SmpShared : CtaScratch {
     u64 x[2][4][SMP_MAX_CLUSTER];  // exchange slots, written by the whole cluster
     float wf[SMP_WARPS];
-    uint32_t n_local, n_list, base;
+    uint32_t n_local, n_list, base, key[4];
     int lo, hi, all;
 };
 
@@ -269,6 +269,7 @@ struct RowBase {
     CtaScratch& sc;
     long long row;
     int tid, warp, lane;
+    int n_bins = SMP_BINS;  // of the histogram over the logits, set before prepare
     float mx, l_floor, l_min, bin_scale;
     double temp, top_p;
     float u;
@@ -299,7 +300,7 @@ struct RowBase {
         set_weight();
         l_floor = l_min = lowest_with(SMP_FLOOR_LOG2, k2);
         if (min_p > 0.0) l_min = fmaxf(l_floor, lowest_with(fmax(SMP_FLOOR_LOG2, log2(fmin(min_p, 1.0))), k2));
-        bin_scale = fminf(float(SMP_BINS) / (0.5f * mx - 0.5f * l_floor), 1e30f);
+        bin_scale = fminf(float(n_bins) / (0.5f * mx - 0.5f * l_floor), 1e30f);
     }
     __device__ __forceinline__ void set_weight() {
         weight.m = double(fminf(mx, -SMP_LOWEST));
@@ -333,7 +334,7 @@ struct RowBase {
     // ---- histogram level 0: bins linear in the logit, bin 0 at the maximum (halves: the difference of two floats
     // may overflow).  The bin falls, or stays, as the logit grows.
     __device__ __forceinline__ int bin0(float l) const {
-        return min(SMP_BINS - 1, int((0.5f * mx - 0.5f * l) * bin_scale));
+        return min(n_bins - 1, int((0.5f * mx - 0.5f * l) * bin_scale));
     }
     // The first key of [lo, hi] that fulfils a predicate which holds from some key on (hi if none before it does),
     // by all threads together
@@ -751,6 +752,10 @@ struct Sampler : RowBase {
         // the keys of bin bd.bin: from the first with bin0 <= bin, up to the one before the first with bin0 < bin
         uint32_t lo = first_key(kmin, kmax, [&](uint32_t q) { return bin0(order_value(q)) <= bd.bin; });
         uint32_t hi = bd.bin == 0 ? kmax : first_key(lo, kmax, [&](uint32_t q) { return bin0(order_value(q)) < bd.bin; }) - 1;
+        return descend_keys(lo, hi, bd, by_mass, target);
+    }
+    // likewise from the keys lo..hi; bd: what lies above them
+    __device__ __forceinline__ Level descend_keys(uint32_t lo, uint32_t hi, Border bd, bool by_mass, u64 target) {
         while (hi > lo) {
             const int shift = max(0, 32 - __clz(hi - lo) - 11);  // (hi - lo) >> shift < SMP_BINS
             const float f_lo = order_value(lo), f_hi = order_value(hi);
@@ -813,7 +818,7 @@ struct Sampler : RowBase {
     // CTA `owner`, with at most SMP_LIST logits.  all: the logits down to hi fit the list, and reach the target for certain.
     struct Window {
         int owner, lo, hi;
-        bool all, none;  // none: the bin of the estimate alone is too full
+        bool all, none;  // none: the bin of the estimate (lo = hi) alone is too full
     };
     __device__ __forceinline__ Window p_window(u64& mass, u64& target, u64 sum) {
         u64 unused = 0;
@@ -914,9 +919,11 @@ struct Sampler : RowBase {
         __syncthreads();
         // sm.all: a bin down to which everything fits the list and reaches the target
         exchange(u64(owner * lay.share + sm.lo), u64(sm.hi < 0 ? 0 : owner * lay.share + sm.hi + 1),
-                 u64(sm.all == lay.share ? 0 : owner * lay.share + sm.all + 1));
+                 u64(sm.all == lay.share ? 0 : owner * lay.share + sm.all + 1),
+                 u64(owner * lay.share + min(int(sm.r[3] >> 40), lay.share - 1)));
         const int hi = int(got(1, owner)) - 1, all = int(got(2, owner)) - 1;
-        return Window{owner, int(got(0, owner)), all >= 0 ? all : hi, all >= 0, hi < 0};
+        if (hi < 0) return Window{owner, int(got(3, owner)), int(got(3, owner)), false, true};
+        return Window{owner, int(got(0, owner)), all >= 0 ? all : hi, all >= 0, false};
     }
 
     // The exact border of top-p in the window.  Leaves the kept weights by blocks in blk_mass; the key of the last
@@ -976,8 +983,73 @@ struct Sampler : RowBase {
         return cut;
     }
 
+    // The border of top-p by exact sums, in bins lo..hi or, one bin after the other, in the few next to them.  False: it
+    // is not there.
+    __device__ __forceinline__ bool search_near(int lo, int hi, u64 target, Level& found) {
+        float edge = lo == 0 ? INFINITY : lowest_of_bins(lo - 1), last = lowest_of_bins(hi);
+        for (int attempt = 0; attempt < 8; ++attempt) {
+            double above_d = 0.0, with_d = 0.0;
+            // keys: the next value below, the (inverted) next from the edge on; the largest and (inverted) smallest between
+            uint32_t q[4] = {0, 0, 0, 0};
+            for (int b = warp; b < n_blk; b += SMP_WARPS)
+                each_piece(b, [&](const float (&l)[VE], int) {
+                    weight.sum_weights(l, edge, above_d);
+                    weight.sum_weights(l, last, with_d);
+#pragma unroll
+                    for (int i = 0; i < VE; ++i) {
+                        const uint32_t key = order_key(l[i]);
+                        if (l[i] >= edge) {
+                            q[1] = max(q[1], ~key);
+                        } else if (l[i] >= last) {
+                            q[2] = max(q[2], key);
+                            q[3] = max(q[3], ~key);
+                        } else if (l[i] >= l_floor) {
+                            q[0] = max(q[0], key);
+                        }
+                    }
+                });
+            u64 above = u64(above_d), with = u64(with_d);
+            __syncthreads();
+            if (tid < 4) sm.key[tid] = 0;
+            cta_sum(above, with);  // its barriers stand between the clearing and the maxima
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t m = __reduce_max_sync(0xffffffffu, q[i]);
+                if (lane == 0) atomicMax(&sm.key[i], m);
+            }
+            __syncthreads();
+            exchange(above, with, u64(sm.key[0]) << 32 | sm.key[1], u64(sm.key[2]) << 32 | sm.key[3]);
+            above = with = 0;
+            for (int i = 0; i < 4; ++i) q[i] = 0;
+            for (int r = 0; r < size; ++r) {
+                above += got(0, r);
+                with += got(1, r);
+                q[0] = max(q[0], uint32_t(got(2, r) >> 32));
+                q[1] = max(q[1], uint32_t(got(2, r)));
+                q[2] = max(q[2], uint32_t(got(3, r) >> 32));
+                q[3] = max(q[3], uint32_t(got(3, r)));
+            }
+            if (above < target && target <= with) {
+                found = descend_keys(~q[3], q[2], Border{0, 0, above, 0, 0}, true, target);
+                return true;
+            }
+            if (target <= above) {
+                if (!q[1]) return false;
+                const int bin = bin0(order_value(~q[1]));
+                last = edge;
+                edge = bin == 0 ? INFINITY : lowest_of_bins(bin - 1);
+            } else {
+                if (!q[0]) return false;
+                edge = last;
+                last = lowest_of_bins(bin0(order_value(q[0])));
+            }
+        }
+        return false;
+    }
+
     // ---- the key of the last kept logit by narrowing histograms, for borders that no list holds
-    __device__ __forceinline__ u64 cut_by_levels(bool top_k_cuts, const Border& k_border, u64 k_target) {
+    // hint_lo..hint_hi: the bins where the border of top-p alone is expected, or -1.
+    __device__ __forceinline__ u64 cut_by_levels(bool top_k_cuts, const Border& k_border, u64 k_target, int hint_lo, int hint_hi) {
         Level lv{-INFINITY, 0, 0};
         long long n_tie = 0;  // how many of the logits equal to lv.value are kept
         if (top_k_cuts) {
@@ -995,9 +1067,12 @@ struct Sampler : RowBase {
             for (int r = 0; r < size; ++r) mass += got(0, r);
             if (n_tie > 0) mass += u64(n_tie) * weight(lv.value);
             const u64 target = p_target(mass);
-            level0(true);
-            exchange_totals();
-            const Level lp = descend(find_border(true, target, 0, 0), true, target);
+            Level lp{0.0f, 0, 0};
+            if (hint_lo < 0 || !search_near(hint_lo, hint_hi, target, lp)) {
+                level0(true);
+                exchange_totals();
+                lp = descend(find_border(true, target, 0, 0), true, target);
+            }
             const u64 w = weight(lp.value);
             long long need = (long long)((target - lp.mass_above + w - 1) / w);  // the mass above is short of the target
             if (n_tie > 0 && lp.value == lv.value) need = min(need, n_tie);
@@ -1160,7 +1235,7 @@ struct Sampler : RowBase {
                 finish_on_list(bd.bin, bd.owner, 0);
                 return;
             }
-            cut = cut_by_levels(u64(k) < cnt, bd, target);
+            cut = cut_by_levels(u64(k) < cnt, bd, target, -1, -1);
         } else {
             const u64 sum = level0_counts_and_sum();
             u64 mass, target;
@@ -1174,7 +1249,7 @@ struct Sampler : RowBase {
                 draw(cut);
                 return;
             }
-            cut = cut_by_levels(false, Border{}, 0);
+            cut = cut_by_levels(false, Border{}, 0, win.lo, win.hi);
         }
         sum_blocks(cut);
         draw(cut);

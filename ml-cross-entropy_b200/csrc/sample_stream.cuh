@@ -23,6 +23,9 @@ namespace cce {
 
 constexpr int STR_BLOCKS = 32;                       // blocks of SMP_BLK positions per chunk
 constexpr int STR_CHUNK = STR_BLOCKS * SMP_BLK;
+// Twice as many as a cluster's: a bin of a long row of 16-bit logits held up to 900 equal or nearly equal ones, so that
+// one beside the estimate's did not fit the window's list and the row went to sample_kernel.
+constexpr int STR_BINS = 2 * SMP_BINS;
 
 // Workspace of a call; per row where not said otherwise.
 struct StreamBuffers {
@@ -30,7 +33,7 @@ struct StreamBuffers {
     float* chunk_max;   // [n_chunk]
     u64* chunk_sum;     // [n_chunk]
     u64* blk_mass;      // [n_chunk * STR_BLOCKS]
-    uint32_t* hist;     // [SMP_BINS]
+    uint32_t* hist;     // [STR_BINS]
     u64* list;          // [SMP_LIST]
     int n_chunk;
 };
@@ -105,8 +108,8 @@ row_max_kernel(const SampleParams p, const StreamBuffers b) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) wf[warp] = m;
-    for (int i = chunk * SMP_THREADS + tid; b.hist && i < SMP_BINS; i += b.n_chunk * SMP_THREADS)
-        b.hist[row * SMP_BINS + i] = 0;
+    for (int i = chunk * SMP_THREADS + tid; b.hist && i < STR_BINS; i += b.n_chunk * SMP_THREADS)
+        b.hist[row * STR_BINS + i] = 0;
     __syncthreads();
     if (tid == 0) {
 #pragma unroll
@@ -125,6 +128,7 @@ row_prepare_kernel(const SampleParams p, const StreamBuffers b, long long B) {
     pdl_wait();
     if (row >= B) return;
     RowBase r(p, sc, row);
+    r.n_bins = STR_BINS;
     float m = -INFINITY;
     for (int i = r.lane; i < b.n_chunk; i += 32) m = fmaxf(m, b.chunk_max[row * b.n_chunk + i]);
 #pragma unroll
@@ -150,14 +154,15 @@ template <typename T, bool FILTERS>
 __global__ void __launch_bounds__(SMP_THREADS, 3)
 row_stats_kernel(const SampleParams p, const StreamBuffers b) {
     __shared__ CtaScratch sc;
-    __shared__ uint32_t hist[FILTERS ? SMP_BINS : 1];
+    __shared__ uint32_t hist[FILTERS ? STR_BINS : 1];
     pdl_launch();
     const long long row = blockIdx.x / b.n_chunk;
     const int chunk = blockIdx.x % b.n_chunk;
     RowBase r(p, sc, row);
+    r.n_bins = STR_BINS;
     r.make_table();
     if (FILTERS)
-        for (int i = r.tid; i < SMP_BINS; i += SMP_THREADS) hist[i] = 0;
+        for (int i = r.tid; i < STR_BINS; i += SMP_THREADS) hist[i] = 0;
     const RowStream<T> rs(p, row);
     pdl_wait();
     const RowState st = b.state[row];
@@ -192,22 +197,23 @@ row_stats_kernel(const SampleParams p, const StreamBuffers b) {
     u64 sum = u64(sum_d), unused = 0;
     r.cta_sum(sum, unused);  // a barrier: the counts are complete
     if (r.tid == 0) b.chunk_sum[row * b.n_chunk + chunk] = sum;
-    for (int i = r.tid; i < SMP_BINS; i += SMP_THREADS)
-        if (hist[i]) atomicAdd(&b.hist[row * SMP_BINS + i], hist[i]);
+    for (int i = r.tid; i < STR_BINS; i += SMP_THREADS)
+        if (hist[i]) atomicAdd(&b.hist[row * STR_BINS + i], hist[i]);
 }
 
 // One CTA per row: the border's bin (top-k) or the window around its estimate (top-p alone), as in sample.cuh.
 __global__ void __launch_bounds__(SMP_THREADS, 2)
 row_plan_kernel(const SampleParams p, const StreamBuffers b) {
-    constexpr int PER = SMP_BINS / SMP_THREADS;
+    constexpr int PER = STR_BINS / SMP_THREADS;
     __shared__ CtaScratch sc;
     __shared__ int lo, hi, all, at_bin;
     __shared__ u64 at_above;
     pdl_launch();
     const long long row = blockIdx.x;
     RowBase r(p, sc, row);
+    r.n_bins = STR_BINS;
     if (r.tid == 0) {
-        lo = all = SMP_BINS;
+        lo = all = STR_BINS;
         hi = at_bin = -1;
     }
     pdl_wait();
@@ -223,7 +229,7 @@ row_plan_kernel(const SampleParams p, const StreamBuffers b) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int bin = r.tid * PER + i;
-            cnt[i] = b.hist[row * SMP_BINS + bin];
+            cnt[i] = b.hist[row * STR_BINS + bin];
             est[i] = cnt[i] ? double(cnt[i]) * unit * double(ex2f(float((double(bin) + 0.5) * step))) : 0.0;
             tm += est[i];
             tc += cnt[i];
@@ -268,7 +274,7 @@ row_plan_kernel(const SampleParams p, const StreamBuffers b) {
             at_above = above;
         }
         __syncthreads();
-        const u64 n_at = at_bin < 0 ? ~0ull : u64(b.hist[row * SMP_BINS + max(at_bin, 0)]);
+        const u64 n_at = at_bin < 0 ? ~0ull : u64(b.hist[row * STR_BINS + max(at_bin, 0)]);
         if (at_bin < 0 || n_at > SMP_LIST) {
             st.mode = ROW_BY_CLUSTER;
         } else if (r.k) {
@@ -290,8 +296,8 @@ row_plan_kernel(const SampleParams p, const StreamBuffers b) {
                 c += cnt[i];
             }
             __syncthreads();
-            st.mode = all < SMP_BINS ? ROW_LIST : ROW_WINDOW;
-            if (all < SMP_BINS) hi = all;  // by every thread alike
+            st.mode = all < STR_BINS ? ROW_LIST : ROW_WINDOW;
+            if (all < STR_BINS) hi = all;  // by every thread alike
         }
         __syncthreads();
         if (st.mode == ROW_LIST || st.mode == ROW_WINDOW) {
@@ -313,6 +319,7 @@ row_pass_kernel(const SampleParams p, const StreamBuffers b) {
     const long long row = blockIdx.x / b.n_chunk;
     const int chunk = blockIdx.x % b.n_chunk;
     RowBase r(p, sc, row);
+    r.n_bins = STR_BINS;
     const RowStream<T> rs(p, row);
     r.make_table();
     if (r.tid == 0) n_local = 0;
@@ -385,6 +392,7 @@ row_draw_kernel(const SampleParams p, const StreamBuffers b) {
     u64* const blk = list + 3 * SMP_LIST;
     const long long row = blockIdx.x;
     RowBase r(p, sc, row);
+    r.n_bins = STR_BINS;
     r.make_table();
     if (r.tid == 0) sc.r[0] = 0;
     pdl_wait();

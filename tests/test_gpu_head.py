@@ -247,7 +247,7 @@ def _check_sample(logits, u, **kw):
     lp = lp.cpu().double()
     none = torch.isinf(ref_lp)
     assert torch.equal(torch.isinf(lp), none)
-    # rounding to fp32 (half a step), and weights rounded to 2^-43 of the largest in a sum of at least one
+    # rounding to fp32 (half a step), and weights rounded to at worst half of 2^-42 of the largest, in a sum of at least one
     tol = 2.0**-24 * ref_lp.abs() * 1.01 + 2.0**-43 * logits.size(-1) + 1e-12
     assert bool(((lp - ref_lp).abs()[~none] <= tol[~none]).all())
     assert torch.equal(sample_tokens(logits, u, **kw), tok)
@@ -389,6 +389,50 @@ def test_sample_strides_and_alignment(dtype):
     assert torch.equal(sample_tokens(x.t().contiguous().t(), u, **kw), want)
     assert torch.equal(sample_tokens(x[:1].expand(9, -1), u, **kw)[:1], want[:1])
     assert torch.equal(sample_tokens(x[::2], u[::2], **kw), want[::2])
+
+
+@pytest.mark.parametrize("dtype, B", [(FP32, 70), (BF16, 140)])
+@pytest.mark.parametrize("name", list(SETTINGS))
+def test_sample_many_long_rows(name, dtype, B):
+    """Enough logits for the streaming kernels, with odd lengths, strides and extreme rows; a row alone, which takes
+    the other path, gives the same token."""
+    V, kw = 120_011, SETTINGS[name]
+    x, u = _rows(B, V + 3, dtype, seed=21)
+    x = x[:, 1 : V + 1]
+    x[0] = -math.inf
+    x[1] = 2.0
+    x[2] = torch.finfo(dtype).min
+    x[3, ::2] = math.nan
+    x[4, 5::7] = -math.inf
+    x[5, 77777] = math.inf
+    x[6, :] = torch.linspace(-40, 0, V, device=DEV).to(dtype)
+    x[7] *= 0.001
+    x[8] = torch.where(torch.arange(V, device=DEV) % 5 == 0, 1.0, -1.0).to(dtype)
+    assert x.numel() * x.element_size() >= 32 << 20
+    tok, lp = sample_tokens(x, u, return_logprobs=True, **kw)
+    rows = list(range(12)) + list(range(12, B, 16))  # the oracle sorts in 64 bits: some of the rows
+    ref_tok, ref_lp = H.sample_tokens(x[rows].cpu(), u[rows].cpu(), **kw)
+    assert torch.equal(tok[rows].cpu(), ref_tok)
+    finite = torch.isfinite(ref_lp)
+    err = (lp[rows].cpu().double() - ref_lp).abs()[finite]
+    assert bool((err <= 2.0**-24 * ref_lp.abs()[finite] * 1.01 + 2.0**-42 * V + 1e-12).all())
+    for i in (0, 1, 5, 8, 30, B - 1):
+        assert sample_tokens(x[i], u[i], **kw).item() == tok[i].item()
+
+
+def test_sample_many_long_rows_with_their_own_settings():
+    B, V = 70, 120_001
+    x, u = _rows(B, V, FP32, seed=31)
+    g = torch.Generator().manual_seed(32)
+    r = lambda: torch.rand(B, generator=g).to(DEV)
+    kw = dict(
+        temperature=torch.where(r() < 0.2, 0.0, 0.2 + 2 * r()),
+        top_k=torch.where(r() < 0.5, 0, (r() ** 4 * 2 * V).long()),
+        top_p=torch.where(r() < 0.4, 1.0, r()),
+        min_p=torch.where(r() < 0.5, 0.0, 0.3 * r()),
+    )
+    kw["top_k"][:5], kw["top_p"][:5] = 0, 1.0  # nothing cut off, in the company of filters
+    _check_sample(x, u, **kw)
 
 
 def test_sample_empty_and_too_large():
