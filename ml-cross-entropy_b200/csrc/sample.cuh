@@ -983,8 +983,8 @@ struct Sampler : RowBase {
         return cut;
     }
 
-    // The border of top-p by exact sums, in bins lo..hi or, one bin after the other, in the few next to them.  False: it
-    // is not there.
+    // The border of top-p by exact sums, in bins lo..hi or in those next to them, 1, 2, 4, .. at a time.  False: it is not
+    // there.
     __device__ __forceinline__ bool search_near(int lo, int hi, u64 target, Level& found) {
         float edge = lo == 0 ? INFINITY : lowest_of_bins(lo - 1), last = lowest_of_bins(hi);
         for (int attempt = 0; attempt < 8; ++attempt) {
@@ -1035,21 +1035,22 @@ struct Sampler : RowBase {
             }
             if (target <= above) {
                 if (!q[1]) return false;
-                const int bin = bin0(order_value(~q[1]));
+                const int bin = bin0(order_value(~q[1])) - (1 << attempt);
                 last = edge;
-                edge = bin == 0 ? INFINITY : lowest_of_bins(bin - 1);
+                edge = bin < 0 ? INFINITY : lowest_of_bins(bin);
             } else {
                 if (!q[0]) return false;
                 edge = last;
-                last = lowest_of_bins(bin0(order_value(q[0])));
+                last = lowest_of_bins(min(n_bins - 1, bin0(order_value(q[0])) + (1 << attempt) - 1));
             }
         }
         return false;
     }
 
     // ---- the key of the last kept logit by narrowing histograms, for borders that no list holds
-    // hint_lo..hint_hi: the bins where the border of top-p alone is expected, or -1.
-    __device__ __forceinline__ u64 cut_by_levels(bool top_k_cuts, const Border& k_border, u64 k_target, int hint_lo, int hint_hi) {
+    // For top-p alone: the mass of all weights, and the bins where the border is expected.
+    __device__ __forceinline__ u64 cut_by_levels(bool top_k_cuts, const Border& k_border, u64 k_target, u64 mass, int hint_lo,
+                                                 int hint_hi) {
         Level lv{-INFINITY, 0, 0};
         long long n_tie = 0;  // how many of the logits equal to lv.value are kept
         if (top_k_cuts) {
@@ -1057,15 +1058,17 @@ struct Sampler : RowBase {
             n_tie = (long long)(k_target - lv.cnt_above);
         }
         if (top_p < 1.0) {
-            // the masses, of the top-k and of every bin
-            u64 s = 0, unused = 0, mass = 0;
-            each_of_slice([&](float l, int) {
-                if (l > lv.value && l >= l_floor) s += weight(l);
-            });
-            cta_sum(s, unused);
-            exchange(s);
-            for (int r = 0; r < size; ++r) mass += got(0, r);
-            if (n_tie > 0) mass += u64(n_tie) * weight(lv.value);
+            if (k) {  // the mass of the top-k
+                const float from = n_tie > 0 ? fmaxf(l_floor, order_value(order_key(lv.value) + 1)) : l_floor;
+                double sum = 0.0;
+                for (int b = warp; b < n_blk; b += SMP_WARPS)
+                    each_piece(b, [&](const float (&l)[VE], int) { weight.sum_weights(l, from, sum); });
+                u64 s = u64(sum), unused = 0;
+                cta_sum(s, unused);
+                exchange(s);
+                mass = n_tie > 0 ? u64(n_tie) * weight(lv.value) : 0;
+                for (int r = 0; r < size; ++r) mass += got(0, r);
+            }
             const u64 target = p_target(mass);
             Level lp{0.0f, 0, 0};
             if (hint_lo < 0 || !search_near(hint_lo, hint_hi, target, lp)) {
@@ -1235,7 +1238,7 @@ struct Sampler : RowBase {
                 finish_on_list(bd.bin, bd.owner, 0);
                 return;
             }
-            cut = cut_by_levels(u64(k) < cnt, bd, target, -1, -1);
+            cut = cut_by_levels(u64(k) < cnt, bd, target, 0, -1, -1);
         } else {
             const u64 sum = level0_counts_and_sum();
             u64 mass, target;
@@ -1249,7 +1252,7 @@ struct Sampler : RowBase {
                 draw(cut);
                 return;
             }
-            cut = cut_by_levels(false, Border{}, 0, win.lo, win.hi);
+            cut = cut_by_levels(false, Border{}, 0, mass, win.lo, win.hi);
         }
         sum_blocks(cut);
         draw(cut);
