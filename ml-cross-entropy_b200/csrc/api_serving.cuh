@@ -255,6 +255,7 @@ int cce_b200_logits(const cce_b200_logits_args* a, void* workspace, size_t works
     const LogitsPlan pl = plan_logits(a);
     if (workspace_bytes < pl.total) return CCE_ERR_WORKSPACE;
     if (reinterpret_cast<uintptr_t>(workspace) & 255) return CCE_ERR_ALIGN;
+    if (pl.n_col >= (1LL << 31) - BN) return CCE_ERR_ARG;
     DeviceInfo* dev;
     rc = device_info(&dev);
     if (rc) return rc;

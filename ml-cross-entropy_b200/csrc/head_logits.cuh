@@ -306,8 +306,10 @@ __device__ __forceinline__ void finish_chunk(const HeadParams& p, const HeadTile
     }
     if (p.has_softcap) {
         const float inv = 1.0f / p.softcap;
+        // fp32 logits: the special-function tanh (1e-7 of the cap) would be their largest error
 #pragma unroll
-        for (int j = 0; j < 32; ++j) x[j] = apply_softcap(x[j], p.softcap, inv);
+        for (int j = 0; j < 32; ++j)
+            x[j] = FP32_OUT ? p.softcap * tanhf(x[j] * inv) : apply_softcap(x[j], p.softcap, inv);
     }
     if (FP32_OUT || p.out_dtype == 2)
         store_chunk<float>(p, v, my_token, x);
