@@ -215,6 +215,12 @@ def test_logits_groups_of_one_adapter_and_mixed_ones(dtype, r):
         _check_logits(kw, out_dtype=out)
 
 
+@pytest.mark.parametrize("T, n", [(1024, 3), (1025, 60), (2500, 200), (9000, 1100), (300, 9000)])
+def test_logits_many_tokens_and_adapters(T, n):
+    """Column orders of more than one block's width of tokens and of adapters, and too many adapters for an order."""
+    _check_logits(_inputs(T, 40, 64, BF16, n=n, r=8, seed=T), out_dtype=FP32)
+
+
 def test_logits_inner_products_beyond_the_16_bit_type():
     """h above fp16's range: such groups take their adapter in fp32."""
     kw = _inputs(64, 300, 128, FP16, n=2, r=16)
