@@ -330,10 +330,10 @@ int cce_b200_logits(const cce_b200_logits_args* a, void* workspace, size_t works
     const long long room = head_segmented(hp) ? 192 : BN;
     const long long n_ntile = cdiv(pl.n_col, room);
     hp.n_tok = n_ntile > 1 && pl.sorted ? (int)room : (int)(cdiv(cdiv(pl.n_col, n_ntile), HEAD_GROUP) * HEAD_GROUP);
-    hp.e_step = n_ntile > 1 && pl.sorted ? hp.n_tok / 2 / HEAD_E_MAPS : hp.n_tok / 2;
+    // where the device counts the columns, four sizes of token loads, in whole groups of 8 rows
+    hp.e_step = pl.sorted ? (int)(cdiv(cdiv(hp.n_tok / 2, HEAD_E_MAPS), 8) * 8) : hp.n_tok / 2;
     hp.n_acc = hp.n_tok <= 64 ? HEAD_MAX_ACC : hp.n_tok <= 128 ? HEAD_MAX_ACC / 2 : 2;
     hp.n_vtile = (int)cdiv(op.V, 2 * BM);
-    hp.n_stage = std::min(HEAD_MAX_STAGES, HEAD_RING_BYTES / (HEAD_KSUB * (A_BYTES + (int)cdiv(hp.n_tok / 2, hp.e_step) * hp.e_step * BK * 2)));
     const int cdt = compute_dtype(&op);
     hp.idesc = make_idesc(cdt == CCE_DT_BF16 ? 1 : 0, 0, 0, 2 * BM, 0);
     hp.status = reinterpret_cast<int*>(ws);
@@ -357,7 +357,7 @@ int cce_b200_logits(const cce_b200_logits_args* a, void* workspace, size_t works
     rc = make_tmap(&maps.c, sg.c, cdt, sg.Dk, op.V, sg.ldc, BK, BM);
     if (rc) return rc;
     for (int i = 0; i < HEAD_E_MAPS; ++i) {
-        if (i > 0 && hp.e_step == hp.n_tok / 2) {
+        if (i > 0 && !pl.sorted) {
             maps.e[i] = maps.e[0];
             continue;
         }

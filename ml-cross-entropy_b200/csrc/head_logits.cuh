@@ -56,7 +56,6 @@ struct HeadParams {
     int n_tok;         // columns (tokens) a tile has room for: a multiple of 16, at most 256
     int n_col;         // columns: T, or with col_token an upper bound of *n_col_dev
     int n_vtile;       // classifier tiles of 256 rows
-    int n_stage;
     int e_step;        // the token maps' boxes have e_step, 2 e_step, .. rows; the smallest that holds half a tile is used
     int n_acc;         // accumulators in TMEM: 512 columns in n_acc parts of at least n_tok
     const int* col_token;  // null (column = token), or [n_col]: the token of every column, -1 for padding
@@ -98,6 +97,25 @@ struct HeadTiles {
         n_tok = ((n_col + n_ntile - 1) / n_ntile + HEAD_GROUP - 1) / HEAD_GROUP * HEAD_GROUP;  // even shares
     }
 };
+
+// The ring of a launch: as many stages as shared memory holds, of HEAD_KSUB sub-blocks of both operands.
+struct HeadRing {
+    int e_size;             // which token map: its boxes have e_size e_step rows
+    uint32_t sub_e, bytes;  // of a sub-block's token operand (this CTA's half of the tile's columns), and of a stage
+    int n_stage;
+    static constexpr uint32_t off_e = HEAD_KSUB * A_BYTES;  // of a stage: the token operand
+    __device__ __forceinline__ HeadRing(const HeadParams& p, const HeadTiles& tiles) {
+        e_size = (tiles.n_tok / 2 + p.e_step - 1) / p.e_step;
+        sub_e = e_size * p.e_step * BK * 2;
+        bytes = off_e + HEAD_KSUB * sub_e;
+        n_stage = min(HEAD_MAX_STAGES, int(HEAD_RING_BYTES / bytes));
+    }
+    // rows of h that a stage of adapters holds per term
+    __device__ __forceinline__ int h_rows() const { return sub_e / (BK * 2); }
+};
+// Classifier stages of its first tile that a CTA brings into L2 while it waits for the kernels that order the columns (they
+// take 15 us, in which HBM could deliver 90 MB: 16 stages are 78 MB)
+constexpr int HEAD_L2_AHEAD = 16;
 
 // Layout of the 16-bit rows of h: rank <= 32 (one 64-element block): hi in columns 0..31, lo in 32..63; above that,
 // for every 64 ranks a block of hi and a block of lo.
@@ -340,10 +358,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HEAD_THREADS, 1)
 head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant__ HeadParams p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    // room for this CTA's half of the tokens x 64 reduction elements
-    const uint32_t sub_e = (p.n_tok / 2 + p.e_step - 1) / p.e_step * p.e_step * BK * 2;
-    const uint32_t off_e = HEAD_KSUB * A_BYTES;   // of a stage: the token operand
-    const uint32_t stage_bytes = off_e + HEAD_KSUB * sub_e;
     HeadSmem s;
     s.stages = base;
     uint64_t* bars = reinterpret_cast<uint64_t*>(base + HEAD_RING_BYTES);
@@ -363,7 +377,7 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
     const int n_pairs = int(gridDim.x >> 1), pair = int(blockIdx.x >> 1);
     const int n_kstage = (p.n_kblk + HEAD_KSUB - 1) / HEAD_KSUB;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < p.n_stage; ++i) {
+        for (int i = 0; i < HEAD_MAX_STAGES; ++i) {
             mbar_init(smem_u32(&s.full[i]), 1);
             mbar_init(smem_u32(&s.empty[i]), 1);
         }
@@ -389,104 +403,97 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(s.tmem_base);
 
     const AdapterPack pack(p.rank);
+    const bool ordered = p.col_token != nullptr;  // the columns come from the kernels before this one
     if (warp == 0) {
-        {
-            int stage = 0;
-            uint32_t phase = 0;
-            auto free_stage = [&]() -> bool {
-                return mbar_wait(smem_u32(&s.empty[stage]), phase ^ 1u, s.abort_flag, p.status, ERR_WAIT_SMEM_EMPTY);
-            };
-            auto next_stage = [&]() {
-                if (++stage == p.n_stage) {
-                    stage = 0;
-                    phase ^= 1u;
-                }
-            };
-            auto sub_blocks = [&](int ks) { return min(HEAD_KSUB, p.n_kblk - ks * HEAD_KSUB); };
-            auto open_stage = [&](uint32_t bytes) {  // announces the bytes of both CTAs
-                if (rank == 0) mbar_expect_tx(smem_u32(&s.full[stage]), 2 * bytes);
-            };
-            auto load_c = [&](int ks, int row) {
-                const uint32_t bar = map_to_cta(smem_u32(&s.full[stage]), 0);
-                const uint32_t sa = smem_u32(s.stages) + stage * stage_bytes;
-                for (int j = 0; j < sub_blocks(ks); ++j)
-                    tma_load_2d_pair(sa + j * A_BYTES, &maps.c, bar, (ks * HEAD_KSUB + j) * BK, row);
-            };
-            auto load_e = [&](int ks, int row, const CUtensorMap* map) {
-                const uint32_t bar = map_to_cta(smem_u32(&s.full[stage]), 0);
-                const uint32_t sb = smem_u32(s.stages) + stage * stage_bytes + off_e;
-                for (int j = 0; j < sub_blocks(ks); ++j)
-                    tma_load_2d_pair(sb + j * sub_e, map, bar, (ks * HEAD_KSUB + j) * BK, row);
-            };
-            // The first tile's classifier rows are known before the columns are, if there is one column tile: a
-            // ring of them is requested before the wait for the kernels that order the columns.
-            int ahead = 0;
-            if (p.lora_b && p.n_col <= p.n_tok && lane == 0) {
-                ahead = min(p.n_stage, n_kstage);
-                for (int ks = 0; ks < ahead; ++ks) {
-                    load_c(ks, pair * 2 * BM + rank * BM);
+        if (ordered) {
+            const int row = pair * 2 * BM + rank * BM;  // of the first tile, if there is one column tile
+            if (lane == 0 && p.n_col <= p.n_tok && row < p.V)
+                for (int kb = 0; kb < min(HEAD_L2_AHEAD * HEAD_KSUB, p.n_kblk); ++kb) tma_prefetch_2d(&maps.c, kb * BK, row);
+            pdl_wait();
+        }
+        const HeadTiles tiles(p);
+        const HeadRing ring(p, tiles);
+        const int n_items = p.n_vtile * tiles.n_ntile;
+        const CUtensorMap* map_e = &maps.e[ring.e_size - 1];
+        int stage = 0;
+        uint32_t phase = 0;
+        auto free_stage = [&]() -> bool {
+            return mbar_wait(smem_u32(&s.empty[stage]), phase ^ 1u, s.abort_flag, p.status, ERR_WAIT_SMEM_EMPTY);
+        };
+        auto next_stage = [&]() {
+            if (++stage == ring.n_stage) {
+                stage = 0;
+                phase ^= 1u;
+            }
+        };
+        auto announce = [&](uint32_t bytes) {  // the bytes of both CTAs
+            if (rank == 0) mbar_expect_tx(smem_u32(&s.full[stage]), 2 * bytes);
+        };
+        bool ok = true, waited = ordered;  // waited: for the kernel that makes h
+        for (int item = pair; item < n_items; item += n_pairs) {
+            const int row_c = (item / tiles.n_ntile) * 2 * BM + rank * BM;
+            const int col0 = (item % tiles.n_ntile) * tiles.n_tok;
+            const int row_e = col0 + rank * (tiles.n_tok / 2);
+            int n_runs = p.lora_b && waited ? find_runs(p, tiles, col0, s.runs) : 0;
+            if (lane == 0) {  // one lane runs the loop over the stages
+                for (int ks = 0; ok && ks < n_kstage; ++ks) {
+                    ok = free_stage();
+                    if (!ok) break;
+                    const int n = min(HEAD_KSUB, p.n_kblk - ks * HEAD_KSUB);
+                    announce(n * (A_BYTES + ring.sub_e));
+                    const uint32_t bar = map_to_cta(smem_u32(&s.full[stage]), 0);
+                    const uint32_t sa = smem_u32(s.stages) + stage * ring.bytes, sb = sa + ring.off_e;
+                    for (int j = 0; j < n; ++j) {
+                        const int x = (ks * HEAD_KSUB + j) * BK;
+                        tma_load_2d_pair(sa + j * A_BYTES, &maps.c, bar, x, row_c);
+                        tma_load_2d_pair(sb + j * ring.sub_e, map_e, bar, x, row_e);
+                    }
                     next_stage();
                 }
-                stage = 0;
-                phase = 0;
             }
-            if (p.lora_b) pdl_wait();
-            const HeadTiles tiles(p);
-            const int n_items = p.n_vtile * tiles.n_ntile;
-            const int size = (tiles.n_tok / 2 + p.e_step - 1) / p.e_step;  // of the token loads, in steps
-            const CUtensorMap* map_e = &maps.e[size - 1];
-            const uint32_t e_bytes = size * p.e_step * BK * 2;
-            bool ok = true;
-            for (int item = pair; item < n_items; item += n_pairs) {
-                const int row_c = (item / tiles.n_ntile) * 2 * BM + rank * BM;
-                const int col0 = (item % tiles.n_ntile) * tiles.n_tok;
-                const int row_e = col0 + rank * (tiles.n_tok / 2);
-                const int n_runs = p.lora_b ? find_runs(p, tiles, col0, s.runs) : 0;
-                if (lane == 0) {  // one lane runs the loop over the stages
-                    for (int ks = 0; ok && ks < n_kstage; ++ks) {
-                        if (ks >= ahead) {
-                            ok = free_stage();
-                            if (!ok) break;
-                        }
-                        open_stage(sub_blocks(ks) * (A_BYTES + e_bytes));
-                        if (ks >= ahead) load_c(ks, row_c);
-                        load_e(ks, row_e, map_e);
+            if (!p.lora_b) continue;  // an abandoned wait ends every later one at once
+            __syncwarp();
+            if (!waited) {
+                pdl_wait();
+                waited = true;
+                n_runs = find_runs(p, tiles, col0, s.runs);
+            }
+            if (lane == 0) {
+                uint32_t bytes = 0;  // announced when the stage is complete: the loads may land before that
+                ok = ok && pack.walk(
+                    s.runs, n_runs, p.rank, ring.h_rows(),
+                    [&]() -> bool {
+                        bytes = 0;
+                        return free_stage();
+                    },
+                    [&](int i, int row, const Run& run, int r0) {
+                        const uint32_t bar = map_to_cta(smem_u32(&s.full[stage]), 0);
+                        const uint32_t sa = smem_u32(s.stages) + stage * ring.bytes, sb = sa + ring.off_e;
+                        const int half = run.cols / 2;  // rows of h that this CTA supplies: a multiple of 8
+                        const int terms = p.rank <= 32 ? 1 : 2;
+                        tma_load_3d_pair(sa + i * pack.a_bytes, &maps.b, bar, r0, row_c, run.adapter);
+                        for (int t = 0; t < terms; ++t)
+                            for (int y = 0; y < half;) {  // few and large loads: each costs its issue
+                                const bool large = half - y >= 32;
+                                tma_load_2d_pair(sb + t * ring.sub_e + (row + y) * BK * 2, large ? &maps.h32 : &maps.h8, bar,
+                                                 r0 * 2 + t * BK, col0 + run.first + rank * half + y);
+                                y += large ? 32 : 8;
+                            }
+                        bytes += pack.a_bytes + terms * half * BK * 2;
+                    },
+                    [&]() {
+                        announce(bytes);
                         next_stage();
-                    }
-                    ahead = 0;
-                    uint32_t bytes = 0;  // announced when the stage is complete: the loads may land before that
-                    ok = ok && pack.walk(
-                        s.runs, n_runs, p.rank, p.n_tok / 2,
-                        [&]() -> bool {
-                            bytes = 0;
-                            return free_stage();
-                        },
-                        [&](int i, int row, const Run& run, int r0) {
-                            const uint32_t bar = map_to_cta(smem_u32(&s.full[stage]), 0);
-                            const uint32_t sa = smem_u32(s.stages) + stage * stage_bytes;
-                            const int half = run.cols / 2;  // rows of h that this CTA supplies: a multiple of 8
-                            const int terms = p.rank <= 32 ? 1 : 2;
-                            tma_load_3d_pair(sa + i * pack.a_bytes, &maps.b, bar, r0, row_c, run.adapter);
-                            for (int t = 0; t < terms; ++t)
-                                for (int y = 0; y < half;) {  // few and large loads: each costs its issue
-                                    const bool large = half - y >= 32;
-                                    tma_load_2d_pair(sa + off_e + t * sub_e + (row + y) * BK * 2,
-                                                     large ? &maps.h32 : &maps.h8, bar, r0 * 2 + t * BK,
-                                                     col0 + run.first + rank * half + y);
-                                    y += large ? 32 : 8;
-                                }
-                            bytes += pack.a_bytes + terms * half * BK * 2;
-                        },
-                        [&]() {
-                            open_stage(bytes);
-                            next_stage();
-                        });
-                }
-                if (!__shfl_sync(0xffffffffu, int(ok), 0)) break;
+                    });
             }
         }
     } else if (warp == 1) {
         if (rank == 0) {
+            if (ordered) pdl_wait();
+            const HeadTiles tiles(p);
+            const HeadRing ring(p, tiles);
+            const int n_items = p.n_vtile * tiles.n_ntile;
+            const uint32_t idesc = p.idesc | (uint32_t(tiles.n_tok >> 3) << 17);
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
             const uint64_t adesc0 = make_smem_desc(smem_u32(s.stages), 16, 1024);
@@ -500,25 +507,31 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
             auto release_stage = [&]() {  // in both CTAs, once the MMAs issued so far have read it
                 tc_commit_pair(empty0 + 8 * stage);
                 tc_commit_pair(empty1 + 8 * stage);
-                if (++stage == p.n_stage) {
+                if (++stage == ring.n_stage) {
                     stage = 0;
                     phase ^= 1u;
                 }
             };
+            auto publish = [&]() {  // the accumulator, to both CTAs' epilogues
+                tc_commit_pair(tfull0 + 8 * acc);
+                tc_commit_pair(tfull1 + 8 * acc);
+                if (++acc == p.n_acc) {
+                    acc = 0;
+                    acc_phase ^= 1u;
+                }
+            };
             constexpr int STEP = UMMA_K * 2 >> 4;  // descriptor units (16 bytes) per MMA step
-            if (p.lora_b) pdl_wait();
-            const HeadTiles tiles(p);
-            const int n_items = p.n_vtile * tiles.n_ntile;
-            const uint32_t idesc = p.idesc | (uint32_t(tiles.n_tok >> 3) << 17);
             Run* runs = s.runs + HEAD_MAX_RUNS;
-            bool ok = true;
+            bool ok = true, waited = ordered;
             for (int item = pair; item < n_items; item += n_pairs) {
-                const int n_runs = p.lora_b ? find_runs(p, tiles, (item % tiles.n_ntile) * tiles.n_tok, runs) : 0;
+                const int col0 = (item % tiles.n_ntile) * tiles.n_tok;
+                int n_runs = p.lora_b && waited ? find_runs(p, tiles, col0, runs) : 0;
+                uint32_t d_tmem = 0;
                 if (lane == 0) {  // one lane issues
-                    uint32_t d_tmem = 0;
                     for (int ks = 0; ok && ks < n_kstage; ++ks) {
-                        const bool opens = SEGMENTED ? ks % HEAD_SEGMENT == 0 : ks == 0, last = ks + 1 == n_kstage;
+                        const bool opens = SEGMENTED ? ks % HEAD_SEGMENT == 0 : ks == 0;
                         if (opens) {
+                            if (SEGMENTED && ks > 0) publish();
                             ok = mbar_wait(smem_u32(&s.tempty[acc]), acc_phase ^ 1u, s.abort_flag, p.status,
                                            ERR_WAIT_TMEM_EMPTY);
                             if (!ok) break;
@@ -527,42 +540,41 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
                         }
                         ok = filled_stage();
                         if (!ok) break;
+                        // the address field of a descriptor counts 16-byte units
+                        const uint64_t ad = adesc0 + ((stage * ring.bytes) >> 4), bd = ad + (ring.off_e >> 4);
                         const int n = min(HEAD_KSUB, p.n_kblk - ks * HEAD_KSUB);
-                        const uint64_t ad = adesc0 + ((stage * stage_bytes) >> 4), bd = ad + (off_e >> 4);
                         for (int j = 0; j < n; ++j)
 #pragma unroll
                             for (int k = 0; k < BK / UMMA_K; ++k)
-                                tc_mma_f16_pair(d_tmem, ad + j * (A_BYTES >> 4) + k * STEP, bd + j * (sub_e >> 4) + k * STEP,
-                                                idesc, (!opens || j || k) ? 1u : 0u);
+                                tc_mma_f16_pair(d_tmem, ad + j * (A_BYTES >> 4) + k * STEP,
+                                                bd + j * (ring.sub_e >> 4) + k * STEP, idesc, (!opens || j || k) ? 1u : 0u);
                         release_stage();
-                        if (last) {
-                            ok = pack.walk(
-                                runs, n_runs, p.rank, p.n_tok / 2, filled_stage,
-                                [&](int i, int row, const Run& run, int r0) {
-                                    const uint32_t run_idesc = p.idesc | (uint32_t(run.cols >> 3) << 17);
-                                    const uint32_t lo = p.rank <= 32 ? 2 * STEP : sub_e >> 4;  // from the hi to the lo terms
-                                    const uint32_t sa = smem_u32(s.stages) + stage * stage_bytes;
-                                    const uint64_t rad = (make_smem_desc(sa + i * pack.a_bytes, 16, pack.sbo) &
-                                                          ~(uint64_t(7) << 61)) | uint64_t(pack.layout) << 61;
-                                    const uint64_t rbd = make_smem_desc(sa + off_e + row * BK * 2, 16, 1024);
-                                    const int steps = (min(BK, p.rank - r0) + UMMA_K - 1) / UMMA_K;
-                                    for (int k = 0; k < steps; ++k) {
-                                        tc_mma_f16_pair(d_tmem + run.first, rad + k * STEP, rbd + k * STEP, run_idesc, 1u);
-                                        tc_mma_f16_pair(d_tmem + run.first, rad + k * STEP, rbd + lo + k * STEP, run_idesc, 1u);
-                                    }
-                                },
-                                release_stage);
-                            if (!ok) break;
-                        }
-                        if (last || (SEGMENTED && (ks + 1) % HEAD_SEGMENT == 0)) {
-                            tc_commit_pair(tfull0 + 8 * acc);
-                            tc_commit_pair(tfull1 + 8 * acc);
-                            if (++acc == p.n_acc) {
-                                acc = 0;
-                                acc_phase ^= 1u;
-                            }
-                        }
                     }
+                }
+                __syncwarp();
+                if (p.lora_b && !waited) {
+                    pdl_wait();
+                    waited = true;
+                    n_runs = find_runs(p, tiles, col0, runs);
+                }
+                if (lane == 0 && ok) {
+                    ok = pack.walk(
+                        runs, n_runs, p.rank, ring.h_rows(), filled_stage,
+                        [&](int i, int row, const Run& run, int r0) {
+                            const uint32_t run_idesc = p.idesc | (uint32_t(run.cols >> 3) << 17);
+                            const uint32_t lo = p.rank <= 32 ? 2 * STEP : ring.sub_e >> 4;  // from the hi to the lo terms
+                            const uint32_t sa = smem_u32(s.stages) + stage * ring.bytes;
+                            const uint64_t rad = (make_smem_desc(sa + i * pack.a_bytes, 16, pack.sbo) & ~(uint64_t(7) << 61)) |
+                                                 uint64_t(pack.layout) << 61;
+                            const uint64_t rbd = make_smem_desc(sa + ring.off_e + row * BK * 2, 16, 1024);
+                            const int steps = (min(BK, p.rank - r0) + UMMA_K - 1) / UMMA_K;
+                            for (int k = 0; k < steps; ++k) {
+                                tc_mma_f16_pair(d_tmem + run.first, rad + k * STEP, rbd + k * STEP, run_idesc, 1u);
+                                tc_mma_f16_pair(d_tmem + run.first, rad + k * STEP, rbd + lo + k * STEP, run_idesc, 1u);
+                            }
+                        },
+                        release_stage);
+                    if (ok) publish();
                 }
                 if (!__shfl_sync(0xffffffffu, int(ok), 0)) break;
             }
