@@ -40,7 +40,9 @@ def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
     if t.dim() != 2:
         t = t.reshape(-1, width)
     s0, s1 = t.stride()
-    if (s1 != 1 and width != 1) or (t.size(0) > 1 and s0 < width):
+    if width == 1 and s1 != 1:  # the stride of one column says nothing
+        t, s1 = t.reshape(-1).unsqueeze(1), 1
+    if s1 != 1 or (t.size(0) > 1 and s0 < width):
         t = t.contiguous()
     return t
 

@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from cut_cross_entropy import _native, linear_logits, linear_sample, sample_tokens
+from cut_cross_entropy.linear_logits import _rows
 from oracle import head_oracle as H
 
 
@@ -71,6 +72,14 @@ def test_sample_tokens_refusals(kw, err):
     args.update(kw)
     with pytest.raises(err):
         sample_tokens(**args)
+
+
+def test_rows_of_one_column_have_unit_stride():
+    wide = torch.arange(12.0).reshape(3, 4)
+    for t in (wide[:1].t(), wide.t()[:, 1:2], wide[:, 2:3], wide[:1, :1], torch.zeros(1).expand(5, 1)):
+        rows = _rows(t, 1)
+        assert rows.stride(1) == 1 and (rows.size(0) == 1 or rows.stride(0) >= 1)
+        assert torch.equal(rows, t)
 
 
 def test_linear_sample_refuses_a_u_of_another_shape():
