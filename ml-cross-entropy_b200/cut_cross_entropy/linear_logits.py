@@ -17,10 +17,10 @@ from .linear_cross_entropy import _reject_dtensors
 MAX_RANK = 256  # CCE_B200_MAX_RANK
 
 
-def _check_no_grad(name: str, *tensors: torch.Tensor | None) -> None:
+def _check_no_grad(name: str, *tensors: torch.Tensor | float | None) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
-            if t is not None and t.requires_grad:
+            if isinstance(t, torch.Tensor) and t.requires_grad:
                 raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or torch.inference_mode().")
 
 
@@ -81,7 +81,7 @@ def linear_logits(
     """
     if type(e) is not torch.Tensor or type(c) is not torch.Tensor:  # plain tensors are no DTensors
         _reject_dtensors(e=e, c=c, bias=bias, lora_a=lora_a, lora_b=lora_b, adapter_ids=adapter_ids)
-    _check_no_grad("linear_logits", e, c, bias, lora_a, lora_b)
+    _check_no_grad("linear_logits", e, c, bias, lora_a, lora_b, lora_scale)
     if e.dim() < 1 or c.dim() != 2 or e.size(-1) != c.size(1):
         raise ValueError(f"Expected e (..., D) and c (V, D), got {tuple(e.shape)} and {tuple(c.shape)}.")
     if bias is not None and bias.shape != c.shape[:1]:

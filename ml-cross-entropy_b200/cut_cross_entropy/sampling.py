@@ -65,7 +65,7 @@ def sample_tokens(
     """
     if type(logits) is not torch.Tensor or type(u) is not torch.Tensor:  # plain tensors are no DTensors
         _reject_dtensors(logits=logits, u=u)
-    _check_no_grad("sample_tokens", logits)
+    _check_no_grad("sample_tokens", logits, u, temperature, top_p, min_p)
     batch_shape = u.shape
     if logits.dim() < 1 or batch_shape != logits.shape[:-1]:
         raise ValueError(f"Expected logits (..., V) and u (...), got {tuple(logits.shape)} and {tuple(u.shape)}.")

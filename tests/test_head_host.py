@@ -74,6 +74,20 @@ def test_sample_tokens_refusals(kw, err):
         sample_tokens(**args)
 
 
+@pytest.mark.parametrize("name", ["u", "temperature", "top_p", "min_p"])
+def test_sample_tokens_refuses_settings_that_want_a_gradient(name):
+    args = dict(logits=torch.zeros(4, 7), u=torch.zeros(4))
+    args[name] = torch.full((4,), 0.5, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no backward"):
+        sample_tokens(**args)
+
+
+def test_linear_logits_refuses_a_scale_that_wants_a_gradient():
+    args = dict(e=torch.zeros(4, 16), c=torch.zeros(10, 16), **_lora())
+    with pytest.raises(RuntimeError, match="no backward"):
+        linear_logits(**args, lora_scale=torch.ones(args["lora_a"].size(0), requires_grad=True))
+
+
 def test_rows_of_one_column_have_unit_stride():
     wide = torch.arange(12.0).reshape(3, 4)
     for t in (wide[:1].t(), wide.t()[:, 1:2], wide[:, 2:3], wide[:1, :1], torch.zeros(1).expand(5, 1)):
