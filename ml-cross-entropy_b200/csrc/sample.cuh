@@ -296,7 +296,8 @@ struct RowBase {
     __device__ __forceinline__ void prepare(float m) {
         mx = m + 0.0f;
         const double min_p = p.min_p ? double(p.min_p[row]) : p.min_p_all;
-        const double k2 = 1.4426950408889634074 / temp;  // exponents of 2 per unit of logit
+        // exponents of 2 per unit of logit; finite, for infinity x 0 would be the largest logit's exponent
+        const double k2 = 1.4426950408889634074 / fmax(temp, 1e-300);
         weight.scale = SMP_TABLE * k2;
         set_weight();
         l_floor = l_min = lowest_with(SMP_FLOOR_LOG2, k2);

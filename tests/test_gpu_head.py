@@ -352,13 +352,14 @@ def test_sample_border_numbers():
         assert torch.equal(sample_tokens(x, torch.full((6,), u, device=DEV), top_k=3), first)
 
 
-@pytest.mark.parametrize("T", [1e-30, 1e-3, 1e4, 1e30, math.inf])
+@pytest.mark.parametrize("T", [5e-324, 1e-310, 1e-30, 1e-3, 1e4, 1e30, 1e308, math.inf])
 @pytest.mark.parametrize("kw", [dict(), dict(top_k=77), dict(top_p=0.7), dict(top_k=999, top_p=0.3, min_p=0.5)])
 def test_sample_extreme_temperatures(T, kw):
     x, u = _rows(4, 12345, FP32, seed=9)
     x[2, ::3] = -math.inf
     x[3, ::3] = torch.finfo(FP32).min
     _check_sample(x, u, temperature=T, **kw)
+    _check_sample(torch.full((4, 5000), 2.5, device=DEV), u, temperature=T, **kw)  # nothing but the largest
 
 
 def test_sample_every_row_has_its_own_settings():
