@@ -347,8 +347,10 @@ row_pass_kernel(const SampleParams p, const StreamBuffers b) {
         const long long block = (long long)chunk * STR_BLOCKS + i;
         u64 kept = 0;
         if (rs.holds(block)) {
+            // The plan counted at most SMP_LIST of them; the bound is for logits that are written while the kernels run.
             auto collect = [&](float l, long long pos) {
-                local[atomicAdd(&n_local, 1u)] = r.rank_key(l, pos - rs.phase);
+                const uint32_t at = atomicAdd(&n_local, 1u);
+                if (at < SMP_LIST) local[at] = r.rank_key(l, pos - rs.phase);
             };
             if (st.mode == ROW_LIST) {
                 rs.each(block, r.lane, [&](float l, long long pos) {
@@ -379,7 +381,7 @@ row_pass_kernel(const SampleParams p, const StreamBuffers b) {
         base = n_local ? atomicAdd(&b.state[row].n_list, n_local) : 0;
     }
     __syncthreads();
-    for (uint32_t i = r.tid; i < n_local; i += SMP_THREADS) b.list[row * SMP_LIST + base + i] = local[i];
+    for (uint32_t i = r.tid; i < n_local && base + i < SMP_LIST; i += SMP_THREADS) b.list[row * SMP_LIST + base + i] = local[i];
 }
 
 // One CTA per row.  Dynamic shared memory: three lists of SMP_LIST keys, then the blocks' masses.
