@@ -44,10 +44,16 @@ __global__ void pack_rows_kernel(const uint16_t* __restrict__ src, long long ld_
         const uint4* s4 = reinterpret_cast<const uint4*>(s);
         uint4* d4 = reinterpret_cast<uint4*>(d);
         for (long long j = threadIdx.x; j < D / 8; j += blockDim.x) d4[j] = s4[j];
-    } else {
-        for (long long j = threadIdx.x; j < D; j += blockDim.x) d[j] = s[j];
+        for (long long j = D + threadIdx.x; j < Dp; j += blockDim.x) d[j] = 0;
+    } else {  // Dp is a multiple of 8: eight loads in flight per thread, one store
+        for (long long j = threadIdx.x * 8; j < Dp; j += blockDim.x * 8) {
+            uint4 w;
+            uint16_t* x = reinterpret_cast<uint16_t*>(&w);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) x[q] = j + q < D ? s[j + q] : uint16_t(0);
+            *reinterpret_cast<uint4*>(d + j) = w;
+        }
     }
-    for (long long j = D + threadIdx.x; j < Dp; j += blockDim.x) d[j] = 0;
 }
 
 // fp32 operands run on the bf16 tensor path as a three-term split: x = hi + lo with hi = bf16(x),
