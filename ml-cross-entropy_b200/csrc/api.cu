@@ -99,7 +99,8 @@ bool pair_enabled() {
 
 template <typename T>
 cudaError_t head_logits_attributes() {
-    for (auto* k : {head_logits_kernel<T, 0>, head_logits_kernel<T, 1>, head_logits_kernel<T, 2>, head_logits_kernel<T, 3>}) {
+    for (auto* k : {head_logits_kernel<T, 0>, head_logits_kernel<T, 1>, head_logits_kernel<T, 2>, head_logits_kernel<T, 3>,
+                    head_logits_kernel<T, 4>}) {
         const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, HEAD_SMEM);
         if (e != cudaSuccess) return e;
     }

@@ -111,7 +111,8 @@ int launch_head(const HeadMaps& maps, const HeadParams& hp, int grid, cudaStream
     const auto kernel = !head_segmented(hp) ? head_logits_kernel<T, 0>
                         : hp.n_tok <= 64    ? head_logits_kernel<T, 1>
                         : hp.n_tok <= 128   ? head_logits_kernel<T, 2>
-                                            : head_logits_kernel<T, 3>;
+                        : hp.n_tok <= 192   ? head_logits_kernel<T, 3>
+                                            : head_logits_kernel<T, 4>;
     return launch_behind(kernel, dim3(grid), HEAD_THREADS, HEAD_SMEM, st, hp.lora_b != nullptr, maps, hp);
 }
 
@@ -325,11 +326,10 @@ int cce_b200_logits(const cce_b200_logits_args* a, void* workspace, size_t works
     hp.col_token = col_token;
     hp.n_col_dev = n_col_dev;
     hp.out_dtype = a->out_dtype;
-    // A tile of 192 columns is what the registers of the segmented form hold.  Columns that only the device can
-    // count may be far fewer than the bound: there a tile has room for as many as possible.
-    const long long room = head_segmented(hp) ? 192 : BN;
-    const long long n_ntile = cdiv(pl.n_col, room);
-    hp.n_tok = n_ntile > 1 && pl.sorted ? (int)room : (int)(cdiv(cdiv(pl.n_col, n_ntile), HEAD_GROUP) * HEAD_GROUP);
+    // Columns that only the device can count may be far fewer than the bound: there a tile has room for as many as
+    // possible.
+    const long long n_ntile = cdiv(pl.n_col, BN);
+    hp.n_tok = n_ntile > 1 && pl.sorted ? BN : (int)(cdiv(cdiv(pl.n_col, n_ntile), HEAD_GROUP) * HEAD_GROUP);
     // where the device counts the columns, four sizes of token loads, in whole groups of 8 rows
     hp.e_step = pl.sorted ? (int)(cdiv(cdiv(hp.n_tok / 2, HEAD_E_MAPS), 8) * 8) : hp.n_tok / 2;
     hp.n_acc = hp.n_tok <= 64 ? HEAD_MAX_ACC : hp.n_tok <= 128 ? HEAD_MAX_ACC / 2 : 2;

@@ -614,11 +614,15 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
                     for (int c = 0; c < CHUNKS; ++c) {
                         const int col = half * 32 + c * 64;
                         if (col0 + col < col_end && ok) {  // uniform over the warp
-                            uint32_t r[32];
-                            tmem_ld32(taddr + col, r);
-                            tmem_ld_wait();
+                            constexpr int W = CHUNKS > 3 ? 16 : 32;  // the sums leave few registers
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) sum[c][j] += __uint_as_float(r[j]);
+                            for (int j0 = 0; j0 < 32; j0 += W) {
+                                uint32_t r[W];
+                                if constexpr (W == 16) tmem_ld16(taddr + col + j0, r); else tmem_ld32(taddr + col + j0, r);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int j = 0; j < W; ++j) sum[c][j0 + j] += __uint_as_float(r[j]);
+                            }
                         }
                     }
                 } else {
