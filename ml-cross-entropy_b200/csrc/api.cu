@@ -101,7 +101,11 @@ template <typename T>
 cudaError_t head_logits_attributes() {
     for (auto* k : {head_logits_kernel<T, 0>, head_logits_kernel<T, 1>, head_logits_kernel<T, 2>, head_logits_kernel<T, 3>,
                     head_logits_kernel<T, 4>}) {
-        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, HEAD_SMEM);
+        cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, HEAD_SMEM);
+        cudaFuncAttributes attr;
+        if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, k);
+        // the split of the registers hands out what the block was launched with: with fewer it would wait for good
+        if (e == cudaSuccess && attr.numRegs != HEAD_REGS) e = cudaErrorInvalidKernelImage;
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;

@@ -13,7 +13,7 @@
 //
 //   warp 0      : TMA producer of both CTAs (128-byte swizzled ring; as many stages as shared memory holds)
 //   warp 1      : tcgen05.mma issuer (leader CTA), owner of the TMEM (2 accumulators of 128 x 256 fp32 per CTA)
-//   warps 2..9  : epilogue; warp w reads TMEM lanes 32*(w%4)..+31, two warps share a quarter
+//   warps 4..11 : epilogue; warp w reads TMEM lanes 32*(w%4)..+31, two warps share a quarter
 //
 // The adapters' second product.  The accumulator's columns are looked at in groups of 16.  A group whose tokens
 // all use one adapter (or none) takes it on the tensor cores, as further reduction blocks of the same columns: A
@@ -35,7 +35,13 @@
 namespace cce {
 
 constexpr int HEAD_EPI_WARPS = 8;
-constexpr int HEAD_THREADS = 64 + 32 * HEAD_EPI_WARPS;
+constexpr int HEAD_EPI_FIRST = 4;              // the epilogue's first warp: registers are handed out by groups of 4
+constexpr int HEAD_THREADS = 32 * (HEAD_EPI_FIRST + HEAD_EPI_WARPS);
+constexpr int HEAD_REGS = 168;                 // per thread at launch: 65536 / 384, in steps of 8
+// wide tiles of fp32 logits: of the others, and of the epilogue, whose running sums then do not spill
+constexpr int HEAD_REGS_FEW = 72, HEAD_REGS_MANY = 216;
+static_assert(HEAD_EPI_FIRST * HEAD_REGS_FEW + HEAD_EPI_WARPS * HEAD_REGS_MANY <= (HEAD_EPI_FIRST + HEAD_EPI_WARPS) * HEAD_REGS,
+              "no more registers than the block was launched with");
 constexpr int HEAD_KSUB = 2;                   // 64-element K sub-blocks per ring stage
 constexpr int HEAD_MAX_STAGES = 8;
 constexpr int HEAD_SMEM = 227 * 1024;          // everything: the ring decides how many bytes are in flight
@@ -404,184 +410,188 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
 
     const AdapterPack pack(p.rank);
     const bool ordered = p.col_token != nullptr;  // the columns come from the kernels before this one
-    if (warp == 0) {
-        if (ordered) {
-            const int row = pair * 2 * BM + rank * BM;  // of the first tile, if there is one column tile
-            if (lane == 0 && p.n_col <= p.n_tok && row < p.V)
-                for (int kb = 0; kb < min(HEAD_L2_AHEAD * HEAD_KSUB, p.n_kblk); ++kb) tma_prefetch_2d(&maps.c, kb * BK, row);
-            pdl_wait();
-        }
-        const HeadTiles tiles(p);
-        const HeadRing ring(p, tiles);
-        const int n_items = p.n_vtile * tiles.n_ntile;
-        const CUtensorMap* map_e = &maps.e[ring.e_size - 1];
-        int stage = 0;
-        uint32_t phase = 0;
-        auto free_stage = [&]() -> bool {
-            return mbar_wait(smem_u32(&s.empty[stage]), phase ^ 1u, s.abort_flag, p.status, ERR_WAIT_SMEM_EMPTY);
-        };
-        auto next_stage = [&]() {
-            if (++stage == ring.n_stage) {
-                stage = 0;
-                phase ^= 1u;
-            }
-        };
-        auto announce = [&](uint32_t bytes) {  // the bytes of both CTAs
-            if (rank == 0) mbar_expect_tx(smem_u32(&s.full[stage]), 2 * bytes);
-        };
-        bool ok = true, waited = ordered;  // waited: for the kernel that makes h
-        for (int item = pair; item < n_items; item += n_pairs) {
-            const int row_c = (item / tiles.n_ntile) * 2 * BM + rank * BM;
-            const int col0 = (item % tiles.n_ntile) * tiles.n_tok;
-            const int row_e = col0 + rank * (tiles.n_tok / 2);
-            int n_runs = p.lora_b && waited ? find_runs(p, tiles, col0, s.runs) : 0;
-            if (lane == 0) {  // one lane runs the loop over the stages
-                for (int ks = 0; ok && ks < n_kstage; ++ks) {
-                    ok = free_stage();
-                    if (!ok) break;
-                    const int n = min(HEAD_KSUB, p.n_kblk - ks * HEAD_KSUB);
-                    announce(n * (A_BYTES + ring.sub_e));
-                    const uint32_t bar = map_to_cta(smem_u32(&s.full[stage]), 0);
-                    const uint32_t sa = smem_u32(s.stages) + stage * ring.bytes, sb = sa + ring.off_e;
-                    for (int j = 0; j < n; ++j) {
-                        const int x = (ks * HEAD_KSUB + j) * BK;
-                        tma_load_2d_pair(sa + j * A_BYTES, &maps.c, bar, x, row_c);
-                        tma_load_2d_pair(sb + j * ring.sub_e, map_e, bar, x, row_e);
-                    }
-                    next_stage();
-                }
-            }
-            if (!p.lora_b) continue;  // an abandoned wait ends every later one at once
-            __syncwarp();
-            if (!waited) {
+    if (warp < HEAD_EPI_FIRST) {
+        if constexpr (CHUNKS > 2) set_max_regs_down<HEAD_REGS_FEW>();
+        if (warp == 0) {
+            if (ordered) {
+                const int row = pair * 2 * BM + rank * BM;  // of the first tile, if there is one column tile
+                if (lane == 0 && p.n_col <= p.n_tok && row < p.V)
+                    for (int kb = 0; kb < min(HEAD_L2_AHEAD * HEAD_KSUB, p.n_kblk); ++kb) tma_prefetch_2d(&maps.c, kb * BK, row);
                 pdl_wait();
-                waited = true;
-                n_runs = find_runs(p, tiles, col0, s.runs);
             }
-            if (lane == 0) {
-                uint32_t bytes = 0;  // announced when the stage is complete: the loads may land before that
-                ok = ok && pack.walk(
-                    s.runs, n_runs, p.rank, ring.h_rows(),
-                    [&]() -> bool {
-                        bytes = 0;
-                        return free_stage();
-                    },
-                    [&](int i, int row, const Run& run, int r0) {
-                        const uint32_t bar = map_to_cta(smem_u32(&s.full[stage]), 0);
-                        const uint32_t sa = smem_u32(s.stages) + stage * ring.bytes, sb = sa + ring.off_e;
-                        const int half = run.cols / 2;  // rows of h that this CTA supplies: a multiple of 8
-                        const int terms = p.rank <= 32 ? 1 : 2;
-                        tma_load_3d_pair(sa + i * pack.a_bytes, &maps.b, bar, r0, row_c, run.adapter);
-                        for (int t = 0; t < terms; ++t)
-                            for (int y = 0; y < half;) {  // few and large loads: each costs its issue
-                                const bool large = half - y >= 32;
-                                tma_load_2d_pair(sb + t * ring.sub_e + (row + y) * BK * 2, large ? &maps.h32 : &maps.h8, bar,
-                                                 r0 * 2 + t * BK, col0 + run.first + rank * half + y);
-                                y += large ? 32 : 8;
-                            }
-                        bytes += pack.a_bytes + terms * half * BK * 2;
-                    },
-                    [&]() {
-                        announce(bytes);
-                        next_stage();
-                    });
-            }
-        }
-    } else if (warp == 1) {
-        if (rank == 0) {
-            if (ordered) pdl_wait();
             const HeadTiles tiles(p);
             const HeadRing ring(p, tiles);
             const int n_items = p.n_vtile * tiles.n_ntile;
-            const uint32_t idesc = p.idesc | (uint32_t(tiles.n_tok >> 3) << 17);
-            int stage = 0, acc = 0;
-            uint32_t phase = 0, acc_phase = 0;
-            const uint64_t adesc0 = make_smem_desc(smem_u32(s.stages), 16, 1024);
-            const uint32_t empty0 = smem_u32(s.empty), empty1 = map_to_cta(empty0, 1);
-            const uint32_t tfull0 = smem_u32(s.tfull), tfull1 = map_to_cta(tfull0, 1);
-            auto filled_stage = [&]() -> bool {
-                if (!mbar_wait(smem_u32(&s.full[stage]), phase, s.abort_flag, p.status, ERR_WAIT_SMEM_FULL)) return false;
-                tc_fence_after();
-                return true;
+            const CUtensorMap* map_e = &maps.e[ring.e_size - 1];
+            int stage = 0;
+            uint32_t phase = 0;
+            auto free_stage = [&]() -> bool {
+                return mbar_wait(smem_u32(&s.empty[stage]), phase ^ 1u, s.abort_flag, p.status, ERR_WAIT_SMEM_EMPTY);
             };
-            auto release_stage = [&]() {  // in both CTAs, once the MMAs issued so far have read it
-                tc_commit_pair(empty0 + 8 * stage);
-                tc_commit_pair(empty1 + 8 * stage);
+            auto next_stage = [&]() {
                 if (++stage == ring.n_stage) {
                     stage = 0;
                     phase ^= 1u;
                 }
             };
-            auto publish = [&]() {  // the accumulator, to both CTAs' epilogues
-                tc_commit_pair(tfull0 + 8 * acc);
-                tc_commit_pair(tfull1 + 8 * acc);
-                if (++acc == p.n_acc) {
-                    acc = 0;
-                    acc_phase ^= 1u;
-                }
+            auto announce = [&](uint32_t bytes) {  // the bytes of both CTAs
+                if (rank == 0) mbar_expect_tx(smem_u32(&s.full[stage]), 2 * bytes);
             };
-            constexpr int STEP = UMMA_K * 2 >> 4;  // descriptor units (16 bytes) per MMA step
-            Run* runs = s.runs + HEAD_MAX_RUNS;
-            bool ok = true, waited = ordered;
+            bool ok = true, waited = ordered;  // waited: for the kernel that makes h
             for (int item = pair; item < n_items; item += n_pairs) {
+                const int row_c = (item / tiles.n_ntile) * 2 * BM + rank * BM;
                 const int col0 = (item % tiles.n_ntile) * tiles.n_tok;
-                int n_runs = p.lora_b && waited ? find_runs(p, tiles, col0, runs) : 0;
-                uint32_t d_tmem = 0;
-                if (lane == 0) {  // one lane issues
+                const int row_e = col0 + rank * (tiles.n_tok / 2);
+                int n_runs = p.lora_b && waited ? find_runs(p, tiles, col0, s.runs) : 0;
+                if (lane == 0) {  // one lane runs the loop over the stages
                     for (int ks = 0; ok && ks < n_kstage; ++ks) {
-                        const bool opens = SEGMENTED ? ks % HEAD_SEGMENT == 0 : ks == 0;
-                        if (opens) {
-                            if (SEGMENTED && ks > 0) publish();
-                            ok = mbar_wait(smem_u32(&s.tempty[acc]), acc_phase ^ 1u, s.abort_flag, p.status,
-                                           ERR_WAIT_TMEM_EMPTY);
-                            if (!ok) break;
-                            tc_fence_after();
-                            d_tmem = tmem_base + acc * acc_cols;
-                        }
-                        ok = filled_stage();
+                        ok = free_stage();
                         if (!ok) break;
-                        // the address field of a descriptor counts 16-byte units
-                        const uint64_t ad = adesc0 + ((stage * ring.bytes) >> 4), bd = ad + (ring.off_e >> 4);
                         const int n = min(HEAD_KSUB, p.n_kblk - ks * HEAD_KSUB);
-                        for (int j = 0; j < n; ++j)
-#pragma unroll
-                            for (int k = 0; k < BK / UMMA_K; ++k)
-                                tc_mma_f16_pair(d_tmem, ad + j * (A_BYTES >> 4) + k * STEP,
-                                                bd + j * (ring.sub_e >> 4) + k * STEP, idesc, (!opens || j || k) ? 1u : 0u);
-                        release_stage();
+                        announce(n * (A_BYTES + ring.sub_e));
+                        const uint32_t bar = map_to_cta(smem_u32(&s.full[stage]), 0);
+                        const uint32_t sa = smem_u32(s.stages) + stage * ring.bytes, sb = sa + ring.off_e;
+                        for (int j = 0; j < n; ++j) {
+                            const int x = (ks * HEAD_KSUB + j) * BK;
+                            tma_load_2d_pair(sa + j * A_BYTES, &maps.c, bar, x, row_c);
+                            tma_load_2d_pair(sb + j * ring.sub_e, map_e, bar, x, row_e);
+                        }
+                        next_stage();
                     }
                 }
+                if (!p.lora_b) continue;  // an abandoned wait ends every later one at once
                 __syncwarp();
-                if (p.lora_b && !waited) {
+                if (!waited) {
                     pdl_wait();
                     waited = true;
-                    n_runs = find_runs(p, tiles, col0, runs);
+                    n_runs = find_runs(p, tiles, col0, s.runs);
                 }
-                if (lane == 0 && ok) {
-                    ok = pack.walk(
-                        runs, n_runs, p.rank, ring.h_rows(), filled_stage,
-                        [&](int i, int row, const Run& run, int r0) {
-                            const uint32_t run_idesc = p.idesc | (uint32_t(run.cols >> 3) << 17);
-                            const uint32_t lo = p.rank <= 32 ? 2 * STEP : ring.sub_e >> 4;  // from the hi to the lo terms
-                            const uint32_t sa = smem_u32(s.stages) + stage * ring.bytes;
-                            const uint64_t rad = (make_smem_desc(sa + i * pack.a_bytes, 16, pack.sbo) & ~(uint64_t(7) << 61)) |
-                                                 uint64_t(pack.layout) << 61;
-                            const uint64_t rbd = make_smem_desc(sa + ring.off_e + row * BK * 2, 16, 1024);
-                            const int steps = (min(BK, p.rank - r0) + UMMA_K - 1) / UMMA_K;
-                            for (int k = 0; k < steps; ++k) {
-                                tc_mma_f16_pair(d_tmem + run.first, rad + k * STEP, rbd + k * STEP, run_idesc, 1u);
-                                tc_mma_f16_pair(d_tmem + run.first, rad + k * STEP, rbd + lo + k * STEP, run_idesc, 1u);
-                            }
+                if (lane == 0) {
+                    uint32_t bytes = 0;  // announced when the stage is complete: the loads may land before that
+                    ok = ok && pack.walk(
+                        s.runs, n_runs, p.rank, ring.h_rows(),
+                        [&]() -> bool {
+                            bytes = 0;
+                            return free_stage();
                         },
-                        release_stage);
-                    if (ok) publish();
+                        [&](int i, int row, const Run& run, int r0) {
+                            const uint32_t bar = map_to_cta(smem_u32(&s.full[stage]), 0);
+                            const uint32_t sa = smem_u32(s.stages) + stage * ring.bytes, sb = sa + ring.off_e;
+                            const int half = run.cols / 2;  // rows of h that this CTA supplies: a multiple of 8
+                            const int terms = p.rank <= 32 ? 1 : 2;
+                            tma_load_3d_pair(sa + i * pack.a_bytes, &maps.b, bar, r0, row_c, run.adapter);
+                            for (int t = 0; t < terms; ++t)
+                                for (int y = 0; y < half;) {  // few and large loads: each costs its issue
+                                    const bool large = half - y >= 32;
+                                    tma_load_2d_pair(sb + t * ring.sub_e + (row + y) * BK * 2, large ? &maps.h32 : &maps.h8, bar,
+                                                     r0 * 2 + t * BK, col0 + run.first + rank * half + y);
+                                    y += large ? 32 : 8;
+                                }
+                            bytes += pack.a_bytes + terms * half * BK * 2;
+                        },
+                        [&]() {
+                            announce(bytes);
+                            next_stage();
+                        });
                 }
-                if (!__shfl_sync(0xffffffffu, int(ok), 0)) break;
+            }
+        } else if (warp == 1) {
+            if (rank == 0) {
+                if (ordered) pdl_wait();
+                const HeadTiles tiles(p);
+                const HeadRing ring(p, tiles);
+                const int n_items = p.n_vtile * tiles.n_ntile;
+                const uint32_t idesc = p.idesc | (uint32_t(tiles.n_tok >> 3) << 17);
+                int stage = 0, acc = 0;
+                uint32_t phase = 0, acc_phase = 0;
+                const uint64_t adesc0 = make_smem_desc(smem_u32(s.stages), 16, 1024);
+                const uint32_t empty0 = smem_u32(s.empty), empty1 = map_to_cta(empty0, 1);
+                const uint32_t tfull0 = smem_u32(s.tfull), tfull1 = map_to_cta(tfull0, 1);
+                auto filled_stage = [&]() -> bool {
+                    if (!mbar_wait(smem_u32(&s.full[stage]), phase, s.abort_flag, p.status, ERR_WAIT_SMEM_FULL)) return false;
+                    tc_fence_after();
+                    return true;
+                };
+                auto release_stage = [&]() {  // in both CTAs, once the MMAs issued so far have read it
+                    tc_commit_pair(empty0 + 8 * stage);
+                    tc_commit_pair(empty1 + 8 * stage);
+                    if (++stage == ring.n_stage) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                };
+                auto publish = [&]() {  // the accumulator, to both CTAs' epilogues
+                    tc_commit_pair(tfull0 + 8 * acc);
+                    tc_commit_pair(tfull1 + 8 * acc);
+                    if (++acc == p.n_acc) {
+                        acc = 0;
+                        acc_phase ^= 1u;
+                    }
+                };
+                constexpr int STEP = UMMA_K * 2 >> 4;  // descriptor units (16 bytes) per MMA step
+                Run* runs = s.runs + HEAD_MAX_RUNS;
+                bool ok = true, waited = ordered;
+                for (int item = pair; item < n_items; item += n_pairs) {
+                    const int col0 = (item % tiles.n_ntile) * tiles.n_tok;
+                    int n_runs = p.lora_b && waited ? find_runs(p, tiles, col0, runs) : 0;
+                    uint32_t d_tmem = 0;
+                    if (lane == 0) {  // one lane issues
+                        for (int ks = 0; ok && ks < n_kstage; ++ks) {
+                            const bool opens = SEGMENTED ? ks % HEAD_SEGMENT == 0 : ks == 0;
+                            if (opens) {
+                                if (SEGMENTED && ks > 0) publish();
+                                ok = mbar_wait(smem_u32(&s.tempty[acc]), acc_phase ^ 1u, s.abort_flag, p.status,
+                                               ERR_WAIT_TMEM_EMPTY);
+                                if (!ok) break;
+                                tc_fence_after();
+                                d_tmem = tmem_base + acc * acc_cols;
+                            }
+                            ok = filled_stage();
+                            if (!ok) break;
+                            // the address field of a descriptor counts 16-byte units
+                            const uint64_t ad = adesc0 + ((stage * ring.bytes) >> 4), bd = ad + (ring.off_e >> 4);
+                            const int n = min(HEAD_KSUB, p.n_kblk - ks * HEAD_KSUB);
+                            for (int j = 0; j < n; ++j)
+    #pragma unroll
+                                for (int k = 0; k < BK / UMMA_K; ++k)
+                                    tc_mma_f16_pair(d_tmem, ad + j * (A_BYTES >> 4) + k * STEP,
+                                                    bd + j * (ring.sub_e >> 4) + k * STEP, idesc, (!opens || j || k) ? 1u : 0u);
+                            release_stage();
+                        }
+                    }
+                    __syncwarp();
+                    if (p.lora_b && !waited) {
+                        pdl_wait();
+                        waited = true;
+                        n_runs = find_runs(p, tiles, col0, runs);
+                    }
+                    if (lane == 0 && ok) {
+                        ok = pack.walk(
+                            runs, n_runs, p.rank, ring.h_rows(), filled_stage,
+                            [&](int i, int row, const Run& run, int r0) {
+                                const uint32_t run_idesc = p.idesc | (uint32_t(run.cols >> 3) << 17);
+                                const uint32_t lo = p.rank <= 32 ? 2 * STEP : ring.sub_e >> 4;  // from the hi to the lo terms
+                                const uint32_t sa = smem_u32(s.stages) + stage * ring.bytes;
+                                const uint64_t rad = (make_smem_desc(sa + i * pack.a_bytes, 16, pack.sbo) & ~(uint64_t(7) << 61)) |
+                                                     uint64_t(pack.layout) << 61;
+                                const uint64_t rbd = make_smem_desc(sa + ring.off_e + row * BK * 2, 16, 1024);
+                                const int steps = (min(BK, p.rank - r0) + UMMA_K - 1) / UMMA_K;
+                                for (int k = 0; k < steps; ++k) {
+                                    tc_mma_f16_pair(d_tmem + run.first, rad + k * STEP, rbd + k * STEP, run_idesc, 1u);
+                                    tc_mma_f16_pair(d_tmem + run.first, rad + k * STEP, rbd + lo + k * STEP, run_idesc, 1u);
+                                }
+                            },
+                            release_stage);
+                        if (ok) publish();
+                    }
+                    if (!__shfl_sync(0xffffffffu, int(ok), 0)) break;
+                }
             }
         }
     } else {
+        if constexpr (CHUNKS > 2) set_max_regs_up<HEAD_REGS_MANY>();
         const int q = warp & 3;              // TMEM lane quarter this warp may read
-        const int half = (warp - 2) >> 2;    // the quarter's two warps take alternate chunks of 32 columns
+        const int half = (warp - HEAD_EPI_FIRST) >> 2;    // the quarter's two warps take alternate chunks of 32 columns
         const uint32_t tempty0 = map_to_cta(smem_u32(s.tempty), 0);
         int acc = 0;
         uint32_t acc_phase = 0;
