@@ -415,7 +415,7 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
         if (warp == 0) {
             if (ordered) {
                 const int row = pair * 2 * BM + rank * BM;  // of the first tile, if there is one column tile
-                if (lane == 0 && p.n_col <= p.n_tok && row < p.V)
+                if (p.n_col <= p.n_tok && row < p.V && elect_one())
                     for (int kb = 0; kb < min(HEAD_L2_AHEAD * HEAD_KSUB, p.n_kblk); ++kb) tma_prefetch_2d(&maps.c, kb * BK, row);
                 pdl_wait();
             }
@@ -443,7 +443,7 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
                 const int col0 = (item % tiles.n_ntile) * tiles.n_tok;
                 const int row_e = col0 + rank * (tiles.n_tok / 2);
                 int n_runs = p.lora_b && waited ? find_runs(p, tiles, col0, s.runs) : 0;
-                if (lane == 0) {  // one lane runs the loop over the stages
+                if (elect_one()) {  // one lane runs the loop over the stages
                     for (int ks = 0; ok && ks < n_kstage; ++ks) {
                         ok = free_stage();
                         if (!ok) break;
@@ -466,7 +466,7 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
                     waited = true;
                     n_runs = find_runs(p, tiles, col0, s.runs);
                 }
-                if (lane == 0) {
+                if (elect_one()) {
                     uint32_t bytes = 0;  // announced when the stage is complete: the loads may land before that
                     ok = ok && pack.walk(
                         s.runs, n_runs, p.rank, ring.h_rows(),
@@ -535,7 +535,7 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
                     const int col0 = (item % tiles.n_ntile) * tiles.n_tok;
                     int n_runs = p.lora_b && waited ? find_runs(p, tiles, col0, runs) : 0;
                     uint32_t d_tmem = 0;
-                    if (lane == 0) {  // one lane issues
+                    if (elect_one()) {  // one lane issues
                         for (int ks = 0; ok && ks < n_kstage; ++ks) {
                             const bool opens = SEGMENTED ? ks % HEAD_SEGMENT == 0 : ks == 0;
                             if (opens) {
@@ -565,7 +565,7 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
                         waited = true;
                         n_runs = find_runs(p, tiles, col0, runs);
                     }
-                    if (lane == 0 && ok) {
+                    if (elect_one() && ok) {
                         ok = pack.walk(
                             runs, n_runs, p.rank, ring.h_rows(), filled_stage,
                             [&](int i, int row, const Run& run, int r0) {
@@ -584,7 +584,7 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
                             release_stage);
                         if (ok) publish();
                     }
-                    if (!__shfl_sync(0xffffffffu, int(ok), 0)) break;
+                    if (!__all_sync(0xffffffffu, ok)) break;
                 }
             }
         }

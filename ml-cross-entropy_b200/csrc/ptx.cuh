@@ -192,6 +192,14 @@ __device__ __forceinline__ void set_max_regs_down() { asm volatile("setmaxnreg.d
 template <int N>
 __device__ __forceinline__ void set_max_regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
+// True in one lane of a converged warp, the same one every time.  Behind this test, unlike `lane == 0`, the compiler knows that
+// a single lane is active.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes != 0;
+}
+
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
