@@ -12,7 +12,7 @@
 // (one TMEM lane) owns one vocabulary entry, so that a warp's store covers 32 neighbouring logits of one token.
 //
 //   warp 0      : TMA producer of both CTAs (128-byte swizzled ring; as many stages as shared memory holds)
-//   warp 1      : tcgen05.mma issuer (leader CTA), owner of the TMEM (2 accumulators of 128 x 256 fp32 per CTA)
+//   warp 1      : tcgen05.mma issuer (leader CTA), owner of the TMEM (512 columns: 2 to 8 accumulators per CTA)
 //   warps 4..11 : epilogue; warp w reads TMEM lanes 32*(w%4)..+31, two warps share a quarter
 //
 // The adapters' second product.  The accumulator's columns are looked at in groups of 16.  A group whose tokens
@@ -438,11 +438,13 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
                 if (rank == 0) mbar_expect_tx(smem_u32(&s.full[stage]), 2 * bytes);
             };
             bool ok = true, waited = ordered;  // waited: for the kernel that makes h
+            int n_runs = 0;
             for (int item = pair; item < n_items; item += n_pairs) {
                 const int row_c = (item / tiles.n_ntile) * 2 * BM + rank * BM;
                 const int col0 = (item % tiles.n_ntile) * tiles.n_tok;
                 const int row_e = col0 + rank * (tiles.n_tok / 2);
-                int n_runs = p.lora_b && waited ? find_runs(p, tiles, col0, s.runs) : 0;
+                // (with one column tile they are the same in every item)
+                if (p.lora_b && waited && (item == pair || tiles.n_ntile > 1)) n_runs = find_runs(p, tiles, col0, s.runs);
                 if (elect_one()) {  // one lane runs the loop over the stages
                     for (int ks = 0; ok && ks < n_kstage; ++ks) {
                         ok = free_stage();
@@ -531,9 +533,11 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
                 constexpr int STEP = UMMA_K * 2 >> 4;  // descriptor units (16 bytes) per MMA step
                 Run* runs = s.runs + HEAD_MAX_RUNS;
                 bool ok = true, waited = ordered;
+                int n_runs = 0;
                 for (int item = pair; item < n_items; item += n_pairs) {
                     const int col0 = (item % tiles.n_ntile) * tiles.n_tok;
-                    int n_runs = p.lora_b && waited ? find_runs(p, tiles, col0, runs) : 0;
+                    // (with one column tile they are the same in every item)
+                    if (p.lora_b && waited && (item == pair || tiles.n_ntile > 1)) n_runs = find_runs(p, tiles, col0, runs);
                     uint32_t d_tmem = 0;
                     if (elect_one()) {  // one lane issues
                         for (int ks = 0; ok && ks < n_kstage; ++ks) {
@@ -599,15 +603,16 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
         if (p.lora_b) pdl_wait();
         const HeadTiles tiles(p);
         const int n_items = p.n_vtile * tiles.n_ntile;
+        unsigned mixed = 0;  // bit g: group g of the tile is mixed
         const int n_seg = SEGMENTED ? (n_kstage + HEAD_SEGMENT - 1) / HEAD_SEGMENT : 1;
         for (int item = pair; item < n_items; item += n_pairs) {
             const int v = (item / tiles.n_ntile) * 2 * BM + rank * BM + q * 32 + lane;
             const int col0 = (item % tiles.n_ntile) * tiles.n_tok;
             const int col_end = min(tiles.n_col, col0 + tiles.n_tok);
             const float bias = (p.bias && v < p.V) ? __ldg(p.bias + v) : 0.0f;
-            // bit g: group g of the tile is mixed
-            const unsigned mixed = __ballot_sync(0xffffffffu, p.lora_b && lane < HEAD_MAX_RUNS && col0 + lane * HEAD_GROUP < col_end &&
-                                                                  group_adapter(p, col0 / HEAD_GROUP + lane) == GROUP_MIXED);
+            if (p.lora_b && (item == pair || tiles.n_ntile > 1))
+                mixed = __ballot_sync(0xffffffffu, lane < HEAD_MAX_RUNS && col0 + lane * HEAD_GROUP < col_end &&
+                                                       group_adapter(p, col0 / HEAD_GROUP + lane) == GROUP_MIXED);
             float sum[SEGMENTED ? CHUNKS : 1][32];
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c)
