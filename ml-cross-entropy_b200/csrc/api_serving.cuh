@@ -158,8 +158,9 @@ int plan_sample(const cce_b200_sample_args* a, SamplePlan* out) {
     SamplePlan pl = {};
     const int elem = a->dtype == CCE_DT_F32 ? 4 : 2;
     if (a->V > (1 << 20)) return CCE_ERR_TOO_LARGE;  // the weights keep at least 42 bits
-    // CTAs per row.  Few rows: short slices (1 x 256000 fp32: 22.5 us with 16384 positions, 24.6 with 32768);
-    // many rows: fewer, longer ones, whose fixed cost is paid less often (512 x 152064: 803 us against 1360).
+    // CTAs per row.  Few rows: short slices (fp32, 1 x 256000: 20 us with 16384 positions, 24 with 32768; 16 x 256000,
+    // top-p: 81 and 88; 31 x 128256: 53 and 51); many rows: fewer, longer ones, whose fixed cost is paid less often
+    // (bf16, 64 x 128256, top-k and top-p: 41 and 29; top-p: 97 and 66; 100 x 152064: 287 and 164).
     const int longest = a->B >= 32 ? 32768 : 16384;
     pl.cluster = 1;
     while (pl.cluster < SMP_MAX_CLUSTER && sample_slice(a->V, pl.cluster) > longest) pl.cluster *= 2;

@@ -24,10 +24,11 @@
 // Unless the adapters are many (api_serving.cuh has the rule) adapter_layout_kernel orders the columns by
 // adapter, each adapter's run padded to whole groups, so that no group is mixed.
 //
-// Measured (bf16, device time): 1 x 152064 x 3584 192 us (5.7 TB/s, as cuBLAS), 64 tokens 201, 256 tokens 246 (cuBLAS
-// 256), 2048 tokens 1540 (1440); with 4 adapters of rank 16 203, 236, 370, 1800.  The loads of a tile cost their issue:
-// 16-row boxes that fit the columns exactly took 2048 tokens from 1.8 to 2.9 ms, so the token loads have four sizes and
-// the runs of h two.
+// Measured (bf16, device time, 152064 x 3584): 1 token 180 us (6.05 TB/s; cuBLAS 188), 64 tokens 191 (197), 256 tokens 238
+// (254), 2048 tokens 1430 (1430); with 4 adapters of rank 16 182, 210, 311, 1650; fp32 logits 178, 191, 254, 1530.  Up to
+// 128 columns HBM bounds it; then the loads from L2 (256 tokens: 2.1 GB of tiles, 9 TB/s), at 2048 the tensor pipe.
+// One lane issues: an MMA of 144 columns then follows the last one after 78 cycles, which is what the tensor pipe takes, a
+// TMA load after 120.  Few and large loads for that reason: the token loads have four sizes, the runs of h two.
 #pragma once
 #include "engine.cuh"
 #include "ptx_pair.cuh"
@@ -52,8 +53,7 @@ constexpr int GROUP_NONE = -1, GROUP_MIXED = -2;
 constexpr int HEAD_MAX_ACC = 8;
 // fp32 logits: the tensor core truncates every addition, so a sum over all of D drifts (2.4e-6 of the logits'
 // norm at D = 2304).  The accumulator is therefore emptied every HEAD_SEGMENT stages into fp32 registers,
-// which add with rounding (4.5e-7; twice as often: 2.7e-7, but 366 instead of 325 us for 144 columns, whose tile then
-// waits for its epilogue).  16-bit logits are rounded far above the drift and take the sum in one piece.
+// which add with rounding (4.5e-7; twice as often: 2.7e-7, but 228 instead of 222 us for 144 columns).  16-bit logits are rounded far above the drift and take the sum in one piece.
 constexpr int HEAD_SEGMENT = 4;
 
 struct HeadParams {
