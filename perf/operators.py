@@ -10,7 +10,6 @@
 
 from __future__ import annotations
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -221,7 +220,6 @@ def run(state):
     )  # fmt: skip
 
 
-@functools.cache
 def _package():
     path = str(Path("ml-cross-entropy_b200").resolve())
     if path not in sys.path:
