@@ -10,7 +10,7 @@
 //   row_max_kernel     the largest logit of every chunk
 //   row_prepare_kernel per row (a warp): its maximum and thresholds, and whether there is anything to do (RowMode)
 //   row_stats_kernel   counts by bin and, for top-p alone, the exact sum of the weights; without any filter: the
-//                      weights by blocks of 512 positions
+//                      weights by blocks of 512 positions, and the first of the largest logits of greedy rows
 //   row_plan_kernel    per row with a filter: which logits are needed in order
 //   row_pass_kernel    gathers them, and sums the kept weights by blocks where not everything is gathered
 //   row_draw_kernel    per row: the border among the gathered, the draw
@@ -150,6 +150,22 @@ row_prepare_kernel(const SampleParams p, const StreamBuffers b, long long B) {
     b.state[row] = st;
 }
 
+// ROW_GREEDY: the lowest index of the largest logits of a chunk joins the row's.
+template <typename T>
+__device__ __forceinline__ void first_of_largest(const RowBase& r, const RowStream<T>& rs, const StreamBuffers& b, int chunk,
+                                                 float mx) {
+    unsigned best = 0xffffffffu;
+    for (int i = r.warp; i < STR_BLOCKS; i += SMP_WARPS) {
+        const long long block = (long long)chunk * STR_BLOCKS + i;
+        if (rs.holds(block))
+            rs.each(block, r.lane, [&](float l, long long pos) {
+                if (l == mx) best = min(best, unsigned(pos - rs.phase));
+            });
+    }
+    best = __reduce_min_sync(0xffffffffu, best);
+    if (r.lane == 0 && best != 0xffffffffu) atomicMin(&b.state[r.row].first, best);
+}
+
 // FILTERS: some row may have top-k or top-p
 template <typename T, bool FILTERS>
 __global__ void __launch_bounds__(SMP_THREADS, 3)
@@ -167,6 +183,10 @@ row_stats_kernel(const SampleParams p, const StreamBuffers b) {
     const RowStream<T> rs(p, row);
     pdl_wait();
     const RowState st = b.state[row];
+    if (!FILTERS && st.mode == ROW_GREEDY) {  // with filters row_pass_kernel does it
+        first_of_largest(r, rs, b, chunk, st.mx);
+        return;
+    }
     if (st.mode != (FILTERS ? ROW_LIST : ROW_SUM)) return;
     r.prepare(st);
     __syncthreads();
@@ -328,16 +348,7 @@ row_pass_kernel(const SampleParams p, const StreamBuffers b) {
     const RowState st = b.state[row];
     if (st.mode == ROW_DONE || st.mode == ROW_BY_CLUSTER) return;
     if (st.mode == ROW_GREEDY) {
-        unsigned best = 0xffffffffu;
-        for (int i = r.warp; i < STR_BLOCKS; i += SMP_WARPS) {
-            const long long block = (long long)chunk * STR_BLOCKS + i;
-            if (rs.holds(block))
-                rs.each(block, r.lane, [&](float l, long long pos) {
-                    if (l == st.mx) best = min(best, unsigned(pos - rs.phase));
-                });
-        }
-        best = __reduce_min_sync(0xffffffffu, best);
-        if (r.lane == 0 && best != 0xffffffffu) atomicMin(&b.state[row].first, best);
+        first_of_largest(r, rs, b, chunk, st.mx);
         return;
     }
     r.prepare(st);

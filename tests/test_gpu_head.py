@@ -442,6 +442,52 @@ def test_sample_many_long_rows_with_their_own_settings():
     _check_sample(x, u, **kw)
 
 
+@pytest.mark.parametrize("dtype, B", [(FP32, 70), (BF16, 140)])
+@pytest.mark.parametrize("min_p", [None, 0.3])
+def test_sample_many_long_greedy_rows_without_filters(dtype, B, min_p):
+    """Enough logits for the streaming kernels and neither top-k nor top-p: greedy rows alone and among others."""
+    V = 120_011
+    x, u = _rows(B, V, dtype, seed=41)
+    x[0] = -math.inf
+    x[1] = 2.0  # all are the largest
+    x[2, [5, 60_000, 119_999]] = 90.0  # tied maxima, the first in the first chunk ..
+    x[3, [119_000, 119_999]] = 90.0  # .. and both in the last one
+    x[4, 1:] = -math.inf
+    x[5] = math.nan
+    x[5, 100_001] = -7.0
+    x[6] = -0.0
+    x[6, 33] = 0.0
+    x[7, [77, 78]] = math.inf
+    assert x.numel() * x.element_size() >= 32 << 20
+    first = torch.tensor([-1, 0, 5, 119_000, 0, 100_001, 0, 77])
+    tok, lp = sample_tokens(x, u, temperature=0.0, min_p=min_p, return_logprobs=True)
+    assert torch.equal(tok[:8].cpu(), first)
+    is_max = x[8:] == x[8:].amax(1, keepdim=True)
+    assert torch.equal(tok[8:], is_max.int().argmax(1))  # the first of the largest
+    assert bool((lp[1:] == 0).all()) and lp[0] == -math.inf
+    for i in (0, 2, 3, 20, B - 1):
+        assert sample_tokens(x[i], u[i], temperature=0.0, min_p=min_p).item() == tok[i].item()
+    temperature = torch.where(torch.arange(B, device=DEV) % 3 == 1, 0.8, torch.zeros(B, device=DEV))
+    temperature[3] = math.nan  # in a tensor: greedy
+    mixed = sample_tokens(x, u, temperature=temperature, min_p=min_p)
+    cold = ~(temperature > 0)
+    assert torch.equal(mixed[cold], tok[cold])
+    some = [1, 4, 7, 10, 13, 16]
+    as_stored = torch.tensor(0.8).item()
+    warm, _ = H.sample_tokens(x[some].cpu(), u[some].cpu(), temperature=as_stored, min_p=min_p)
+    assert torch.equal(mixed[some].cpu(), warm)
+
+
+def test_linear_sample_of_a_large_greedy_batch():
+    """The float32 logits of 70 x 120011 go through the streaming kernels."""
+    kw = _to_dev(_inputs(70, 120_011, 64, BF16))
+    u = torch.rand(70, generator=torch.Generator().manual_seed(2)).to(DEV)
+    x = linear_logits(**kw, out_dtype=FP32)
+    tok = linear_sample(**kw, u=u, temperature=0.0)
+    assert torch.equal(tok, (x == x.amax(1, keepdim=True)).int().argmax(1))  # compared, never used as an index
+    assert torch.equal(tok, torch.stack([sample_tokens(x[i], u[i], temperature=0.0) for i in range(70)]))
+
+
 def test_sample_empty_and_too_large():
     assert sample_tokens(torch.zeros(0, 10, device=DEV), torch.zeros(0, device=DEV)).shape == (0,)
     with pytest.raises(_native.NativeError):
