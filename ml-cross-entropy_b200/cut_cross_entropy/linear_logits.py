@@ -17,6 +17,16 @@ from .linear_cross_entropy import _reject_dtensors
 MAX_RANK = 256  # CCE_B200_MAX_RANK
 
 
+def _check_plain(**named: torch.Tensor | float | None) -> None:
+    """Refuses DTensors and other wrappers: they have no memory of their own, and the C interface reads their null
+    pointer as "not given"."""
+    for name, t in named.items():
+        if type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter and isinstance(t, torch.Tensor):
+            _reject_dtensors(**{name: t})
+            if t.numel() > 0 and t.data_ptr() == 0:
+                raise ValueError(f"{name} is a {type(t).__name__}, which has no memory of its own: pass a plain tensor.")
+
+
 def _check_no_grad(name: str, *tensors: torch.Tensor | float | None) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
@@ -62,6 +72,7 @@ def linear_logits(
 
     With ``a = adapter_ids[t]``, token ``t`` adds ``lora_scale[a] * (e[t] @ lora_a[a].T) @ lora_b[a].T``.
     No gradient is computed: inputs that require one are refused unless gradients are switched off.
+    Arguments are plain tensors or parameters: DTensors and other wrappers without memory of their own are refused.
 
     :param e: embeddings ``(..., D)``: bf16, fp16, or fp32 (computed as a three-term bf16 split:
         about 16 mantissa bits).
@@ -79,8 +90,7 @@ def linear_logits(
 
     Under autocast ``e``, ``c`` and the adapters are cast to the autocast dtype first.
     """
-    if type(e) is not torch.Tensor or type(c) is not torch.Tensor:  # plain tensors are no DTensors
-        _reject_dtensors(e=e, c=c, bias=bias, lora_a=lora_a, lora_b=lora_b, adapter_ids=adapter_ids)
+    _check_plain(e=e, c=c, bias=bias, lora_a=lora_a, lora_b=lora_b, adapter_ids=adapter_ids, lora_scale=lora_scale)
     _check_no_grad("linear_logits", e, c, bias, lora_a, lora_b, lora_scale)
     if e.dim() < 1 or c.dim() != 2 or e.size(-1) != c.size(1):
         raise ValueError(f"Expected e (..., D) and c (V, D), got {tuple(e.shape)} and {tuple(c.shape)}.")

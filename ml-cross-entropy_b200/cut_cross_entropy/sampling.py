@@ -11,8 +11,7 @@ import math
 import torch
 
 from . import _native
-from .linear_cross_entropy import _reject_dtensors
-from .linear_logits import _check_device, _check_no_grad, _on_device, _rows, linear_logits
+from .linear_logits import _check_device, _check_no_grad, _check_plain, _on_device, _rows, linear_logits
 
 
 def _setting(name, value, batch_shape, device, dtype, hi):
@@ -62,9 +61,9 @@ def sample_tokens(
 
     The numbers in tensors are not looked at on the host: there, a temperature of 0 or less (or NaN) is greedy,
     ``top_p`` outside (0, 1) and ``min_p`` outside (0, 1] act like the nearest value inside, or like "off".
+    Arguments are plain tensors or parameters: DTensors and other wrappers without memory of their own are refused.
     """
-    if type(logits) is not torch.Tensor or type(u) is not torch.Tensor:  # plain tensors are no DTensors
-        _reject_dtensors(logits=logits, u=u)
+    _check_plain(logits=logits, u=u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
     _check_no_grad("sample_tokens", logits, u, temperature, top_p, min_p)
     batch_shape = u.shape
     if logits.dim() < 1 or batch_shape != logits.shape[:-1]:

@@ -88,6 +88,67 @@ def test_linear_logits_refuses_a_scale_that_wants_a_gradient():
         linear_logits(**args, lora_scale=torch.ones(args["lora_a"].size(0), requires_grad=True))
 
 
+@pytest.fixture(scope="module")
+def as_dtensor():
+    """Wraps a host tensor as a DTensor on a mesh of one rank."""
+    import torch.distributed as dist
+    from torch.distributed.device_mesh import DeviceMesh
+    from torch.distributed.tensor import DTensor, Replicate
+
+    dist.init_process_group("gloo", store=dist.HashStore(), rank=0, world_size=1)
+    try:
+        mesh = DeviceMesh("cpu", [0])
+        yield lambda t: DTensor.from_local(t, mesh, [Replicate()])
+    finally:
+        dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("name", ["e", "c", "bias", "lora_a", "lora_b", "adapter_ids", "lora_scale"])
+def test_linear_logits_refuses_dtensors(name, as_dtensor):
+    args = dict(e=torch.zeros(4, 16), c=torch.zeros(10, 16), bias=torch.zeros(10), **_lora(), lora_scale=torch.ones(2))
+    args[name] = as_dtensor(args[name])
+    with pytest.raises(ValueError, match=f"{name} as a torch.distributed.tensor.DTensor"):
+        linear_logits(**args)
+    with pytest.raises(ValueError, match=f"{name} as a torch.distributed.tensor.DTensor"):
+        linear_sample(**args, u=torch.zeros(4))
+
+
+@pytest.mark.parametrize("name", ["logits", "u", "temperature", "top_k", "top_p", "min_p"])
+def test_sample_tokens_refuses_dtensors(name, as_dtensor):
+    args = dict(logits=torch.zeros(4, 7), u=torch.zeros(4), temperature=torch.ones(4), top_k=torch.ones(4).long(),
+                top_p=torch.ones(4), min_p=torch.zeros(4))  # fmt: skip
+    args[name] = as_dtensor(args[name])
+    with pytest.raises(ValueError, match=f"{name} as a torch.distributed.tensor.DTensor"):
+        sample_tokens(**args)
+
+
+class _Wrapper(torch.Tensor):
+    """A tensor whose values are kept elsewhere."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError(str(func))
+
+
+class _Marked(torch.Tensor):
+    """A tensor with memory of its own, of another class."""
+
+
+def test_wrappers_without_memory_are_refused_and_other_subclasses_are_not():
+    args = dict(e=torch.zeros(4, 16), c=torch.zeros(10, 16), bias=torch.zeros(10))
+    with pytest.raises(ValueError, match="bias is a _Wrapper"):
+        linear_logits(**dict(args, bias=_Wrapper(args["bias"])))
+    with pytest.raises(ValueError, match="temperature is a _Wrapper"):
+        sample_tokens(torch.zeros(4, 7), torch.zeros(4), temperature=_Wrapper(torch.ones(4)))
+    # these get as far as host tensors do
+    with pytest.raises(RuntimeError, match="needs CUDA tensors"):
+        linear_logits(**dict(args, bias=args["bias"].as_subclass(_Marked), c=torch.nn.Parameter(args["c"], requires_grad=False)))
+
+
 def test_rows_of_one_column_have_unit_stride():
     wide = torch.arange(12.0).reshape(3, 4)
     for t in (wide[:1].t(), wide.t()[:, 1:2], wide[:, 2:3], wide[:1, :1], torch.zeros(1).expand(5, 1)):
