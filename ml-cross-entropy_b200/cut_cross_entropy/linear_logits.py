@@ -10,6 +10,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .linear_cross_entropy import _reject_dtensors
@@ -32,6 +33,10 @@ def _check_no_grad(name: str, *tensors: torch.Tensor | float | None) -> None:
         for t in tensors:
             if isinstance(t, torch.Tensor) and t.requires_grad:
                 raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or torch.inference_mode().")
+    if forward_ad._current_level >= 0:  # inside a dual_level; torch.no_grad() does not drop tangents
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name} has no forward-mode derivative: pass the primal, or call it under torch.inference_mode().")
 
 
 def _check_device(device: torch.device, *named: tuple[str, torch.Tensor | None]) -> None:
@@ -71,7 +76,8 @@ def linear_logits(
     """``softcap(e @ c.T + bias + adapters)``, where every token adds its own request's low-rank adapter.
 
     With ``a = adapter_ids[t]``, token ``t`` adds ``lora_scale[a] * (e[t] @ lora_a[a].T) @ lora_b[a].T``.
-    No gradient is computed: inputs that require one are refused unless gradients are switched off.
+    No gradient is computed: inputs that require one are refused unless gradients are switched off, and inputs with a
+    forward-mode tangent are refused.
     Arguments are plain tensors or parameters: DTensors and other wrappers without memory of their own are refused.
 
     :param e: embeddings ``(..., D)``: bf16, fp16, or fp32 (computed as a three-term bf16 split:

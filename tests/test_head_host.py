@@ -149,6 +149,33 @@ def test_wrappers_without_memory_are_refused_and_other_subclasses_are_not():
         linear_logits(**dict(args, bias=args["bias"].as_subclass(_Marked), c=torch.nn.Parameter(args["c"], requires_grad=False)))
 
 
+@pytest.mark.parametrize("name", ["e", "c", "bias", "lora_a", "lora_b", "lora_scale"])
+def test_linear_logits_refuses_tangents(name):
+    import torch.autograd.forward_ad as fwd
+
+    args = dict(e=torch.zeros(4, 16), c=torch.zeros(10, 16), bias=torch.zeros(10), **_lora(), lora_scale=torch.ones(2))
+    with fwd.dual_level():
+        with pytest.raises(RuntimeError, match="needs CUDA tensors"):  # no tangent in sight
+            linear_logits(**args)
+        args[name] = fwd.make_dual(args[name], torch.ones_like(args[name]))
+        for context in (torch.enable_grad(), torch.no_grad()):
+            with context, pytest.raises(RuntimeError, match="forward-mode"):
+                linear_logits(**args)
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda x: linear_logits(x, torch.zeros(10, 16)), (torch.zeros(4, 16),), (torch.ones(4, 16),))
+
+
+@pytest.mark.parametrize("name", ["logits", "u", "temperature", "top_p", "min_p"])
+def test_sample_tokens_refuses_tangents(name):
+    import torch.autograd.forward_ad as fwd
+
+    args = dict(logits=torch.zeros(4, 7), u=torch.zeros(4))
+    with fwd.dual_level():
+        args[name] = fwd.make_dual(torch.full((4, 7) if name == "logits" else (4,), 0.5), torch.ones(4, 7) if name == "logits" else torch.ones(4))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            sample_tokens(**args)
+
+
 def test_rows_of_one_column_have_unit_stride():
     wide = torch.arange(12.0).reshape(3, 4)
     for t in (wide[:1].t(), wide.t()[:, 1:2], wide[:, 2:3], wide[:1, :1], torch.zeros(1).expand(5, 1)):
