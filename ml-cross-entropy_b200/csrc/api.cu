@@ -97,24 +97,12 @@ bool pair_enabled() {
     return on;
 }
 
-template <typename T>
-cudaError_t head_logits_attributes() {
-    for (auto* k : {head_logits_kernel<T, 0>, head_logits_kernel<T, 1>, head_logits_kernel<T, 2>, head_logits_kernel<T, 3>,
-                    head_logits_kernel<T, 4>}) {
-        cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, HEAD_SMEM);
-        cudaFuncAttributes attr;
-        if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, k);
-        // the split of the registers hands out what the block was launched with: with fewer it would wait for good
-        if (e == cudaSuccess && attr.numRegs != HEAD_REGS) e = cudaErrorInvalidKernelImage;
-        if (e != cudaSuccess) return e;
-    }
-    return cudaSuccess;
-}
-
 struct DeviceInfo {
     int sms = 0;
     int cc_major = 0;
     bool attr_set = false;
+    // The serving kernels are set up when they are first launched (api_serving.cuh): the loss does not depend on them.
+    std::atomic<bool> head_set[3][HEAD_FORMS] = {}, sample_set[3] = {};
 };
 
 // Per-device facts, looked up once per device (immutable afterwards).
@@ -144,14 +132,6 @@ int device_info(DeviceInfo** out) {
                                       PAIR_SMEM));
         CCE_CUDA(cudaFuncSetAttribute(pair_engine_kernel<MODE_GEMM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       PAIR_SMEM + PEER_STAGE_BYTES));
-        CCE_CUDA(head_logits_attributes<float>());
-        CCE_CUDA(head_logits_attributes<__half>());
-        CCE_CUDA(head_logits_attributes<__nv_bfloat16>());
-        for (const void* k : {(const void*)sample_kernel<float>, (const void*)sample_kernel<__half>,
-                              (const void*)sample_kernel<__nv_bfloat16>}) {
-            CCE_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMP_SMEM));
-            CCE_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        }
         d.attr_set = true;
     }
     *out = &d;

@@ -105,15 +105,38 @@ inline bool head_segmented(const HeadParams& hp) {
     return hp.out_dtype == CCE_DT_F32 && cdiv(hp.n_kblk, HEAD_KSUB) > HEAD_SEGMENT;
 }
 
+// What a form of the kernel needs before its first launch on a device.
+template <typename T, int CHUNKS>
+int setup_head() {
+    CCE_CUDA(cudaFuncSetAttribute(head_logits_kernel<T, CHUNKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, HEAD_SMEM));
+    if (CHUNKS > HEAD_SPLIT_ABOVE) {
+        // the split hands out what the block was launched with: with fewer it would wait for good
+        cudaFuncAttributes attr;
+        CCE_CUDA(cudaFuncGetAttributes(&attr, head_logits_kernel<T, CHUNKS>));
+        if (attr.numRegs != HEAD_REGS) return CCE_ERR_UNSUPPORTED;
+    }
+    return CCE_OK;
+}
+
 // With adapters the projection may start while the shrink kernel, launched just before it, still runs.
+template <typename T, int CHUNKS>
+int launch_head_form(DeviceInfo* dev, int dtype, const HeadMaps& maps, const HeadParams& hp, int grid, cudaStream_t st) {
+    std::atomic<bool>& set = dev->head_set[dtype][CHUNKS];
+    if (!set) {
+        const int rc = setup_head<T, CHUNKS>();
+        if (rc) return rc;
+        set = true;
+    }
+    return launch_behind(head_logits_kernel<T, CHUNKS>, dim3(grid), HEAD_THREADS, HEAD_SMEM, st, hp.lora_b != nullptr, maps, hp);
+}
+
 template <typename T>
-int launch_head(const HeadMaps& maps, const HeadParams& hp, int grid, cudaStream_t st) {
-    const auto kernel = !head_segmented(hp) ? head_logits_kernel<T, 0>
-                        : hp.n_tok <= 64    ? head_logits_kernel<T, 1>
-                        : hp.n_tok <= 128   ? head_logits_kernel<T, 2>
-                        : hp.n_tok <= 192   ? head_logits_kernel<T, 3>
-                                            : head_logits_kernel<T, 4>;
-    return launch_behind(kernel, dim3(grid), HEAD_THREADS, HEAD_SMEM, st, hp.lora_b != nullptr, maps, hp);
+int launch_head(DeviceInfo* dev, int dtype, const HeadMaps& maps, const HeadParams& hp, int grid, cudaStream_t st) {
+    if (!head_segmented(hp)) return launch_head_form<T, 0>(dev, dtype, maps, hp, grid, st);
+    if (hp.n_tok <= 64) return launch_head_form<T, 1>(dev, dtype, maps, hp, grid, st);
+    if (hp.n_tok <= 128) return launch_head_form<T, 2>(dev, dtype, maps, hp, grid, st);
+    if (hp.n_tok <= 192) return launch_head_form<T, 3>(dev, dtype, maps, hp, grid, st);
+    return launch_head_form<T, 4>(dev, dtype, maps, hp, grid, st);
 }
 
 // The adapters' rows of B, [n][V][rank], as a 3-D map: a box of 16, 32 or 64 ranks x 128 classifier rows of one
@@ -196,7 +219,14 @@ int plan_sample(const cce_b200_sample_args* a, SamplePlan* out) {
 }
 
 template <typename T>
-int launch_sample(const SampleParams& sp, const SamplePlan& pl, long long B, char* ws, cudaStream_t st) {
+int launch_sample(DeviceInfo* dev, int dtype, const SampleParams& sp, const SamplePlan& pl, long long B, char* ws,
+                  cudaStream_t st) {
+    std::atomic<bool>& set = dev->sample_set[dtype];
+    if (!set) {
+        CCE_CUDA(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMP_SMEM));
+        CCE_CUDA(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        set = true;
+    }
     RowState* only = nullptr;
     if (pl.stream) {
         StreamBuffers b = {};
@@ -377,9 +407,9 @@ int cce_b200_logits(const cce_b200_logits_args* a, void* workspace, size_t works
     const long long n_items = (long long)hp.n_vtile * n_ntile;
     if (n_items >= (1LL << 30)) return CCE_ERR_ARG;
     const int grid = 2 * (int)std::min<long long>(dev->sms / 2, n_items);
-    if (op.dtype == CCE_DT_F32) return launch_head<float>(maps, hp, grid, st);
-    if (op.dtype == CCE_DT_BF16) return launch_head<__nv_bfloat16>(maps, hp, grid, st);
-    return launch_head<__half>(maps, hp, grid, st);
+    if (op.dtype == CCE_DT_F32) return launch_head<float>(dev, op.dtype, maps, hp, grid, st);
+    if (op.dtype == CCE_DT_BF16) return launch_head<__nv_bfloat16>(dev, op.dtype, maps, hp, grid, st);
+    return launch_head<__half>(dev, op.dtype, maps, hp, grid, st);
 }
 
 size_t cce_b200_sample_workspace_bytes(const cce_b200_sample_args* a) {
@@ -423,9 +453,9 @@ int cce_b200_sample(const cce_b200_sample_args* a, void* workspace, size_t works
     for (int j = 0; j < SMP_TABLE; ++j) sp.table[j] = WeightFn::entry(j, sp.frac_bits);
     char* ws = reinterpret_cast<char*>(workspace);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (a->dtype == CCE_DT_F32) return launch_sample<float>(sp, pl, a->B, ws, st);
-    if (a->dtype == CCE_DT_BF16) return launch_sample<__nv_bfloat16>(sp, pl, a->B, ws, st);
-    return launch_sample<__half>(sp, pl, a->B, ws, st);
+    if (a->dtype == CCE_DT_F32) return launch_sample<float>(dev, a->dtype, sp, pl, a->B, ws, st);
+    if (a->dtype == CCE_DT_BF16) return launch_sample<__nv_bfloat16>(dev, a->dtype, sp, pl, a->B, ws, st);
+    return launch_sample<__half>(dev, a->dtype, sp, pl, a->B, ws, st);
 }
 
 }  // extern "C"

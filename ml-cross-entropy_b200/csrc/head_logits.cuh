@@ -43,6 +43,7 @@ constexpr int HEAD_REGS = 168;                 // per thread at launch: 65536 / 
 constexpr int HEAD_REGS_FEW = 72, HEAD_REGS_MANY = 216;
 static_assert(HEAD_EPI_FIRST * HEAD_REGS_FEW + HEAD_EPI_WARPS * HEAD_REGS_MANY <= (HEAD_EPI_FIRST + HEAD_EPI_WARPS) * HEAD_REGS,
               "no more registers than the block was launched with");
+constexpr int HEAD_SPLIT_ABOVE = 2;            // chunks of 32 columns per warp above which the registers are split
 constexpr int HEAD_KSUB = 2;                   // 64-element K sub-blocks per ring stage
 constexpr int HEAD_MAX_STAGES = 8;
 constexpr int HEAD_SMEM = 227 * 1024;          // everything: the ring decides how many bytes are in flight
@@ -51,6 +52,7 @@ constexpr int HEAD_GROUP = 16;                 // tokens that share one decision
 constexpr int ADAPTER_RANK_PAD = 16;           // fp32 rows of h are padded to this many ranks with zeros
 constexpr int GROUP_NONE = -1, GROUP_MIXED = -2;
 constexpr int HEAD_MAX_ACC = 8;
+constexpr int HEAD_FORMS = 5;  // of head_logits_kernel: CHUNKS 0 to 4
 // fp32 logits: the tensor core truncates every addition, so a sum over all of D drifts (2.4e-6 of the logits'
 // norm at D = 2304).  The accumulator is therefore emptied every HEAD_SEGMENT stages into fp32 registers,
 // which add with rounding (4.5e-7; twice as often: 2.7e-7, but 228 instead of 222 us for 144 columns).  16-bit logits are rounded far above the drift and take the sum in one piece.
@@ -411,7 +413,7 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
     const AdapterPack pack(p.rank);
     const bool ordered = p.col_token != nullptr;  // the columns come from the kernels before this one
     if (warp < HEAD_EPI_FIRST) {
-        if constexpr (CHUNKS > 2) set_max_regs_down<HEAD_REGS_FEW>();
+        if constexpr (CHUNKS > HEAD_SPLIT_ABOVE) set_max_regs_down<HEAD_REGS_FEW>();
         if (warp == 0) {
             if (ordered) {
                 const int row = pair * 2 * BM + rank * BM;  // of the first tile, if there is one column tile
@@ -593,7 +595,7 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
             }
         }
     } else {
-        if constexpr (CHUNKS > 2) set_max_regs_up<HEAD_REGS_MANY>();
+        if constexpr (CHUNKS > HEAD_SPLIT_ABOVE) set_max_regs_up<HEAD_REGS_MANY>();
         const int q = warp & 3;              // TMEM lane quarter this warp may read
         const int half = (warp - HEAD_EPI_FIRST) >> 2;    // the quarter's two warps take alternate chunks of 32 columns
         const uint32_t tempty0 = map_to_cta(smem_u32(s.tempty), 0);

@@ -245,6 +245,17 @@ def test_c_entry_points_check_their_arguments():
     assert L.cce_b200_sample(sample_args(B=0, logits=None), None, 0, None) == 0
 
 
+def test_the_loss_does_not_depend_on_the_serving_kernels():
+    """What every entry point asks of the device names none of them: they are set up at their own first launch."""
+    from pathlib import Path
+
+    src = (Path(__file__).resolve().parent.parent / "ml-cross-entropy_b200" / "csrc" / "api.cu").read_text()
+    body = src[src.index("int device_info(DeviceInfo** out) {") :]
+    body = body[: body.index("\n}\n")]
+    assert "engine_kernel" in body
+    assert "head_" not in body and "sample_" not in body
+
+
 def test_struct_sizes_match_the_header(tmp_path):
     import shutil
     import subprocess
