@@ -19,6 +19,8 @@ int check_logits_args(const cce_b200_logits_args* a) {
     return CCE_OK;
 }
 
+inline int h_terms(int dtype) { return dtype == CCE_DT_BF16 ? H_TERMS<__nv_bfloat16> : H_TERMS<__half>; }
+
 struct LogitsPlan {
     OperandPlan ops;
     long long ldh, n_col, n_group;
@@ -66,8 +68,9 @@ LogitsPlan plan_logits(const cce_b200_logits_args* a) {
     }
     if (a->lora_b) {
         pl.ldh = cdiv(a->rank, ADAPTER_RANK_PAD) * ADAPTER_RANK_PAD;
-        pl.pitch16 = mma ? h16_pitch((int)a->rank) : 0;
-        pl.shrink_ranks = (int)(!mma ? pl.ldh : a->rank <= 32 ? 32 : cdiv(a->rank, 64) * 64);
+        const HPack pack((int)a->rank, h_terms(a->op.dtype));
+        pl.pitch16 = mma ? pack.pitch : 0;
+        pl.shrink_ranks = mma ? pack.ranks : (int)pl.ldh;
         pl.off_h = take((size_t)pl.n_col * pl.ldh * 4);
         pl.off_h16 = take((size_t)pl.n_col * pl.pitch16 * 2);
     }
@@ -149,7 +152,7 @@ int make_tmap_adapters(CUtensorMap* m, const void* base, int dtype, long long ra
     }
     cuuint64_t dims[3] = {(cuuint64_t)rank, (cuuint64_t)V, (cuuint64_t)n};
     cuuint64_t strides[2] = {(cuuint64_t)rank * 2, (cuuint64_t)(rank * V) * 2};
-    const int width = AdapterPack((int)rank).a_bytes / (BM * 2);
+    const int width = AdapterPack((int)rank, h_terms(dtype)).width;
     cuuint32_t box[3] = {(cuuint32_t)width, (cuuint32_t)BM, 1};
     cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = enc(m, dtype == CCE_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,

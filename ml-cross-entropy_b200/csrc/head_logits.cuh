@@ -17,8 +17,8 @@
 //
 // The adapters' second product.  The accumulator's columns are looked at in groups of 16.  A group whose tokens
 // all use one adapter (or none) takes it on the tensor cores, as further reduction blocks of the same columns: A
-// operand = the tile's rows of B, B operand = the group's h, split into two 16-bit terms (hi + lo) so that it keeps
-// 16 or more bits.  A group of several adapters is added by the epilogue in fp32, every token with its own rows
+// operand = the tile's rows of B, B operand = the group's h, split into 16-bit terms of one sign: two in fp16
+// (22 bits), three in bf16 (23).  A group of several adapters is added by the epilogue in fp32, every token with its own rows
 // of B: a masked tensor-core product would multiply one request's adapter by another's zeros, and an infinity
 // there would reach the wrong row.  The same holds for groups whose h does not fit the 16-bit type.
 // Unless the adapters are many (api_serving.cuh has the rule) adapter_layout_kernel orders the columns by
@@ -125,9 +125,29 @@ struct HeadRing {
 // take 15 us, in which HBM could deliver 90 MB: 16 stages are 78 MB)
 constexpr int HEAD_L2_AHEAD = 16;
 
-// Layout of the 16-bit rows of h: rank <= 32 (one 64-element block): hi in columns 0..31, lo in 32..63; above that,
-// for every 64 ranks a block of hi and a block of lo.
-__host__ __device__ inline int h16_pitch(int rank) { return rank <= 32 ? 64 : (rank + 63) / 64 * 128; }
+// The terms of h in its 16-bit type, see SplitH
+template <typename T>
+constexpr int H_TERMS = 2;
+template <>
+constexpr int H_TERMS<__nv_bfloat16> = 3;
+
+// How h and B meet on the tensor cores: `width` ranks at a time.  The 16-bit rows of h consist of blocks of 64 elements
+// (128 bytes, a swizzle row); `width` ranks take one or two of them.
+//   two terms    rank <= 32: one block, 32 ranks of each term; above: 64 ranks, a block per term
+//   three terms  rank <= 16: one block, 16 ranks of each; above: 32 ranks, a block with the first two and a block with the third
+struct HPack {
+    int width, blocks;
+    int pitch, ranks;  // elements of a row of h, and the ranks it has room for
+    __host__ __device__ HPack(int rank, int terms) {
+        width = terms == 3 ? (rank <= 16 ? 16 : 32) : (rank <= 32 ? 32 : 64);
+        blocks = rank <= (terms == 3 ? 16 : 32) ? 1 : 2;
+        const int n = (rank + width - 1) / width;
+        pitch = n * blocks * BK;
+        ranks = n * width;
+    }
+    // where term t of rank k stands in the row
+    __host__ __device__ int at(int k, int t) const { return k / width * blocks * BK + t * width + k % width; }
+};
 
 template <typename T>
 __device__ __forceinline__ float to_float(T x) { return float(x); }
@@ -165,13 +185,15 @@ __device__ __forceinline__ int find_runs(const HeadParams& p, const HeadTiles& t
     return __popc(starts);
 }
 
-// How the adapters' second product uses the ring: an entry is one run x up to 64 ranks; its rows of B take
+// How the adapters' second product uses the ring: an entry is one run x up to h.width ranks; its rows of B take
 // 128 x (32, 64 or 128) bytes, in the swizzle of that width, so that 8, 4 or 2 entries share a stage.
 struct AdapterPack {
+    HPack h;
+    int width;  // ranks per entry as B's boxes have them: 16 where that is all
     int a_bytes, max_entries;
     uint32_t layout, sbo;  // of the descriptor: swizzle type, distance of 8-row groups
-    __host__ __device__ explicit AdapterPack(int rank) {
-        const int width = rank <= 16 ? 16 : rank <= 32 ? 32 : 64;
+    __host__ __device__ AdapterPack(int rank, int terms) : h(rank, terms) {
+        width = rank <= 16 ? 16 : h.width;
         a_bytes = BM * width * 2;
         max_entries = HEAD_KSUB * A_BYTES / a_bytes;
         layout = width == 16 ? 6 : width == 32 ? 4 : 2;
@@ -186,7 +208,7 @@ struct AdapterPack {
         for (int k = 0; k < n_runs; ++k) {
             const Run run = runs[k];
             const int half = run.cols / 2;
-            for (int r0 = 0; r0 < rank; r0 += BK) {
+            for (int r0 = 0; r0 < rank; r0 += h.width) {
                 if (i > 0 && (i == max_entries || row + half > rows)) {
                     close();
                     i = row = 0;
@@ -410,7 +432,8 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
     tc_fence_after();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(s.tmem_base);
 
-    const AdapterPack pack(p.rank);
+    constexpr int TERMS = H_TERMS<BT>;
+    const AdapterPack pack(p.rank, TERMS);
     const bool ordered = p.col_token != nullptr;  // the columns come from the kernels before this one
     if (warp < HEAD_EPI_FIRST) {
         if constexpr (CHUNKS > HEAD_SPLIT_ABOVE) set_max_regs_down<HEAD_REGS_FEW>();
@@ -482,16 +505,16 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
                             const uint32_t bar = map_to_cta(smem_u32(&s.full[stage]), 0);
                             const uint32_t sa = smem_u32(s.stages) + stage * ring.bytes, sb = sa + ring.off_e;
                             const int half = run.cols / 2;  // rows of h that this CTA supplies: a multiple of 8
-                            const int terms = p.rank <= 32 ? 1 : 2;
+                            const int blocks = pack.h.blocks;
                             tma_load_3d_pair(sa + i * pack.a_bytes, &maps.b, bar, r0, row_c, run.adapter);
-                            for (int t = 0; t < terms; ++t)
+                            for (int t = 0; t < blocks; ++t)
                                 for (int y = 0; y < half;) {  // few and large loads: each costs its issue
                                     const bool large = half - y >= 32;
                                     tma_load_2d_pair(sb + t * ring.sub_e + (row + y) * BK * 2, large ? &maps.h32 : &maps.h8, bar,
-                                                     r0 * 2 + t * BK, col0 + run.first + rank * half + y);
+                                                     pack.h.at(r0, 0) + t * BK, col0 + run.first + rank * half + y);
                                     y += large ? 32 : 8;
                                 }
-                            bytes += pack.a_bytes + terms * half * BK * 2;
+                            bytes += pack.a_bytes + blocks * half * BK * 2;
                         },
                         [&]() {
                             announce(bytes);
@@ -576,15 +599,20 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
                             runs, n_runs, p.rank, ring.h_rows(), filled_stage,
                             [&](int i, int row, const Run& run, int r0) {
                                 const uint32_t run_idesc = p.idesc | (uint32_t(run.cols >> 3) << 17);
-                                const uint32_t lo = p.rank <= 32 ? 2 * STEP : ring.sub_e >> 4;  // from the hi to the lo terms
+                                // from the first term to the second and the third (two blocks are sub_e apart)
+                                const uint32_t half_row = pack.h.width / UMMA_K * STEP, block = ring.sub_e >> 4;
+                                const uint32_t term2 = TERMS == 2 && pack.h.blocks == 2 ? block : half_row;
+                                const uint32_t term3 = pack.h.blocks == 2 ? block : 2 * half_row;
                                 const uint32_t sa = smem_u32(s.stages) + stage * ring.bytes;
                                 const uint64_t rad = (make_smem_desc(sa + i * pack.a_bytes, 16, pack.sbo) & ~(uint64_t(7) << 61)) |
                                                      uint64_t(pack.layout) << 61;
                                 const uint64_t rbd = make_smem_desc(sa + ring.off_e + row * BK * 2, 16, 1024);
-                                const int steps = (min(BK, p.rank - r0) + UMMA_K - 1) / UMMA_K;
+                                const int steps = (min(pack.h.width, p.rank - r0) + UMMA_K - 1) / UMMA_K;
                                 for (int k = 0; k < steps; ++k) {
                                     tc_mma_f16_pair(d_tmem + run.first, rad + k * STEP, rbd + k * STEP, run_idesc, 1u);
-                                    tc_mma_f16_pair(d_tmem + run.first, rad + k * STEP, rbd + lo + k * STEP, run_idesc, 1u);
+                                    tc_mma_f16_pair(d_tmem + run.first, rad + k * STEP, rbd + term2 + k * STEP, run_idesc, 1u);
+                                    if constexpr (TERMS == 3)
+                                        tc_mma_f16_pair(d_tmem + run.first, rad + k * STEP, rbd + term3 + k * STEP, run_idesc, 1u);
                                 }
                             },
                             release_stage);
@@ -779,7 +807,7 @@ adapter_layout_kernel(const LayoutParams p) {
 }
 
 // h[column][j] = scale[a] * (A[a][j] . e_t), t and a the column's token and its adapter; zero without an adapter and
-// for the padding ranks; in fp32 and in the two 16-bit terms.  Without a column order the blocks of rank 0 also
+// for the padding ranks; in fp32 and in the 16-bit terms.  Without a column order the blocks of rank 0 also
 // write the groups' adapters; with one, the blocks of the last eight y gather the columns' rows of e, a column each.
 // One block per (8 consecutive columns, 4 ranks): its 8 warps split D, each lane reads 16 bytes of the
 // four rows of A and of every token of a run that shares an adapter, and the 32 sums are joined
@@ -803,7 +831,7 @@ struct ShrinkParams {
     int vec;  // 16-byte loads are possible for every row
     float* h;
     int ldh;
-    void* h16;          // [T][h16_pitch(rank)] in the 16-bit type of e, or null: every group is mixed
+    void* h16;          // [T][HPack::pitch] in the 16-bit type of e, or null: every group is mixed
     int* group;         // [ceil(T / 16)]
     int* group_bad;     // [ceil(T / 16)], zero before the launch
 };
@@ -818,6 +846,32 @@ __device__ __forceinline__ uint4 load_piece(const T* q, long long left, bool vec
     for (int i = 0; i < 16 / int(sizeof(T)); ++i) x[i] = i < left ? q[i] : T(0.0f);
     return u;
 }
+
+__device__ __forceinline__ __nv_bfloat16 cut_off(float x, __nv_bfloat16) { return __float2bfloat16_rz(x); }
+__device__ __forceinline__ __half cut_off(float x, __half) { return __float2half_rz(x); }
+__device__ __forceinline__ __nv_bfloat16 next_to_zero(__nv_bfloat16 x) { return __ushort_as_bfloat16(__bfloat16_as_ushort(x) - 1); }
+__device__ __forceinline__ __half next_to_zero(__half x) { return __ushort_as_half(__half_as_ushort(x) - 1); }
+
+// x as the sum of H_TERMS 16-bit numbers of its sign, none of them zero: an infinite entry of B then gives an infinity,
+// where terms of two signs would give inf - inf and a zero term inf x 0.  Every term but the last is what it has to
+// represent cut off, one step less where nothing would be left.  What is lost is half a step of the last term: 2^-22 of x in
+// fp16 with two terms, 2^-23 in bf16 with three (with two it would be 2^-16, and show in fp32 logits).
+template <typename T>
+struct SplitH {
+    T term[H_TERMS<T>];
+    __device__ __forceinline__ explicit SplitH(float x) {
+#pragma unroll
+        for (int t = 0; t < H_TERMS<T>; ++t) {
+            if (t == H_TERMS<T> - 1) {
+                term[t] = T(x);
+            } else {
+                term[t] = cut_off(x, T());
+                if (float(T(x - float(term[t]))) == 0.0f && float(term[t]) != 0.0f) term[t] = next_to_zero(term[t]);
+                x -= float(term[t]);
+            }
+        }
+    }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(SHRINK_WARPS * 32)
@@ -955,18 +1009,12 @@ adapter_shrink_kernel(const ShrinkParams p) {
                         p.group_bad[(tok0 + i) / HEAD_GROUP] = 1;
                         sum = 0.0f;
                     }
-                    T* row = reinterpret_cast<T*>(p.h16) + (size_t)(tok0 + i) * h16_pitch(p.rank);
-                    const T hi = T(sum), lo = T(sum - float(hi));
-                    if (p.rank <= 32) {
-                        if (k < 32) {
-                            row[k] = hi;
-                            row[32 + k] = lo;
-                        }
-                    } else {
-                        const int at = k / 64 * 128 + k % 64;
-                        row[at] = hi;
-                        row[at + 64] = lo;
-                    }
+                    const HPack pack(p.rank, H_TERMS<T>);
+                    T* row = reinterpret_cast<T*>(p.h16) + (size_t)(tok0 + i) * pack.pitch;
+                    const SplitH<T> h(sum);
+#pragma unroll
+                    for (int t = 0; t < H_TERMS<T>; ++t)
+                        if (k < pack.ranks) row[pack.at(k, t)] = h.term[t];
                 }
             }
         }

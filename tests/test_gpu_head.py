@@ -129,6 +129,36 @@ def test_logits_a_broken_adapter_stays_with_its_own_requests(bad):
     assert not torch.isfinite(got[~others]).any()
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("r", [8, 12, 16, 40, 64, 136])
+@pytest.mark.parametrize("layout", ["each", "runs"])
+def test_logits_infinite_entries_of_b_give_infinities(dtype, r, layout):
+    """One infinity in some rows of B, finite h: the definition's infinity, on the tensor cores (groups of one adapter)
+    and in the epilogue (rank 12, fp32) alike."""
+    T, V = 96, 400
+    kw = _inputs(T, V, 128, dtype, n=3, r=r, seed=r, layout=layout)
+    # whole numbers among the inner products, which leave nothing for a low term
+    kw["lora_a"][:, 0] = 0
+    kw["lora_a"][:, 0, 0] = 1
+    kw["lora_scale"] = torch.ones(3)
+    kw["e"][::2, 0] = torch.arange(1, T // 2 + 1).to(dtype)
+    g = torch.Generator().manual_seed(r)
+    rows = torch.randperm(V, generator=g)[:100]
+    where = torch.randint(0, r, (100,), generator=g)
+    where[:30] = 0
+    kw["lora_b"][1, rows, where] = math.inf * (1 - 2 * torch.randint(0, 2, (100,), generator=g)).to(dtype)
+    ref, mag = H.linear_logits(**kw)
+    assert not torch.isnan(ref).any() and torch.isinf(ref).any()
+    finite = torch.isfinite(ref)
+    for out in (dtype, FP32):
+        for t in (slice(None), slice(5, 6)):
+            got = linear_logits(**_to_dev(dict(kw, e=kw["e"][t], adapter_ids=kw["adapter_ids"][t])), out_dtype=out).cpu().double()
+            f = finite[t]
+            assert torch.equal(got[~f], ref[t][~f])
+            tol = _tolerance(ref[t], mag[t], dtype, out, 128 + r + 8, None)
+            assert bool(((got - ref[t]).abs() <= tol)[f].all())
+
+
 def test_logits_strides_and_shapes():
     kw = _inputs(24, 300, 128, BF16, n=2, r=16, bias=BF16)
     want = linear_logits(**_to_dev(kw), out_dtype=FP32)
