@@ -28,7 +28,7 @@ struct LogitsPlan {
     int pitch16;         // row length of the 16-bit h; 0: every group of columns is mixed
     int shrink_ranks;    // ranks that the shrink kernel writes: whole padding blocks of both forms of h
     long long ld_cols;
-    size_t off_bad, off_group, off_cols, off_ncol, off_e_cols, off_h, off_h16, total;
+    size_t off_bad, off_h_max, cleared, off_group, off_cols, off_ncol, off_e_cols, off_h, off_h16, total;
 };
 
 LogitsPlan plan_logits(const cce_b200_logits_args* a) {
@@ -55,6 +55,8 @@ LogitsPlan plan_logits(const cce_b200_logits_args* a) {
         return at;
     };
     pl.off_bad = take((size_t)pl.n_group * 4);
+    pl.off_h_max = take(mma && a->op.dtype == CCE_DT_F16 ? (size_t)pl.n_group * HEAD_GROUP * 4 : 0);
+    pl.cleared = off;
     pl.off_group = take((size_t)pl.n_group * 4);
     if (pl.sorted) {
         pl.off_cols = take((size_t)pl.n_col * 4);
@@ -296,13 +298,14 @@ int cce_b200_logits(const cce_b200_logits_args* a, void* workspace, size_t works
     if (rc) return rc;
     char* ws = reinterpret_cast<char*>(workspace);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    CCE_CUDA(cudaMemsetAsync(ws, 0, pl.off_bad + (size_t)pl.n_group * 4, st));
+    CCE_CUDA(cudaMemsetAsync(ws, 0, pl.cleared, st));
     Staged sg;
     rc = stage_operands(&op, pl.ops, ws, st, &sg, pl.sorted ? ws + pl.off_e_cols : nullptr);
     if (rc) return rc;
 
     const int elem = op.dtype == CCE_DT_F32 ? 4 : 2;
     auto aligned16 = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
+    unsigned* const h_max = pl.pitch16 && op.dtype == CCE_DT_F16 ? reinterpret_cast<unsigned*>(ws + pl.off_h_max) : nullptr;
     const int* col_token = pl.sorted ? reinterpret_cast<const int*>(ws + pl.off_cols) : nullptr;
     const int* n_col_dev = pl.sorted ? reinterpret_cast<const int*>(ws + pl.off_ncol) : nullptr;
     if (pl.sorted) {
@@ -343,6 +346,7 @@ int cce_b200_logits(const cce_b200_logits_args* a, void* workspace, size_t works
         sp.h16 = pl.pitch16 ? ws + pl.off_h16 : nullptr;
         sp.group = reinterpret_cast<int*>(ws + pl.off_group);
         sp.group_bad = reinterpret_cast<int*>(ws + pl.off_bad);
+        sp.h_max = h_max;
         if (op.dtype == CCE_DT_F32)
             rc = launch_shrink<float>(sp, pl.n_col, st);
         else if (op.dtype == CCE_DT_BF16)
@@ -386,6 +390,7 @@ int cce_b200_logits(const cce_b200_logits_args* a, void* workspace, size_t works
         hp.ldh = (int)pl.ldh;
         hp.group = reinterpret_cast<const int*>(ws + pl.off_group);
         hp.group_bad = reinterpret_cast<const int*>(ws + pl.off_bad);
+        hp.h_max = h_max;
     }
     HeadMaps maps;
     rc = make_tmap(&maps.c, sg.c, cdt, sg.Dk, op.V, sg.ldc, BK, BM);

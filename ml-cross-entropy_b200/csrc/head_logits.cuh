@@ -18,9 +18,9 @@
 // The adapters' second product.  The accumulator's columns are looked at in groups of 16.  A group whose tokens
 // all use one adapter (or none) takes it on the tensor cores, as further reduction blocks of the same columns: A
 // operand = the tile's rows of B, B operand = the group's h, split into 16-bit terms of one sign: two in fp16
-// (22 bits), three in bf16 (23).  A group of several adapters is added by the epilogue in fp32, every token with its own rows
+// (22 bits, down to 2^-25), three in bf16 (23).  A group of several adapters is added by the epilogue in fp32, every token with its own rows
 // of B: a masked tensor-core product would multiply one request's adapter by another's zeros, and an infinity
-// there would reach the wrong row.  The same holds for groups whose h does not fit the 16-bit type.
+// there would reach the wrong row.  The same is done for groups whose h does not fit the 16-bit type.
 // Unless the adapters are many (api_serving.cuh has the rule) adapter_layout_kernel orders the columns by
 // adapter, each adapter's run padded to whole groups, so that no group is mixed.
 //
@@ -86,6 +86,7 @@ struct HeadParams {
     int ldh;
     const int* group;    // [ceil(columns / 16)]: the adapter of a group, GROUP_NONE or GROUP_MIXED
     const int* group_bad;  // likewise; non-zero: h does not fit the 16-bit type, treat as mixed
+    const unsigned* h_max;  // null, or [16 ceil(columns / 16)]: the bits of the largest |h| of every column
 };
 
 constexpr int HEAD_E_MAPS = 4;
@@ -152,9 +153,23 @@ struct HPack {
 template <typename T>
 __device__ __forceinline__ float to_float(T x) { return float(x); }
 
+// fp16 ends at 2^-24, and so does what two terms keep of h: half a step, 2^-25, is lost of every value.  Columns whose
+// largest |h| lies below this (but is not 0) would lose more than 2^-17 of it; their groups take the fp32 path.
+constexpr float HEAD_H_MIN_FP16 = 0.00390625f;  // 2^-8
+
 __device__ __forceinline__ int group_adapter(const HeadParams& p, int g) {
     const int a = p.group[g];
-    return a >= 0 && p.group_bad[g] ? GROUP_MIXED : a;
+    if (a < 0) return a;
+    bool bad = p.group_bad[g] != 0;
+    if (p.h_max) {
+        const uint4* m = reinterpret_cast<const uint4*>(p.h_max + (size_t)g * HEAD_GROUP);
+#pragma unroll
+        for (int i = 0; i < HEAD_GROUP / 4; ++i) {
+            const uint4 w = m[i];
+            for (const unsigned x : {w.x, w.y, w.z, w.w}) bad |= x != 0 && x < __float_as_uint(HEAD_H_MIN_FP16);
+        }
+    }
+    return bad ? GROUP_MIXED : a;
 }
 
 // A run of neighbouring groups of a column tile that share an adapter.
@@ -834,6 +849,7 @@ struct ShrinkParams {
     void* h16;          // [T][HPack::pitch] in the 16-bit type of e, or null: every group is mixed
     int* group;         // [ceil(T / 16)]
     int* group_bad;     // [ceil(T / 16)], zero before the launch
+    unsigned* h_max;    // fp16: [16 ceil(T / 16)], zero before the launch; else null
 };
 
 // 16 bytes of a row, `left` of whose elements remain (zeros past them); vec: loaded at once
@@ -854,8 +870,8 @@ __device__ __forceinline__ __half next_to_zero(__half x) { return __ushort_as_ha
 
 // x as the sum of H_TERMS 16-bit numbers of its sign, none of them zero: an infinite entry of B then gives an infinity,
 // where terms of two signs would give inf - inf and a zero term inf x 0.  Every term but the last is what it has to
-// represent cut off, one step less where nothing would be left.  What is lost is half a step of the last term: 2^-22 of x in
-// fp16 with two terms, 2^-23 in bf16 with three (with two it would be 2^-16, and show in fp32 logits).
+// represent cut off, one step less where nothing would be left.  What is lost is half a step of the last term: 2^-22 of x, but
+// at least 2^-25, in fp16 with two terms, 2^-23 of x in bf16 with three (with two it would be 2^-16, and show in fp32 logits).
 template <typename T>
 struct SplitH {
     T term[H_TERMS<T>];
@@ -1004,11 +1020,15 @@ adapter_shrink_kernel(const ShrinkParams p) {
             if (k < p.ldh) p.h[(size_t)(tok0 + i) * p.ldh + k] = sum;
             if constexpr (sizeof(T) == 2) {
                 if (p.h16) {
-                    // |x| up to 2^15: above it, or not finite, and the group goes to the fp32 path
-                    if (!(fabsf(sum) <= 32768.0f)) {
+                    // |x| up to 2^15: above it, or not finite, and the group goes to the fp32 path; so it does for x too
+                    // small for terms that are not zero (2^-23 is two steps of fp16; bf16 reaches as far as fp32)
+                    const float x = fabsf(sum), least = H_TERMS<T> == 2 ? 0x1p-23f : 0x1p-100f;
+                    if (!(x <= 32768.0f) || (x < least && x > 0.0f)) {
                         p.group_bad[(tok0 + i) / HEAD_GROUP] = 1;
                         sum = 0.0f;
                     }
+                    // the order of the bits is the order of the numbers
+                    if (p.h_max && x > 0.0f && k < p.rank) atomicMax(&p.h_max[tok0 + i], __float_as_uint(x));
                     const HPack pack(p.rank, H_TERMS<T>);
                     T* row = reinterpret_cast<T*>(p.h16) + (size_t)(tok0 + i) * pack.pitch;
                     const SplitH<T> h(sum);

@@ -262,6 +262,33 @@ def test_logits_inner_products_beyond_the_16_bit_type():
     _check_logits(kw, out_dtype=FP32)
 
 
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("r", [8, 16, 48])
+@pytest.mark.parametrize("exponent", [-2, -7, -8, -9, -12, -16, -20, -24, -30])
+def test_logits_small_inner_products(dtype, r, exponent):
+    """Adapters alone (c = 0) whose inner products h come near the end of fp16, with large entries of B.  Of h is lost, beside
+    D + 2 roundings of its fp32 sum: 2^-22 or, in fp16, 2^-25 where the column's largest is 2^-8 or more; and of the second
+    product a step 2^-23 for each of its up to 3 r additions."""
+    T, V, D = 40, 300, 128
+    kw = _inputs(T, V, D, dtype, n=2, r=r, seed=r)
+    kw["c"].zero_()
+    kw["adapter_ids"] = torch.arange(T) // 20
+    kw["lora_b"] = (kw["lora_b"].float() * 1e4).clamp(-6e4, 6e4).to(dtype)
+    kw["lora_scale"] = torch.tensor([2.0**exponent, 2.0**exponent])
+    kw["lora_a"][0, 1] *= 2.0**-4  # a smaller one among the others
+    ref, _ = H.linear_logits(**kw)
+    A, B = (kw[k].double()[kw["adapter_ids"]] for k in ("lora_a", "lora_b"))
+    e, s = kw["e"].double(), 2.0**exponent
+    h = s * torch.einsum("td,trd->tr", e, A)
+    h_mag = s * torch.einsum("td,trd->tr", e.abs(), A.abs())
+    assert ref.abs().max() > 0
+    lost = torch.full_like(h, 0.0) if dtype == BF16 else torch.where(h.abs().amax(1, keepdim=True) >= 2.0**-8 * 0.99, 2.0**-25, 0.0) + 0 * h
+    h_err = (D + 2) * 2.0**-24 * h_mag + torch.maximum(2.0**-22 * h.abs(), lost)
+    tol = torch.einsum("tvr,tr->tv", B.abs(), h_err + 3 * r * 2.0**-23 * h.abs())
+    got = linear_logits(**_to_dev(kw), out_dtype=FP32).cpu().double()
+    assert bool(((got - ref).abs() <= tol * 1.01).all())
+
+
 def test_logits_output_past_two_to_the_31():
     """16384 x 140000 16-bit logits: offsets pass 2^31 elements."""
     kw = _to_dev(_inputs(16384, 140000, 64, BF16))
