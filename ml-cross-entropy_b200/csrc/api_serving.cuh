@@ -105,11 +105,6 @@ int launch_shrink(const ShrinkParams& sp, long long n_col, cudaStream_t st) {
     return launch_behind(adapter_shrink_kernel<T>, grid, SHRINK_WARPS * 32, 0, st, sp.col_token != nullptr, sp);
 }
 
-// Whether the accumulators are emptied by segments: fp32 logits of a long reduction
-inline bool head_segmented(const HeadParams& hp) {
-    return hp.out_dtype == CCE_DT_F32 && cdiv(hp.n_kblk, HEAD_KSUB) > HEAD_SEGMENT;
-}
-
 // What a form of the kernel needs before its first launch on a device.
 template <typename T, int CHUNKS>
 int setup_head() {
@@ -137,7 +132,7 @@ int launch_head_form(DeviceInfo* dev, int dtype, const HeadMaps& maps, const Hea
 
 template <typename T>
 int launch_head(DeviceInfo* dev, int dtype, const HeadMaps& maps, const HeadParams& hp, int grid, cudaStream_t st) {
-    if (!head_segmented(hp)) return launch_head_form<T, 0>(dev, dtype, maps, hp, grid, st);
+    if (hp.out_dtype != CCE_DT_F32) return launch_head_form<T, 0>(dev, dtype, maps, hp, grid, st);
     if (hp.n_tok <= 64) return launch_head_form<T, 1>(dev, dtype, maps, hp, grid, st);
     if (hp.n_tok <= 128) return launch_head_form<T, 2>(dev, dtype, maps, hp, grid, st);
     if (hp.n_tok <= 192) return launch_head_form<T, 3>(dev, dtype, maps, hp, grid, st);

@@ -380,7 +380,7 @@ __device__ __forceinline__ void finish_chunk(const HeadParams& p, const HeadTile
         for (int j = 0; j < 32; ++j)
             x[j] = FP32_OUT ? p.softcap * tanhf(x[j] * inv) : apply_softcap(x[j], p.softcap, inv);
     }
-    if (FP32_OUT || p.out_dtype == 2)
+    if (FP32_OUT)
         store_chunk<float>(p, v, my_token, x);
     else if (p.out_dtype == 1)
         store_chunk<__nv_bfloat16>(p, v, my_token, x);
@@ -396,8 +396,9 @@ struct HeadSmem {
     Run* runs;  // [2][HEAD_MAX_RUNS]: producer, MMA issuer
 };
 
-// BT: element type of the adapters (and of e).  CHUNKS > 0: the accumulator is emptied every HEAD_SEGMENT stages
-// into the epilogue's registers, CHUNKS chunks of 32 columns per warp (tiles of up to 64 CHUNKS columns); 0: it is not.
+// BT: element type of the adapters (and of e).  CHUNKS > 0: fp32 logits; the accumulator is emptied every HEAD_SEGMENT
+// stages into the epilogue's registers, CHUNKS chunks of 32 columns per warp (tiles of up to 64 CHUNKS columns).  0: 16-bit
+// logits, the sum in one piece.
 template <typename BT, int CHUNKS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HEAD_THREADS, 1)
 head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant__ HeadParams p) {

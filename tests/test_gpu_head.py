@@ -262,6 +262,21 @@ def test_logits_inner_products_beyond_the_16_bit_type():
     _check_logits(kw, out_dtype=FP32)
 
 
+@pytest.mark.parametrize("D", [64, 512, 520, 1024])
+@pytest.mark.parametrize("T", [5, 100, 150, 250])
+@pytest.mark.parametrize("softcap", [5.0, 30.0, 1000.0])
+def test_logits_softcap_of_fp32_logits(D, T, softcap):
+    """Small whole numbers, whose sums are exact: what is left is x / softcap (two roundings), tanh (2 steps of its
+    value) and the product with the cap (half a step), at any D."""
+    g = torch.Generator().manual_seed(D + T)
+    e, c = (torch.randint(-2, 3, (n, D), generator=g).to(BF16) for n in (T, 300))
+    x = e.double() @ c.double().T
+    want = softcap * torch.tanh(x / softcap)
+    got = linear_logits(e.to(DEV), c.to(DEV), softcap=softcap, out_dtype=FP32).cpu().double()
+    tol = 2.5 * 2.0**-23 * want.abs() + 2.0**-23 * x.abs() * (1 - (want / softcap) ** 2)
+    assert bool(((got - want).abs() <= tol * 1.01).all())
+
+
 @pytest.mark.parametrize("dtype", [FP16, BF16])
 @pytest.mark.parametrize("r", [8, 16, 48])
 @pytest.mark.parametrize("exponent", [-2, -7, -8, -9, -12, -16, -20, -24, -30])
