@@ -54,9 +54,11 @@ constexpr int GROUP_NONE = -1, GROUP_MIXED = -2;
 constexpr int HEAD_MAX_ACC = 8;
 constexpr int HEAD_FORMS = 5;  // of head_logits_kernel: CHUNKS 0 to 4
 // fp32 logits: the tensor core truncates every addition, so a sum over all of D drifts (2.4e-6 of the logits'
-// norm at D = 2304).  The accumulator is therefore emptied every HEAD_SEGMENT stages into fp32 registers,
-// which add with rounding (4.5e-7; twice as often: 2.7e-7, but 228 instead of 222 us for 144 columns).  16-bit logits are rounded far above the drift and take the sum in one piece.
-constexpr int HEAD_SEGMENT = 4;
+// norm at D = 2304).  The accumulator is therefore emptied every HEAD_SEGMENT stages (256 elements) into fp32 registers,
+// which add with rounding.  Against twice as long segments, 2304 and 4096 elements: error 2.4e-7 (4.5e-7 and 4.8e-7), time
+// 189 us (188) for 8 x 256000 x 2304, 305 (286) for 32 tokens of 8 adapters, whose 144 columns have two accumulators.
+// 16-bit logits are rounded far above the drift and take the sum in one piece.
+constexpr int HEAD_SEGMENT = 2;
 
 struct HeadParams {
     int T, V;          // tokens, classifier rows

@@ -277,6 +277,25 @@ def test_logits_softcap_of_fp32_logits(D, T, softcap):
     assert bool(((got - want).abs() <= tol * 1.01).all())
 
 
+@pytest.mark.parametrize("T", [5, 100, 150, 250])
+@pytest.mark.parametrize("D", [256, 520, 2048])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_logits_fp32_sums_do_not_drift(T, D, dtype):
+    """Whole numbers whose sums over 256 elements stay below 2^24, hence are exact on the tensor cores; the sums of these
+    round to the nearest: off by at most half a step for each, and by nothing on average."""
+    g = torch.Generator().manual_seed(T + D)
+    e, c = (torch.randint(200, 256, (n, D), generator=g).to(dtype) for n in (T, 2000))
+    parts = torch.stack([e[:, i : i + 256].double() @ c[:, i : i + 256].double().T for i in range(0, D, 256)])
+    assert parts.max() < 2**24
+    run = parts.cumsum(0)
+    half_steps = torch.exp2(run[1:].log2().floor() - 24)  # of the results of the additions
+    err = linear_logits(e.to(DEV), c.to(DEV), out_dtype=FP32).cpu().double() - run[-1]
+    assert bool((err.abs() <= 1.01 * half_steps.sum(0)).all())
+    # the mean of N errors bounded by b and as often up as down: 6 b / sqrt(N)
+    bound = float(half_steps.sum(0).max()) if len(half_steps) else 0.0
+    assert abs(float(err.mean())) <= 6 * bound / err.numel() ** 0.5
+
+
 @pytest.mark.parametrize("dtype", [FP16, BF16])
 @pytest.mark.parametrize("r", [8, 16, 48])
 @pytest.mark.parametrize("exponent", [-2, -7, -8, -9, -12, -16, -20, -24, -30])
