@@ -277,6 +277,44 @@ def test_logits_softcap_of_fp32_logits(D, T, softcap):
     assert bool(((got - want).abs() <= tol * 1.01).all())
 
 
+# Column widths of 16 to 256 (with an order of the adapters: up to 15 more per run), and several column tiles
+WIDTHS = [10, 64, 80, 128, 144, 190, 208, 256, 300, 700]
+
+
+@pytest.mark.parametrize("T", WIDTHS)
+@pytest.mark.parametrize("D", [520, 1001, 1024])
+@pytest.mark.parametrize("adapters", ["none", "ordered", "runs", "many", "odd_rank"])
+def test_logits_fp32_of_long_reductions(T, D, adapters):
+    """fp32 logits whose sums are handed over several times, with each form of the adapters' product."""
+    n, r, layout = {"none": (0, 0, "each"), "ordered": (3, 24, "each"), "runs": (3, 40, "runs"),
+                    "many": (200, 16, "each"), "odd_rank": (4, 12, "each")}[adapters]  # fmt: skip
+    kw = _inputs(T, 700, D, FP16 if T == 128 else BF16, n=n, r=r, layout=layout, bias=FP32, seed=T + D)
+    _check_logits(kw, out_dtype=FP32, softcap=20.0 if T % 3 else None)
+
+
+@pytest.mark.parametrize("T", [9, 100, 150, 250])
+@pytest.mark.parametrize("adapters", [0, 3])
+def test_logits_fp32_of_more_tiles_than_cta_pairs(T, adapters):
+    """19700 rows: 77 tiles for at most 74 pairs, 2304 reduction elements."""
+    _check_logits(_inputs(T, 19_700, 2304, BF16, n=adapters, r=16, bias=BF16, seed=T), out_dtype=FP32, softcap=30.0)
+
+
+@pytest.mark.parametrize("T", WIDTHS)
+@pytest.mark.parametrize("D", [176, 520])
+def test_logits_fp32_operands_of_long_reductions(T, D):
+    """The three-term split makes 3 D of them."""
+    _check_logits(_inputs(T, 600, D, FP32, n=2 if T % 2 else 0, r=8, bias=FP32, seed=T))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_logits_of_long_reductions_do_not_depend_on_the_batch_mates(dtype):
+    kw = _to_dev(_inputs(700, 500, 1000, dtype))
+    full = linear_logits(**kw, out_dtype=FP32)
+    for n in WIDTHS:
+        assert torch.equal(linear_logits(**dict(kw, e=kw["e"][:n]), out_dtype=FP32), full[:n]), n
+        assert torch.equal(linear_logits(**dict(kw, e=kw["e"][700 - n :]), out_dtype=FP32), full[700 - n :]), n
+
+
 @pytest.mark.parametrize("T", [5, 100, 150, 250])
 @pytest.mark.parametrize("D", [256, 520, 2048])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
