@@ -52,6 +52,7 @@ constexpr int HEAD_GROUP = 16;                 // tokens that share one decision
 constexpr int ADAPTER_RANK_PAD = 16;           // fp32 rows of h are padded to this many ranks with zeros
 constexpr int GROUP_NONE = -1, GROUP_MIXED = -2;
 constexpr int HEAD_MAX_ACC = 8;
+constexpr long long HEAD_DRAIN_CYCLES = 20000000;  // 10 ms, many times what a load takes
 constexpr int HEAD_FORMS = 5;  // of head_logits_kernel: CHUNKS 0 to 4
 // fp32 logits: the tensor core truncates every addition, so a sum over all of D drifts (2.4e-6 of the logits'
 // norm at D = 2304).  The accumulator is therefore emptied every HEAD_SEGMENT stages (256 elements) into fp32 registers,
@@ -395,6 +396,7 @@ struct HeadSmem {
     uint64_t *full, *empty, *tfull, *tempty, *tdown;
     uint32_t* tmem_base;
     volatile int* abort_flag;
+    int* ring_end;  // where the producer's use of the ring ended: stage, phase, number of stages
     Run* runs;  // [2][HEAD_MAX_RUNS]: producer, MMA issuer
 };
 
@@ -416,6 +418,7 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
     s.tdown = s.tempty + HEAD_MAX_ACC;
     s.tmem_base = reinterpret_cast<uint32_t*>(s.tdown + 1);
     s.abort_flag = reinterpret_cast<int*>(s.tmem_base + 1);
+    s.ring_end = reinterpret_cast<int*>(s.tmem_base + 2);
     s.runs = reinterpret_cast<Run*>(base + HEAD_RING_BYTES + 512);
 
     constexpr bool SEGMENTED = CHUNKS > 0;
@@ -539,6 +542,11 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
                             next_stage();
                         });
                 }
+            }
+            if (elect_one()) {
+                s.ring_end[0] = stage;
+                s.ring_end[1] = int(phase);
+                s.ring_end[2] = ring.n_stage;
             }
         } else if (warp == 1) {
             if (rank == 0) {
@@ -725,17 +733,25 @@ head_logits_kernel(const __grid_constant__ HeadMaps maps, const __grid_constant_
         }
     }
 
-    // tear-down: the leader waits (bounded) for its MMAs; neither CTA leaves, or frees TMEM, while
-    // the other may still read its shared memory or signal its barriers
+    // tear-down: the leader waits (bounded, whether or not a wait was abandoned before) for its MMAs, and after an abandoned
+    // wait for the loads of both CTAs that it announced; neither CTA leaves, or frees TMEM, while the other may still read
+    // its shared memory or signal its barriers
     tc_fence_before();
     __syncthreads();
-    if (warp == 1 && rank == 0) {
-        if (lane == 0) {
+    if (rank == 0) {
+        int unset = 0;
+        if (warp == 1 && elect_one()) {  // the lane that issued them: a commit covers its own thread's MMAs
             tc_commit_pair(smem_u32(s.tdown));
-            mbar_wait(smem_u32(s.tdown), 0, s.abort_flag, p.status, ERR_WAIT_TEARDOWN);
+            mbar_wait(smem_u32(s.tdown), 0, &unset, p.status, ERR_WAIT_TEARDOWN);
         }
-        __syncwarp();
+        if (warp == 0 && *s.abort_flag && elect_one()) {
+            const int stage = s.ring_end[0], phase = s.ring_end[1], n_stage = s.ring_end[2];
+            for (int i = 0; i < n_stage && !unset; ++i)  // stages from `stage` on were last filled a round earlier, if ever
+                mbar_wait(smem_u32(&s.full[i]), uint32_t(i < stage ? phase : phase ^ 1), &unset, p.status, ERR_WAIT_TEARDOWN,
+                          HEAD_DRAIN_CYCLES);
+        }
     }
+    __syncwarp();
     cluster_arrive();
     cluster_wait();
     if (warp == 1) {
