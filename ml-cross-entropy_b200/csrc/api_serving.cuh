@@ -195,7 +195,12 @@ int plan_sample(const cce_b200_sample_args* a, SamplePlan* out) {
     // From 32 MB of logits on the streaming kernels win: fp32, no filters / top-p / top-k and top-p, 64 x 128000: 41 / 84 /
     // 55 us against one cluster per row's 41 / 109 / 55, 128 x 256000: 92 / 182 / 121 against 133 / 334 / 162; bf16,
     // 64 x 128000: 37 / 80 / 53 against 31 / 72 / 39, 128 x 128000: 51 / 109 / 72 against 51 / 127 / 64.
-    pl.stream = a->B * a->V * elem >= (32LL << 20);
+    // But only with long rows: while a row's logits leave room for a second CTA on the SM the clusters win.  64 MB,
+    // streaming against clusters: fp32, rows of 15000: 67 / 182 / 121 against 60 / 157 / 95, 16000: 66 / 176 / 118 against
+    // 85 / 200 / 120; bf16, 31000: 91 / 230 / 146 against 79 / 204 / 114, 33000: 95 / 242 / 157 against 104 / 283 / 167.
+    // (Their workspace, 24 KB for a row with a filter, would be many times the logits of short rows.)
+    const long long row_bytes = a->V * elem;
+    pl.stream = row_bytes >= (62LL << 10) && a->B * row_bytes >= (32LL << 20);
     pl.total = 256;
     if (pl.stream) {
         pl.n_chunk = (int)cdiv(a->V + 16 / elem - 1, STR_CHUNK);

@@ -607,6 +607,25 @@ def test_sample_many_long_greedy_rows_without_filters(dtype, B, min_p):
     assert torch.equal(mixed[some].cpu(), warm)
 
 
+@pytest.mark.parametrize("dtype, B, V", [(FP32, 300_000, 33), (BF16, 3000, 9000), (FP32, 560, 15_900), (FP16, 520, 32_500)])
+@pytest.mark.parametrize("name", ["plain", "greedy", "p", "all"])
+def test_sample_many_short_rows(dtype, B, V, name):
+    """As many bytes as the streaming kernels begin with, in rows too short for them, or just long enough."""
+    kw = SETTINGS[name]
+    x, u = _rows(B, V, dtype, seed=V)
+    assert x.numel() * x.element_size() >= 32 << 20
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    tok = sample_tokens(x, u, **kw)
+    assert torch.cuda.max_memory_allocated() - before <= 0.6 * x.numel() * x.element_size() + 16 * B + 4096
+    for lo in range(0, B, max(1, B // 5)):  # parts of the batch, too small for them
+        part = slice(lo, lo + (8 << 20) // (V * x.element_size()))
+        assert torch.equal(sample_tokens(x[part], u[part], **kw), tok[part])
+    rows = list(range(0, B, B // 12))
+    want, _ = H.sample_tokens(x[rows].cpu(), u[rows].cpu(), **kw)
+    assert torch.equal(tok[rows].cpu(), want)
+
+
 def test_linear_sample_of_a_large_greedy_batch():
     """The float32 logits of 70 x 120011 go through the streaming kernels."""
     kw = _to_dev(_inputs(70, 120_011, 64, BF16))

@@ -245,6 +245,18 @@ def test_c_entry_points_check_their_arguments():
     assert L.cce_b200_sample(sample_args(B=0, logits=None), None, 0, None) == 0
 
 
+@pytest.mark.parametrize("dtype, elem", [(_native.DT_F32, 4), (_native.DT_BF16, 2), (_native.DT_F16, 2)])
+@pytest.mark.parametrize("B, V", [(10**6, 32), (10**7, 5), (2100, 4000), (600, 15_000), (600, 33_000), (200, 60_000), (64, 256_000), (512, 152_064), (1, 700_000)])  # fmt: skip
+@pytest.mark.parametrize("filters", [dict(), dict(top_k_all=5), dict(top_p_all=0.5)])
+def test_sampling_workspace_stays_below_the_logits(dtype, elem, B, V, filters):
+    a = _native.SampleArgs()
+    a.B, a.V, a.ld, a.dtype, a.top_p_all = B, V, V, dtype, 1.0
+    for k, v in filters.items():
+        setattr(a, k, v)
+    got = _native.lib().cce_b200_sample_workspace_bytes(a)
+    assert 0 < got <= B * V * elem // 2 + 256
+
+
 def test_the_loss_does_not_depend_on_the_serving_kernels():
     """What every entry point asks of the device names none of them: they are set up at their own first launch."""
     from pathlib import Path
