@@ -626,6 +626,25 @@ def test_sample_many_short_rows(dtype, B, V, name):
     assert torch.equal(tok[rows].cpu(), want)
 
 
+@pytest.mark.parametrize("name", ["plain", "greedy", "p", "all"])
+def test_sample_offsets_past_two_to_the_31(name):
+    """Rows more than 2^31 elements apart, and a batch of more than 2^31 logits (the streaming kernels)."""
+    kw = SETTINGS[name]
+    x, u = _rows(3, 20_000, BF16, seed=51)
+    apart = 2**31 + 24
+    far = torch.empty(apart + 40_000, dtype=BF16, device=DEV).as_strided((2, 20_000), (apart, 1))
+    far.copy_(x[:2])
+    assert torch.equal(sample_tokens(far, u[:2], **kw), sample_tokens(x[:2], u[:2], **kw))
+    del far
+    B, V = 16_400, 131_000
+    few, _ = _rows(40, V, BF16, seed=52)
+    big = few.repeat(B // 40, 1)
+    u = torch.rand(B, generator=torch.Generator().manual_seed(53)).to(DEV)
+    tok = sample_tokens(big, u, **kw)
+    for rows in (slice(0, 3), slice(8000, 8003), slice(16_390, 16_400)):
+        assert torch.equal(sample_tokens(few[torch.arange(B, device=DEV)[rows] % 40], u[rows], **kw), tok[rows])
+
+
 def test_linear_sample_of_a_large_greedy_batch():
     """The float32 logits of 70 x 120011 go through the streaming kernels."""
     kw = _to_dev(_inputs(70, 120_011, 64, BF16))
