@@ -53,7 +53,8 @@ enum {
     CCE_ERR_KERNEL_WAIT = -6, /* status word non-zero: a kernel abandoned a bounded wait */
     CCE_ERR_TOO_LARGE = -7,   /* problem needs more scratch than the entry point has: the fixed buffer of
                                  cce_b200_lse_forward_static, the shared memory of cce_b200_sample */
-    CCE_ERR_UNSUPPORTED = -8  /* feature not compiled into this build (wait tracing needs -DCCE_TRACE=1) */
+    CCE_ERR_UNSUPPORTED = -8  /* feature not compiled into this build (wait tracing needs -DCCE_TRACE=1; wide fp32 tiles of
+                                 cce_b200_logits need kernels with exactly the registers that they hand out) */
 };
 
 /* Shape and operand description shared by the three entry points.

@@ -24,9 +24,9 @@
 // Unless the adapters are many (api_serving.cuh has the rule) adapter_layout_kernel orders the columns by
 // adapter, each adapter's run padded to whole groups, so that no group is mixed.
 //
-// Measured (bf16, device time, 152064 x 3584): 1 token 180 us (6.05 TB/s; cuBLAS 188), 64 tokens 191 (197), 256 tokens 238
-// (254), 2048 tokens 1430 (1430); with 4 adapters of rank 16 182, 210, 311, 1650; fp32 logits 178, 191, 254, 1530.  Up to
-// 128 columns HBM bounds it; then the loads from L2 (256 tokens: 2.1 GB of tiles, 9 TB/s), at 2048 the tensor pipe.
+// Measured (bf16, 152064 x 3584, one box; others and other moments differ by 10 % from 256 tokens on): 1 token 170 us
+// (6.4 TB/s; cuBLAS 177), 64 tokens 181 (188), 256 tokens 247 (287), 2048 tokens 1560 (1740); with 4 adapters of rank 16
+// 174, 202, 325, 1940; fp32 logits 171, 184, 290, 1900.  Up to 128 columns HBM bounds it; then the loads from L2 (256 tokens: 2.1 GB of tiles, 9 TB/s), at 2048 the tensor pipe.
 // One lane issues: an MMA of 144 columns then follows the last one after 78 cycles, which is what the tensor pipe takes, a
 // TMA load after 120.  Few and large loads for that reason: the token loads have four sizes, the runs of h two.
 #pragma once
@@ -57,7 +57,8 @@ constexpr int HEAD_FORMS = 5;  // of head_logits_kernel: CHUNKS 0 to 4
 // fp32 logits: the tensor core truncates every addition, so a sum over all of D drifts (2.4e-6 of the logits'
 // norm at D = 2304).  The accumulator is therefore emptied every HEAD_SEGMENT stages (256 elements) into fp32 registers,
 // which add with rounding.  Against twice as long segments, 2304 and 4096 elements: error 2.4e-7 (4.5e-7 and 4.8e-7), time
-// 189 us (188) for 8 x 256000 x 2304, 305 (286) for 32 tokens of 8 adapters, whose 144 columns have two accumulators.
+// 189 us (188) for 8 x 256000 x 2304, 305 (286) for 32 tokens of 8 adapters, whose 144 columns have two accumulators,
+// 262 to 274 (257 to 260) for 256 x 128256 x 4096.
 // 16-bit logits are rounded far above the drift and take the sum in one piece.
 constexpr int HEAD_SEGMENT = 2;
 

@@ -21,9 +21,10 @@
 //    summed exactly (by blocks, which the draw needs anyway), and the border is found, exactly, in the list.
 //  - Otherwise (a large k, thousands of equal logits, an estimate that was off): further histograms narrow the
 //    border down over the integer keys of its bin until it is a single value.
-// A cluster barrier costs 0.5 to 0.8 us, a pass over a slice of 16384 logits 1 to 3 us: the latency of a row is its
-// five to seven barriers (1 x 256000 fp32, all filters: 22 us on the device, 64 x 128256 bf16, top-k and top-p: 36 us),
-// its throughput the fp64 weights (0.4 cycles per logit and SM) and the atomics (0.3).
+// A cluster barrier costs 0.5 to 0.8 us, a pass over a slice of 16384 logits 1 to 3 us: five to seven barriers are 3 to 5
+// of the 17 us that 1 x 256000 fp32 with all filters takes on the device (64 x 128256 bf16, top-k and top-p: 34 us); how
+// the rest divides among the passes has not been measured.  Throughput is the fp64 weights (0.4 cycles per logit and SM) and
+// the atomics (0.3).
 #pragma once
 #include <cooperative_groups.h>
 #include "engine.cuh"

@@ -3,9 +3,10 @@
 // In sample.cuh a row's passes are separated by cluster barriers, and an SM holds two CTAs at most: 512 rows x 152064
 // fp32 logits took 640 us with top-p, 256 x 256000 without filters 268 us, mostly waiting.  Here every pass is a
 // kernel with full occupancy that streams the logits from HBM (or L2), so that a pass costs what its bytes or its fp64
-// weights cost (0.4 cycles per logit and SM), and what a barrier did is the end of a kernel: 360 and 141 us.  Of the 360:
+// weights cost (0.4 cycles per logit and SM), and what a barrier did is the end of a kernel: 366 and 141 us.  Of the 366:
 // maximum 47 (6.6 TB/s), counts and sum 149, plan 14, pass 116, draw 40; of the 141: maximum 38, weights 95, draw 8.
-// Below some tens of megabytes the launches cost more than the barriers (api_serving.cuh has the rule).
+// Below some tens of megabytes the launches cost more than the barriers, and rows that two CTAs of an SM can hold are
+// faster there (api_serving.cuh has the rule).
 //
 //   row_max_kernel     the largest logit of every chunk
 //   row_prepare_kernel per row (a warp): its maximum and thresholds, and whether there is anything to do (RowMode)

@@ -81,7 +81,7 @@ def linear_logits(
     Arguments are plain tensors or parameters: DTensors and other wrappers without memory of their own are refused.
 
     :param e: embeddings ``(..., D)``: bf16, fp16, or fp32 (computed as a three-term bf16 split:
-        about 16 mantissa bits).
+        about 16 mantissa bits; infinite entries of ``e`` or ``c`` give NaN).
     :param c: classifier ``(V, D)`` of the same dtype.
     :param bias: optional ``(V,)``, bf16, fp16 or fp32.
     :param softcap: if set, logits become ``softcap * tanh(logits / softcap)``.
