@@ -736,6 +736,66 @@ def test_decoding_steps_captured_and_replayed():
             assert torch.equal(a, b)
 
 
+FIRST_LAUNCH = """
+import torch
+from cut_cross_entropy import linear_logits, linear_sample, sample_tokens
+
+g = torch.Generator().manual_seed(0)
+r = lambda *shape: torch.randn(*shape, generator=g).to("cuda", torch.bfloat16)
+e, c, a, b, u = r(250, 640), r(900, 640), r(2, 16, 640), r(2, 900, 16), torch.rand(250, generator=g).cuda()
+ids = torch.arange(250, device="cuda") % 3 - 1
+step = lambda: (linear_logits(e, c, lora_a=a, lora_b=b, adapter_ids=ids, out_dtype=torch.float32),
+                linear_logits(e[:20], c), linear_sample(e[:70], c, u[:70], top_p=0.9), sample_tokens(r2, u[:70]))
+r2 = r(70, 240_000)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+for x, y in zip(got, step()):
+    assert torch.equal(x, y)
+print("captured")
+"""
+
+
+def test_first_launch_of_every_form_inside_a_capture():
+    """A process whose first calls are captured: the kernels are loaded and set up there."""
+    import os
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    root = Path(__file__).resolve().parent.parent
+    env = dict(os.environ, PYTHONPATH=str(root / "ml-cross-entropy_b200"))
+    out = subprocess.run([sys.executable, "-c", FIRST_LAUNCH], cwd=root, env=env, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "captured" in out.stdout, out.stderr[-2000:]
+
+
+def test_forms_first_launched_by_two_threads_at_once():
+    """Two threads on their own streams, with shapes that take different forms of the kernels."""
+    import threading
+
+    kw = _to_dev(_inputs(250, 900, 640, FP16, n=2, r=16))
+    x, u = _rows(40, 9000, FP16)
+    jobs = [lambda: linear_logits(**kw, out_dtype=FP32), lambda: sample_tokens(x, u, top_p=0.8),
+            lambda: linear_logits(kw["e"][:100], kw["c"], out_dtype=FP32), lambda: linear_logits(**kw)]  # fmt: skip
+    got: dict = {}
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[i] = [jobs[i]() for _ in range(20)]
+            torch.cuda.current_stream().synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(jobs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i, job in enumerate(jobs):
+        want = job()
+        assert len(got[i]) == 20 and all(torch.equal(y, want) for y in got[i])
+
+
 def test_training_and_answering_share_the_head():
     """The loss's own numbers from the logits: lse and the correct-token logit agree with linear_cross_entropy."""
     from cut_cross_entropy import linear_cross_entropy
